@@ -1,0 +1,898 @@
+// Paged KV cache held in 8 bits (sm_100a): appending rotated keys and values, and attention over the cache.
+//
+// Cache of one layer: codes [num_blocks][2 (K, V)][kv_heads][16 tokens][128] E4M3, scales [num_blocks][kv_heads][2]
+// float32. A value is code * scale; one scale serves the 16 tokens of a page for one kv head and K or V.
+//
+// append (`kv8_append_kernel`). k' = R(pos) n(k), v' = v in fp32 (n: optional RMSNorm with a weight, R: the rotation of
+// the first `rotary` dims), one rounding to E4M3. The tokens of a call that follow one another in a page are its run;
+// the page's tokens before the run are kept, those behind it are dead. The page's scale becomes
+//     s' = max(s of the kept tokens, the least power of two with amax(run) <= 448 s', 2^-60)
+// and kept codes move to it: code' = rne(code * s / s'). s / s' is a power of two, so a kept value changes only where
+// it falls below E4M3's normal range. Powers of two make code * scale exact in bf16 and in fp32.
+// A value that is not finite is stored as NaN and does not raise the scale.
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace sdc {
+namespace kv8 {
+
+constexpr int D = 128;
+constexpr int PAGE = 16;
+// Biases of the decode kernel's weights and row sums (powers of two), see there.
+constexpr float SUM_BIAS = 30.f;
+constexpr float W_SCALE = 1.f / 65536.f;    // 2^(14 - SUM_BIAS)
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, m));
+  return v;
+}
+// E4M3 pair (low 8 bits = lo) of two floats, round to nearest even; |x| <= 448 or NaN.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Two E4M3 codes (low 16 bits) -> two halves, exact.
+__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_h2_hi(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ float2 h2_to_f2(uint32_t h) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+// The least power of two s >= 2^-60 with amax <= 448 s: 448 = 1.75 * 2^8, so from amax's exponent and fraction.
+__device__ __forceinline__ float scale_of(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  int e = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = e < -60 ? -60 : e;
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+
+struct AppendParams {
+  const __nv_bfloat16* qkv;   // [T] rows of (nq + 2 nkv) x 128, `ld` apart
+  long long ld;
+  int T, nq, nkv;
+  const int* pos;             // [T]
+  const long long* slots;     // [T] block * 16 + place; negative: not stored
+  const __nv_bfloat16* qw;
+  const __nv_bfloat16* kw;
+  float eps;
+  const float2* cs;           // [table_rows][rotary / 2] (cos, sin)
+  int table_rows, rotary, interleaved;
+  __nv_bfloat16* q_out;       // [T][nq][128]
+  uint8_t* codes;
+  float* scales;
+  long long capacity;         // num_blocks * 16
+  const int* rows;            // check mode: the sampled tokens
+  int nrows;
+  unsigned long long* check;
+};
+
+// The slot token t is stored at; -1: skipped; -2: its slot or position lies outside the cache or the table.
+__device__ __forceinline__ long long slot_of(const AppendParams& p, int t) {
+  const long long s = p.slots[t];
+  if (s >= p.capacity) return -2;
+  if (p.rotary > 0) {
+    const int ps = p.pos[t];
+    if (ps < 0 || ps >= p.table_rows) return -2;
+  }
+  return s < 0 ? -1 : s;
+}
+
+// Lane l owns dims 4l .. 4l + 3 of the head. Norm (when w is given) and rotation, in fp32.
+__device__ __forceinline__ void norm_rotate(const AppendParams& p, float (&v)[4], const __nv_bfloat16* w, bool rotate,
+                                            int t, int lane) {
+  if (w != nullptr) {
+    const float ss = warp_sum(fmaf(v[0], v[0], fmaf(v[1], v[1], fmaf(v[2], v[2], v[3] * v[3]))));
+    const float inv = rsqrtf(ss / static_cast<float>(D) + p.eps);
+    const uint2 u = *reinterpret_cast<const uint2*>(w + 4 * lane);
+    const float2 w0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+    const float2 w1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+    v[0] *= inv * w0.x;
+    v[1] *= inv * w0.y;
+    v[2] *= inv * w1.x;
+    v[3] *= inv * w1.y;
+  }
+  if (!rotate || p.rotary == 0) return;
+  const int half = p.rotary / 2;
+  const float2* cs = p.cs + static_cast<long long>(p.pos[t]) * half;
+  if (p.interleaved) {
+    if (4 * lane < p.rotary) {
+      const float4 c = *reinterpret_cast<const float4*>(cs + 2 * lane);     // pairs (4l, 4l + 1), (4l + 2, 4l + 3)
+      const float a0 = v[0], b0 = v[1], a1 = v[2], b1 = v[3];
+      v[0] = a0 * c.x - b0 * c.y;
+      v[1] = b0 * c.x + a0 * c.y;
+      v[2] = a1 * c.z - b1 * c.w;
+      v[3] = b1 * c.z + a1 * c.w;
+    }
+    return;
+  }
+  // halves: dim i pairs with i + half; half is a multiple of 4, so the partner dims are another lane's four
+  const bool low = 4 * lane < half, in = 4 * lane < p.rotary;
+  const int other = in ? (low ? lane + half / 4 : lane - half / 4) : lane;
+  float o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = __shfl_sync(0xffffffffu, v[i], other);
+  if (in) {
+    const float4* c = reinterpret_cast<const float4*>(cs + (low ? 4 * lane : 4 * lane - half));
+    const float4 c0 = c[0], c1 = c[1];
+    const float co[4] = {c0.x, c0.z, c1.x, c1.z}, si[4] = {c0.y, c0.w, c1.y, c1.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = low ? v[i] * co[i] - o[i] * si[i] : v[i] * co[i] + o[i] * si[i];
+  }
+}
+
+__device__ __forceinline__ void unpack4(const uint2& u, float (&v)[4]) {
+  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
+  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+  v[0] = a.x;
+  v[1] = a.y;
+  v[2] = b.x;
+  v[3] = b.y;
+}
+
+__device__ __forceinline__ float amax_of(const float (&v)[4], float m) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (finite(v[i])) m = fmaxf(m, fabsf(v[i]));
+  return m;
+}
+// The four codes of a lane at scale 1 / inv.
+__device__ __forceinline__ uint32_t codes_of(const float (&v)[4], float inv) {
+  float s[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] = finite(v[i]) ? v[i] * inv : __int_as_float(0x7fffffff);
+  return e4m3x2(s[0], s[1]) | (e4m3x2(s[2], s[3]) << 16);
+}
+
+// One warp per (group of TG consecutive tokens, head); heads [0, nq) queries, then nkv keys, then nkv values. A query
+// warp handles its group's tokens; a key or value warp handles the runs that begin in its group, so one warp alone
+// writes a page's scale and codes. TG = 1 gives a decode step a warp for every row (latency), TG = 16 gives a prefill
+// one warp for a page (16 rows in flight, no warps that find nothing to do).
+template <int TG>
+__global__ void __launch_bounds__(256) kv8_append_kernel(const AppendParams p) {
+  const int lane = threadIdx.x & 31, h = blockIdx.y * 8 + (threadIdx.x >> 5);
+  if (h >= p.nq + 2 * p.nkv) return;
+  const int t0 = blockIdx.x * TG;
+  const __nv_bfloat16* col = p.qkv + static_cast<long long>(h) * D + 4 * lane;
+  if (h < p.nq) {
+    uint2 raw[TG];
+#pragma unroll
+    for (int j = 0; j < TG; ++j)
+      raw[j] = t0 + j < p.T ? *reinterpret_cast<const uint2*>(col + (t0 + j) * p.ld) : make_uint2(0, 0);
+#pragma unroll
+    for (int j = 0; j < TG; ++j) {
+      const int t = t0 + j;
+      if (t >= p.T) return;
+      float v[4];
+      unpack4(raw[j], v);
+      uint2 o = make_uint2(0x7fff7fffu, 0x7fff7fffu);     // NaN: a slot or position outside must not pass unseen
+      if (slot_of(p, t) != -2) {
+        norm_rotate(p, v, p.qw, true, t, lane);
+        o = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+      }
+      *reinterpret_cast<uint2*>(p.q_out + (static_cast<long long>(t) * p.nq + h) * D + 4 * lane) = o;
+    }
+    return;
+  }
+  const bool is_k = h < p.nq + p.nkv;
+  const int kvh = is_k ? h - p.nq : h - p.nq - p.nkv;
+  // lane j looks at token t0 - 1 + j: the token before the group, the group, and the tokens a run may reach behind it
+  const int tl = t0 - 1 + lane;
+  const long long sl = lane <= TG + PAGE - 1 && tl >= 0 && tl < p.T ? slot_of(p, tl) : -1;
+  const long long before = __shfl_up_sync(0xffffffffu, sl, 1);
+  const bool follows = lane > 0 && sl >= 0 && before >= 0 && sl == before + 1 && sl % PAGE != 0;
+  const uint32_t chain = __ballot_sync(0xffffffffu, follows);
+  uint32_t starts = __ballot_sync(0xffffffffu, sl >= 0 && !follows && lane >= 1 && lane <= TG);
+  while (starts != 0) {
+    const int first = __ffs(starts) - 1;
+    starts &= starts - 1;
+    const uint32_t rest = ~(chain >> 1 >> first);          // bit i: token first + 1 + i does not continue the run
+    const int len = 1 + (rest == 0 ? 31 : __ffs(rest) - 1);   // <= 16: a run stays in its page
+    const long long slot = __shfl_sync(0xffffffffu, sl, first);
+    const int t = t0 - 1 + first;
+    const long long blk = slot / PAGE;
+    const int at = static_cast<int>(slot % PAGE);
+    constexpr int ROWS = PAGE;
+    uint2 raw[ROWS];
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j)
+      if (j < len) raw[j] = *reinterpret_cast<const uint2*>(col + (t + j) * p.ld);
+    float v[ROWS][4];
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j)
+      if (j < len) {
+        unpack4(raw[j], v[j]);
+        if (is_k) norm_rotate(p, v[j], p.kw, true, t + j, lane);
+        m = amax_of(v[j], m);
+      }
+    float* sp = p.scales + (blk * p.nkv + kvh) * 2 + (is_k ? 0 : 1);
+    const float old = at > 0 ? *sp : 0.f;
+    const float s = fmaxf(scale_of(warp_max(m)), old);
+    const float inv = 1.f / s;
+    uint8_t* page = p.codes + ((blk * 2 + (is_k ? 0 : 1)) * p.nkv + kvh) * (PAGE * D) + 4 * lane;
+    if (old < s && at > 0) {
+      const float r = old * inv;
+      for (int j = 0; j < at; ++j) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(page + j * D);
+        const float2 a = h2_to_f2(e4m3x2_to_h2(*w)), b = h2_to_f2(e4m3x2_to_h2_hi(*w));
+        *w = e4m3x2(a.x * r, a.y * r) | (e4m3x2(b.x * r, b.y * r) << 16);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j)
+      if (j < len) *reinterpret_cast<uint32_t*>(page + (at + j) * D) = codes_of(v[j], inv);
+    __syncwarp();
+    if (lane == 0) *sp = s;
+  }
+}
+
+// Check mode: one warp per (sampled token, head) recomputes the row and compares it with what the append stored: the
+// query's bits, or the codes at the page's scale (which must cover the row). Valid until a later append moves the page.
+__global__ void __launch_bounds__(256) kv8_append_check_kernel(const AppendParams p) {
+  const int lane = threadIdx.x & 31, h = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const int heads = p.nq + 2 * p.nkv;
+  if (h >= heads) return;
+  const int t = p.rows[blockIdx.x];
+  if (blockIdx.x == 0 && h == 0 && lane == 0) atomicAdd(p.check + 2, 1ull);
+  if (t < 0 || t >= p.T) return;
+  const long long slot = slot_of(p, t);
+  float v[4];
+  unpack4(*reinterpret_cast<const uint2*>(p.qkv + t * p.ld + static_cast<long long>(h) * D + 4 * lane), v);
+  int bad = -1;
+  if (h < p.nq) {
+    uint2 o = make_uint2(0x7fff7fffu, 0x7fff7fffu);
+    if (slot != -2) {
+      norm_rotate(p, v, p.qw, true, t, lane);
+      o = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+    }
+    const uint2 have = *reinterpret_cast<const uint2*>(p.q_out + (static_cast<long long>(t) * p.nq + h) * D + 4 * lane);
+    const int d1 = bf16x2_diff(o.y, have.y), d0 = bf16x2_diff(o.x, have.x);
+    bad = d0 >= 0 ? 4 * lane + d0 : d1 >= 0 ? 4 * lane + 2 + d1 : -1;
+  } else {
+    if (slot < 0) return;
+    const bool is_k = h < p.nq + p.nkv;
+    const int kvh = is_k ? h - p.nq : h - p.nq - p.nkv;
+    if (is_k) norm_rotate(p, v, p.kw, true, t, lane);
+    const long long blk = slot / PAGE;
+    const float s = p.scales[(blk * p.nkv + kvh) * 2 + (is_k ? 0 : 1)];
+    const float need = scale_of(warp_max(amax_of(v, 0.f)));
+    const uint32_t have = *reinterpret_cast<const uint32_t*>(
+        p.codes + ((blk * 2 + (is_k ? 0 : 1)) * p.nkv + kvh) * (PAGE * D) + (slot % PAGE) * D + 4 * lane);
+    if (!(s >= need)) {
+      bad = 4 * lane;
+    } else {
+      const uint32_t want = codes_of(v, 1.f / s);
+#pragma unroll
+      for (int i = 3; i >= 0; --i) {
+        const uint32_t a = (want >> (8 * i)) & 0xffu, b = (have >> (8 * i)) & 0xffu;
+        const bool same = a == b || ((a | b) & 0x7fu) == 0 || ((a & 0x7fu) == 0x7fu && (b & 0x7fu) == 0x7fu);
+        if (!same) bad = 4 * lane + i;
+      }
+    }
+  }
+  const unsigned who = __ballot_sync(0xffffffffu, bad >= 0);
+  if (who && lane == __ffs(who) - 1)
+    report_replay_mismatch(p.check, (static_cast<unsigned long long>(t) * heads + h) * D + bad);
+}
+
+// ------------------------------------------------------------------------------------------------ pages to bf16
+// Pages of the list in bf16 (exact while scales are powers of two), for the tensor-core prefill: a prefill reads each
+// page once for every 256 / group of its query rows, so expanding it once costs less than expanding it in every CTA.
+// One warp per (page, K / V, kv head): 2 KB in, 4 KB out. A page id outside the cache gives NaN. The first warps also
+// bring the positions into the plan's table (pos >= limit becomes -1, a row without keys). With `check`: the pages
+// every `step`-th of the list from `from` are compared instead of written.
+struct ExpandParams {
+  const uint8_t* codes;
+  const float* scales;
+  const int* pages;
+  int npages, nkv;
+  long long num_blocks;
+  __nv_bfloat16* out;
+  const int* pos;
+  int* pos_out;
+  int T, limit;
+  int from, step;
+  unsigned long long* check;
+};
+
+__global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
+  const long long gt = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  for (long long i = gt; i < p.T; i += static_cast<long long>(gridDim.x) * 256) {
+    const int v = p.pos[i];
+    p.pos_out[i] = v >= p.limit ? -1 : v;
+  }
+  const long long gw = gt >> 5;
+  const int lane = threadIdx.x & 31, per = 2 * p.nkv;
+  const long long i = p.check == nullptr ? gw / per : p.from + gw / per * p.step;
+  if (i >= p.npages) return;
+  const int unit = static_cast<int>(gw % per), kv = unit / p.nkv, h = unit % p.nkv;
+  const int blk = p.pages[i];
+  const bool in = blk >= 0 && blk < p.num_blocks;
+  const float s = in ? p.scales[(static_cast<long long>(blk) * p.nkv + h) * 2 + kv] : __int_as_float(0x7fffffff);
+  const uint4* src = reinterpret_cast<const uint4*>(
+      p.codes + ((static_cast<long long>(in ? blk : 0) * 2 + kv) * p.nkv + h) * (PAGE * D));
+  uint4* dst = reinterpret_cast<uint4*>(p.out + ((i * 2 + kv) * p.nkv + h) * (PAGE * D));
+  uint4 c[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c[j] = src[j * 32 + lane];
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t w[4] = {c[j].x, c[j].y, c[j].z, c[j].w};
+    uint32_t o[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 a = h2_to_f2(e4m3x2_to_h2(w[e])), b = h2_to_f2(e4m3x2_to_h2_hi(w[e]));
+      o[2 * e] = pack_bf16x2(a.x * s, a.y * s);
+      o[2 * e + 1] = pack_bf16x2(b.x * s, b.y * s);
+    }
+    uint4* d = dst + 2 * (j * 32 + lane);
+    if (p.check == nullptr) {
+      d[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      d[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    } else {
+      const uint4 a = d[0], b = d[1];
+      const uint32_t have[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bad |= bf16x2_diff(o[e], have[e]) >= 0;
+    }
+  }
+  if (p.check != nullptr) {
+    const unsigned who = __ballot_sync(0xffffffffu, bad);
+    if (who && lane == 0) report_replay_mismatch(p.check, static_cast<unsigned long long>(i) * per + unit);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ decode
+// One new token per sequence, o = sum_j w_j v_j / sum_j w_j with w_j = exp(scale q . k_j). Bound by the cache bytes
+// (256 a key and kv head); the queries of a kv head (<= 16) share every key that is read.
+//
+// Tensor cores on converted codes (mma.m16n8k16, f16 inputs, fp32 sums): E4M3 is exact in f16, so scales stay outside
+// the products. Both products have the cache as their A operand, whose fragments a lane fills from its own 16-byte
+// loads: S^T (16 keys x heads) = K Q^T, with the order of the dims permuted alike in K and Q so that a lane's four
+// codes of a k step are neighbours; O^T (dims x heads) += V^T P^T, with the pairs of keys put together by byte
+// permutes. Nothing passes through shared memory until the warps of a CTA merge.
+//   q: bf16 values times a power of two per head (largest in [2^14, 2^15)), exact in f16 down to 2^-38 of the largest.
+//   x = log2(e) scale s_K q . k, and with V's page scale in the exponent y = x + log2 s_V. The running maximum M is of
+//   y, so the weights w = 2^(x - M + 14) s_V <= 2^15 are the largest f16 can hold whatever the pages' scales; the row
+//   sum takes 2^(x - M + 30) in fp32: x - M reaches from 60 (a page of the least scale) to -128 and below, so the bias
+//   keeps both ends inside fp32. Rounding w to f16 costs 2^-11 of it, less than the output's rounding to bf16 (2^-8).
+//   Masked keys: x = -inf and V's codes cleared (0 * NaN); rows without keys give 0.
+//
+// A CTA (4 warps) takes one segment of seg_pages pages of one (sequence, kv head), warp w its pages w, w + 4, ...; a
+// sequence of one segment is written at once, else a partial record per segment and head goes to `part` and
+// kv8_combine_kernel merges them in order. Segments start at absolute multiples, so a row's arithmetic does not depend
+// on the batch around it: running a subset of rows again with the same plan gives the same bits (check mode).
+// A sequence whose length or table row does not fit gives NaN, as does a page id outside the cache.
+constexpr int WARPS = 4;
+constexpr int REC = D + 4;               // floats a record: o[D], M, l, pad
+
+struct DecodeParams {
+  const __nv_bfloat16* q;
+  __nv_bfloat16* o;
+  const uint8_t* codes;
+  const float2* scales;      // [num_blocks][nkv] (K, V)
+  long long num_blocks;
+  const int* table;          // [table_rows][max_pages], rows `table_ld` apart
+  int table_rows, max_pages;
+  long long table_ld;
+  const int* seq_req;
+  const int* ctx;
+  const int* seq_idx;
+  int nseqs;                 // sequences of q (bound of seq_idx)
+  int nq, nkv, G;
+  int seg_pages, max_segs;
+  float scale_log2;
+  float* part;               // [nseqs][nkv][max_segs][G][REC]
+  float* row_sq;
+  unsigned long long* check;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+struct PageRegs {
+  uint4 k[4];      // key g: dims 16t.., 64 + 16t..; key g + 8: the same
+  uint4 v[4];      // keys 2t, 2t + 1, 2t + 8, 2t + 9: dims 16g..
+};
+__device__ __forceinline__ void load_page(PageRegs& r, const uint8_t* kp, const uint8_t* vp, int g, int t) {
+  r.k[0] = ld_stream(kp + g * D + 16 * t);
+  r.k[1] = ld_stream(kp + g * D + 64 + 16 * t);
+  r.k[2] = ld_stream(kp + (g + 8) * D + 16 * t);
+  r.k[3] = ld_stream(kp + (g + 8) * D + 64 + 16 * t);
+  r.v[0] = ld_stream(vp + (2 * t) * D + 16 * g);
+  r.v[1] = ld_stream(vp + (2 * t + 1) * D + 16 * g);
+  r.v[2] = ld_stream(vp + (2 * t + 8) * D + 16 * g);
+  r.v[3] = ld_stream(vp + (2 * t + 9) * D + 16 * g);
+}
+__device__ __forceinline__ uint32_t word(const uint4& u, int j) { return j == 0 ? u.x : j == 1 ? u.y : j == 2 ? u.z : u.w; }
+
+// The value at output element i of row (sequence b), or its comparison with what is there.
+__device__ __forceinline__ float put(const DecodeParams& p, int b, int head, int d, float v) {
+  const long long at = (static_cast<long long>(b) * p.nq + head) * D + d;
+  const __nv_bfloat16 r = __float2bfloat16(v);
+  const float x = __bfloat162float(r);
+  if (p.check == nullptr) {
+    p.o[at] = r;
+  } else {
+    const float y = __bfloat162float(p.o[at]);
+    if (!(x == y) && !(x != x && y != y)) report_replay_mismatch(p.check, static_cast<unsigned long long>(at));
+  }
+  return x * x;
+}
+
+__device__ __forceinline__ int pages_of(int n) { return n / PAGE + (n % PAGE > 0 ? 1 : 0); }
+__device__ __forceinline__ bool row_fits(const DecodeParams& p, int n, int req) {
+  return n >= 0 && pages_of(n) <= p.max_pages && pages_of(n) <= p.max_segs * p.seg_pages && req >= 0 &&
+         req < p.table_rows;
+}
+
+// NT: groups of eight heads (1: up to 8 queries a kv head, 2: up to 16).
+template <int NT>
+__global__ void __launch_bounds__(WARPS * 32) kv8_decode_kernel(const DecodeParams p) {
+  pdl_trigger();
+  __shared__ float osm[WARPS][NT * 8][D];
+  __shared__ float msm[WARPS][NT * 8], lsm[WARPS][NT * 8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int b = p.seq_idx ? p.seq_idx[blockIdx.x] : blockIdx.x;
+  if (b < 0 || b >= p.nseqs) return;
+  const int kvh = blockIdx.y;
+  const int n = p.ctx[b], req = p.seq_req[b];
+  const int pages = pages_of(n);
+  const bool fits = row_fits(p, n, req);
+  if (p.check != nullptr && blockIdx.x == 0 && kvh == 0 && blockIdx.z == 0 && tid == 0) atomicAdd(p.check + 2, 1ull);
+  if (!fits || n == 0) {
+    if (blockIdx.z != 0) return;
+    const float v = fits ? 0.f : __int_as_float(0x7fffffff);
+    for (int h = 0; h < p.G; ++h) put(p, b, kvh * p.G + h, tid, v);
+    return;
+  }
+  const int nseg = (pages + p.seg_pages - 1) / p.seg_pages;
+  if (static_cast<int>(blockIdx.z) >= nseg) return;
+  // Q^T fragments: b0 = dims 64c + 16t + 4j + {0, 1}, b1 = + {2, 3} of head g, k step 4c + j
+  uint32_t qb[NT][8][2];
+  float f[NT][2];                    // heads 2t, 2t + 1: scale log2(e) / (the head's power of two)
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int h = nt * 8 + g;
+    uint32_t w[16];
+    float m = 0.f;
+    const __nv_bfloat16* row = p.q + (static_cast<long long>(b) * p.nq + kvh * p.G + (h < p.G ? h : 0)) * D;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint4 u = h < p.G ? *reinterpret_cast<const uint4*>(row + 64 * c + 16 * t + 8 * e) : make_uint4(0, 0, 0, 0);
+        w[c * 8 + e * 4] = u.x;
+        w[c * 8 + e * 4 + 1] = u.y;
+        w[c * 8 + e * 4 + 2] = u.z;
+        w[c * 8 + e * 4 + 3] = u.w;
+      }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+      m = fmaxf(m, fmaxf(fabsf(x.x), fabsf(x.y)));
+    }
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    int e = static_cast<int>(__float_as_uint(m) >> 23) - 127;
+    e = e < -100 ? -100 : e > 127 ? 14 : e;            // not finite: as it is
+    const float up = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
+    const float down = __uint_as_float(static_cast<uint32_t>(e - 14 + 127) << 23);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+      qb[nt][i >> 1][i & 1] = pack_h2(x.x * up, x.y * up);
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) f[nt][c] = p.scale_log2 * __shfl_sync(0xffffffffu, down, (2 * t + c) * 4);
+  }
+  const int* row = p.table + req * p.table_ld;
+  const long long kv_stride = static_cast<long long>(p.nkv) * PAGE * D;
+  for (int seg = blockIdx.z; seg < nseg; seg += gridDim.z) {
+    const int first = seg * p.seg_pages + warp, end = min(pages, (seg + 1) * p.seg_pages);
+    const int count = first < end ? (end - first + WARPS - 1) / WARPS : 0;
+    float M[NT][2], l[NT][2], o[NT][8][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      M[nt][0] = M[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+    }
+    long long blk = 0;
+    float2 sc = make_float2(0.f, 0.f);
+    PageRegs cur;
+    // 32 of this warp's pages at a time: lane i holds the id and the scales of page i
+    for (int k0 = 0; k0 < count; k0 += 32) {
+      {
+        const int k = k0 + lane;
+        int id = k < count ? row[first + WARPS * k] : 0;
+        const bool in = id >= 0 && id < p.num_blocks;
+        blk = in ? id : 0;
+        sc = k < count ? p.scales[blk * p.nkv + kvh] : make_float2(0.f, 0.f);
+        if (!in) sc.x = sc.y = __int_as_float(0x7fffffff);
+      }
+      const int kn = min(32, count - k0);
+      {
+        const uint8_t* kp = p.codes + (__shfl_sync(0xffffffffu, blk, 0) * 2 * p.nkv + kvh) * (PAGE * D);
+        load_page(cur, kp, kp + kv_stride, g, t);
+      }
+      for (int k = 0; k < kn; ++k) {
+        PageRegs nxt;
+        const float ks = __shfl_sync(0xffffffffu, sc.x, k), vs = __shfl_sync(0xffffffffu, sc.y, k);
+        const long long nb = __shfl_sync(0xffffffffu, blk, (k + 1) & 31);
+        if (k + 1 < kn) {
+          const uint8_t* kp = p.codes + (nb * 2 * p.nkv + kvh) * (PAGE * D);
+          load_page(nxt, kp, kp + kv_stride, g, t);
+        }
+        const int key0 = (first + WARPS * (k0 + k)) * PAGE;
+        if (key0 + PAGE > n) {         // the sequence's last page: nothing behind its end may reach a product
+          const uint4 z = make_uint4(0, 0, 0, 0);
+          if (key0 + 2 * t >= n) cur.v[0] = z;
+          if (key0 + 2 * t + 1 >= n) cur.v[1] = z;
+          if (key0 + 2 * t + 8 >= n) cur.v[2] = z;
+          if (key0 + 2 * t + 9 >= n) cur.v[3] = z;
+        }
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t w0 = word(cur.k[c], j), w1 = word(cur.k[2 + c], j);
+            const uint32_t a0 = e4m3x2_to_h2(w0), a2 = e4m3x2_to_h2_hi(w0);
+            const uint32_t a1 = e4m3x2_to_h2(w1), a3 = e4m3x2_to_h2_hi(w1);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a0, a1, a2, a3, qb[nt][4 * c + j][0], qb[nt][4 * c + j][1]);
+          }
+        const float ev = static_cast<float>(max(static_cast<int>((__float_as_uint(vs) >> 23) & 255u) - 127, -60));
+        const float vw = vs * W_SCALE;       // s_V 2^(14 - SUM_BIAS)
+        const bool in0 = key0 + g < n, in1 = key0 + g + 8 < n;
+        uint32_t pb[NT][2];
+        bool moved = false;
+        float a[NT][2], Mn[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float fk = f[nt][c] * ks;
+            s[nt][c] = in0 ? s[nt][c] * fk : -INFINITY;
+            s[nt][2 + c] = in1 ? s[nt][2 + c] * fk : -INFINITY;
+            float mx = fmaxf(s[nt][c], s[nt][2 + c]) + ev;
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            Mn[nt][c] = fmaxf(M[nt][c], mx);
+            moved |= Mn[nt][c] != M[nt][c];
+          }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              a[nt][c] = Mn[nt][c] == M[nt][c] ? 1.f : ex2(M[nt][c] - Mn[nt][c]);
+              M[nt][c] = Mn[nt][c];
+              l[nt][c] *= a[nt][c];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              o[nt][i][0] *= a[nt][0];
+              o[nt][i][1] *= a[nt][1];
+              o[nt][i][2] *= a[nt][0];
+              o[nt][i][3] *= a[nt][1];
+            }
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float w[4];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float ref = M[nt][c] == -INFINITY ? 0.f : M[nt][c] - SUM_BIAS;
+            const float p0 = ex2(s[nt][c] - ref), p1 = ex2(s[nt][2 + c] - ref);
+            l[nt][c] += p0 + p1;
+            w[c] = p0 * vw;
+            w[2 + c] = p1 * vw;
+          }
+          pb[nt][0] = transpose8(pack_h2(w[0], w[1]));
+          pb[nt][1] = transpose8(pack_h2(w[2], w[3]));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w0 = word(cur.v[0], j), w1 = word(cur.v[1], j), w2 = word(cur.v[2], j), w3 = word(cur.v[3], j);
+          const uint32_t x01 = __byte_perm(w0, w1, 0x5140), y01 = __byte_perm(w0, w1, 0x7362);
+          const uint32_t x23 = __byte_perm(w2, w3, 0x5140), y23 = __byte_perm(w2, w3, 0x7362);
+          const uint32_t a0 = e4m3x2_to_h2(x01), a1 = e4m3x2_to_h2_hi(x01);
+          const uint32_t a2 = e4m3x2_to_h2(x23), a3 = e4m3x2_to_h2_hi(x23);
+          const uint32_t c0 = e4m3x2_to_h2(y01), c1 = e4m3x2_to_h2_hi(y01);
+          const uint32_t c2 = e4m3x2_to_h2(y23), c3 = e4m3x2_to_h2_hi(y23);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_f16(o[nt][2 * j], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+            mma_f16(o[nt][2 * j + 1], c0, c1, c2, c3, pb[nt][0], pb[nt][1]);
+          }
+        }
+        cur = nxt;
+      }
+    }
+    // merge of the four warps: o[nt][i] holds dims 16g + 2i + {0, 1} of heads 2t, 2t + 1
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int h = nt * 8 + 2 * t + c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<float2*>(&osm[warp][h][16 * g + 2 * i]) = make_float2(o[nt][i][c], o[nt][i][2 + c]);
+        float s = l[nt][c];
+        s += __shfl_xor_sync(0xffffffffu, s, 4);
+        s += __shfl_xor_sync(0xffffffffu, s, 8);
+        s += __shfl_xor_sync(0xffffffffu, s, 16);
+        if (g == 0) {
+          msm[warp][h] = M[nt][c];
+          lsm[warp][h] = s;
+        }
+      }
+    }
+    __syncthreads();
+    float sq = 0.f;
+    for (int h = 0; h < p.G; ++h) {
+      const float m = fmaxf(fmaxf(msm[0][h], msm[1][h]), fmaxf(msm[2][h], msm[3][h]));
+      const float ref = m == -INFINITY ? 0.f : m;
+      float acc = 0.f, ls = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float e = ex2(msm[w][h] - ref);
+        acc = fmaf(osm[w][h][tid], e, acc);
+        ls = fmaf(lsm[w][h], e, ls);
+      }
+      if (nseg == 1) {
+        sq += put(p, b, kvh * p.G + h, tid, ls == 0.f ? 0.f : acc / ls * (1.f / W_SCALE));
+      } else {
+        float* rec = p.part + (((static_cast<long long>(b) * p.nkv + kvh) * p.max_segs + seg) * p.G + h) * REC;
+        rec[tid] = acc;
+        if (tid == 0) {
+          rec[D] = m;
+          rec[D + 1] = ls;
+        }
+      }
+    }
+    if (nseg == 1 && p.check == nullptr && p.row_sq != nullptr) {
+      sq = warp_sum(sq);
+      if (lane == 0) atomicAdd(p.row_sq + b, sq);
+    }
+    __syncthreads();
+  }
+}
+
+// Merges the segments of each (sequence, head), in segment order within four interleaved parts: thread (part, dim).
+constexpr int PARTS = 4;
+constexpr int MAX_SEGS = 256;
+__global__ void __launch_bounds__(PARTS * D) kv8_combine_kernel(const DecodeParams p) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ float wsm[MAX_SEGS], red[PARTS * D / 32], osm[PARTS][D], lsum;
+  const int tid = threadIdx.x, part = tid / D, d = tid % D;
+  const int b = p.seq_idx ? p.seq_idx[blockIdx.x] : blockIdx.x;
+  if (b < 0 || b >= p.nseqs) return;
+  const int head = blockIdx.y, kvh = head / p.G, h = head % p.G;
+  const int n = p.ctx[b];
+  const int nseg = (pages_of(n) + p.seg_pages - 1) / p.seg_pages;
+  if (!row_fits(p, n, p.seq_req[b]) || nseg <= 1) return;
+  const long long step = static_cast<long long>(p.G) * REC;
+  const float* base = p.part + (((static_cast<long long>(b) * p.nkv + kvh) * p.max_segs) * p.G + h) * REC;
+  const float m = tid < nseg ? base[tid * step + D] : -INFINITY;
+  const float wm = warp_max(m);
+  if ((tid & 31) == 0) red[tid >> 5] = wm;
+  __syncthreads();
+  float M = red[0];
+#pragma unroll
+  for (int i = 1; i < PARTS * D / 32; ++i) M = fmaxf(M, red[i]);
+  const float ref = M == -INFINITY ? 0.f : M;
+  float lp = 0.f;
+  if (tid < nseg) {
+    const float e = ex2(m - ref);
+    wsm[tid] = e;
+    lp = base[tid * step + D + 1] * e;
+  }
+  __syncthreads();
+  lp = warp_sum(lp);
+  if ((tid & 31) == 0) red[tid >> 5] = lp;
+  float acc = 0.f;
+#pragma unroll 8
+  for (int s = part; s < nseg; s += PARTS) acc = fmaf(base[s * step + d], wsm[s], acc);
+  osm[part][d] = acc;
+  __syncthreads();
+  if (tid == 0) {
+    float s = 0.f;
+    for (int i = 0; i < PARTS * D / 32; ++i) s += red[i];
+    lsum = s;
+  }
+  __syncthreads();
+  if (part != 0) return;
+  const float o = (osm[0][d] + osm[1][d]) + (osm[2][d] + osm[3][d]);
+  float sq = put(p, b, head, d, lsum == 0.f ? 0.f : o / lsum * (1.f / W_SCALE));
+  if (p.check == nullptr && p.row_sq != nullptr) {
+    sq = warp_sum(sq);
+    if ((tid & 31) == 0) atomicAdd(p.row_sq + b, sq);
+  }
+}
+
+template <int NT>
+static int launch_decode(const DecodeParams& p, int nrun, int z, cudaStream_t st) {
+  kv8_decode_kernel<NT><<<dim3(nrun, p.nkv, z), WARPS * 32, 0, st>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || p.max_segs == 1) return static_cast<int>(e);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(nrun, p.nq);
+  cfg.blockDim = dim3(PARTS * D);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kv8_combine_kernel, p));
+}
+
+}  // namespace kv8
+}  // namespace sdc
+
+using namespace sdc::kv8;
+
+extern "C" {
+
+int sdc_kv8_append(const void* qkv, long long ld, int T, int nq, int nkv, const int* pos, const long long* slots,
+                   const void* qw, const void* kw, float eps, const void* cos_sin, int table_rows, int rotary,
+                   int interleaved, void* q_out, void* codes, void* scales, long long num_blocks, const int* rows,
+                   int nrows, void* check, void* stream) {
+  if (T <= 0 || (check != nullptr && nrows <= 0)) return 0;
+  if (ld % 4 || rotary < 0 || rotary > D || rotary % 8 || nq < 0 || nkv < 1 || (check != nullptr) != (rows != nullptr))
+    return -1;
+  AppendParams p;
+  p.qkv = static_cast<const __nv_bfloat16*>(qkv);
+  p.ld = ld;
+  p.T = T;
+  p.nq = nq;
+  p.nkv = nkv;
+  p.pos = pos;
+  p.slots = slots;
+  p.qw = static_cast<const __nv_bfloat16*>(qw);
+  p.kw = static_cast<const __nv_bfloat16*>(kw);
+  p.eps = eps;
+  p.cs = static_cast<const float2*>(cos_sin);
+  p.table_rows = table_rows;
+  p.rotary = rotary;
+  p.interleaved = interleaved;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.codes = static_cast<uint8_t*>(codes);
+  p.scales = static_cast<float*>(scales);
+  p.capacity = num_blocks * PAGE;
+  p.rows = rows;
+  p.nrows = nrows;
+  p.check = static_cast<unsigned long long*>(check);
+  const int gy = (nq + 2 * nkv + 7) / 8;
+  auto st = static_cast<cudaStream_t>(stream);
+  if (p.check != nullptr) kv8_append_check_kernel<<<dim3(nrows, gy), 256, 0, st>>>(p);
+  else if (T < 1024) kv8_append_kernel<1><<<dim3(T, gy), 256, 0, st>>>(p);
+  else kv8_append_kernel<16><<<dim3((T + 15) / 16, gy), 256, 0, st>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+
+int sdc_kv8_expand(const void* codes, const void* scales, long long num_blocks, const int* pages, int npages, int nkv,
+                   void* out, const int* pos, int* pos_out, int T, int limit, int from, int step, void* check,
+                   void* stream) {
+  if (npages <= 0) return 0;
+  if (nkv < 1 || num_blocks < 1 || (check != nullptr && (from < 0 || step < 1))) return -1;
+  ExpandParams p;
+  p.codes = static_cast<const uint8_t*>(codes);
+  p.scales = static_cast<const float*>(scales);
+  p.pages = pages;
+  p.npages = npages;
+  p.nkv = nkv;
+  p.num_blocks = num_blocks;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.pos = pos;
+  p.pos_out = pos_out;
+  p.T = T;
+  p.limit = limit;
+  p.from = from;
+  p.step = step;
+  p.check = static_cast<unsigned long long*>(check);
+  const long long n = check == nullptr ? npages : (npages - from + step - 1) / step;
+  const long long blocks = n <= 0 ? 1 : (n * 2 * nkv * 32 + 255) / 256;
+  kv8_expand_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// part: nseqs * nkv * max_segs * (nq / nkv) * 132 floats (not read where max_segs is 1); rows of `nrun` sequences are
+// computed: seq_idx's, or the first nrun.
+int sdc_kv8_decode(const void* q, void* o, const void* codes, const void* scales, long long num_blocks,
+                   const int* table, int table_rows, int max_pages, long long table_ld, const int* seq_req,
+                   const int* ctx, const int* seq_idx, int nrun, int nseqs, int nq, int nkv, int seg_pages,
+                   int max_segs, float scale, void* part, void* row_sq, void* check, void* stream) {
+  if (nrun <= 0) return 0;
+  if (nkv < 1 || nq % nkv || nq / nkv < 1 || nq / nkv > 16 || seg_pages < 1 || max_segs < 1 || max_segs > MAX_SEGS ||
+      (max_segs > 1 && part == nullptr) || (check != nullptr && seq_idx == nullptr) ||
+      (seq_idx == nullptr && nrun > nseqs))
+    return -1;
+  DecodeParams p;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.o = static_cast<__nv_bfloat16*>(o);
+  p.codes = static_cast<const uint8_t*>(codes);
+  p.scales = static_cast<const float2*>(scales);
+  p.num_blocks = num_blocks;
+  p.table = table;
+  p.table_rows = table_rows;
+  p.max_pages = max_pages;
+  p.table_ld = table_ld;
+  p.seq_req = seq_req;
+  p.ctx = ctx;
+  p.seq_idx = seq_idx;
+  p.nseqs = nseqs;
+  p.nq = nq;
+  p.nkv = nkv;
+  p.G = nq / nkv;
+  p.seg_pages = seg_pages;
+  p.max_segs = max_segs;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.part = static_cast<float*>(part);
+  p.row_sq = static_cast<float*>(row_sq);
+  p.check = static_cast<unsigned long long*>(check);
+  // every segment its own CTA while that is at most 32768 CTAs (an empty one costs nanoseconds); else CTAs take several
+  const long long rows = static_cast<long long>(nrun) * nkv;
+  long long z = 32768 / rows;
+  z = z < 1 ? 1 : z > max_segs ? max_segs : z;
+  auto st = static_cast<cudaStream_t>(stream);
+  return p.G <= 8 ? launch_decode<1>(p, nrun, static_cast<int>(z), st) : launch_decode<2>(p, nrun, static_cast<int>(z), st);
+}
+
+}  // extern "C"

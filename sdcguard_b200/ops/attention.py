@@ -1,5 +1,6 @@
 """Paged attention entry points (`csrc/attention.cu`): causal prefill over a batch of requests and single-token
-decode, both over a paged KV cache with 16-token pages, plus the host-side tiling of prefill work.
+decode, both over a paged KV cache with 16-token pages, plus the host-side tiling of prefill work; `decode8` and
+`prefill8` do the same over a cache held in 8 bits (`csrc/kv8.cu`, `ops.kv8`).
 
 Rows of both kernels are deterministic (see the kernel file), so `replay_*` recompute a sample of rows on
 separate CTAs and `ops.layers.compare_rows` checks them bit for bit. The reference samples (token, head) pairs
@@ -9,11 +10,14 @@ and recomputes them in fp32 against an error bound (src/sdcguard/serve_attn.py:5
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
 from typing import Optional, Sequence
 
 import torch
 
 from .. import _native
+from . import kv8
+from .kv8 import PAGE, KV8Cache
 
 ROWS = 128
 
@@ -110,6 +114,172 @@ def decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, seq_
         int(max_ctx), float(scale), scratch.data_ptr(), None if row_sq is None else row_sq.data_ptr(),
         None if check is None else check.data_ptr(), _s(q)), "attention decode")
     return out
+
+
+# ------------------------------------------------------------------------------------ cache in 8 bits (csrc/kv8.cu)
+DECODE8_CTAS = 148 * 9      # CTAs a decode step is cut into where it has the keys: about three rounds of three per SM
+DECODE8_MAX_SEGS = 256
+
+
+@dataclass
+class Decode8Plan:
+    """How `decode8` cuts the keys of up to nseq sequences of up to max_ctx keys, and its scratch. A replay (check mode)
+    takes the plan of the call that it repeats: the cut decides the order of the sums. One launch at a time may use a
+    plan; two streams, or two graphs that may run at once, take a plan each."""
+    nseq: int
+    nq: int
+    nkv: int
+    max_ctx: int
+    seg_pages: int
+    max_segs: int
+    part: Optional[torch.Tensor]
+
+
+def decode8_cut(nseq: int, nkv: int, max_ctx: int) -> tuple[int, int]:
+    """(pages a segment, segments of the longest sequence) of a decode step: segments of equal size, so many that all
+    SMs have work, from 4 pages (one per warp) to 256 pages, and at most 256 of them (what one combine CTA merges)."""
+    pages = -(-max_ctx // PAGE)
+    seg = -(-nseq * nkv * pages // DECODE8_CTAS)
+    seg = max(4, min(256, -(-seg // 4) * 4), -(-pages // DECODE8_MAX_SEGS))
+    return seg, -(-pages // seg)
+
+
+def decode8_plan(nseq: int, nq: int, nkv: int, max_ctx: int, device) -> Decode8Plan:
+    """Plan and scratch of `decode8` for up to nseq sequences of up to max_ctx keys."""
+    if nseq < 1 or nkv < 1 or nq % nkv or not 1 <= nq // nkv <= 16 or not 1 <= max_ctx <= 1 << 24:
+        raise ValueError(f"nseq {nseq}, nq {nq}, nkv {nkv}, max_ctx {max_ctx}: at least one sequence, 1 to 16 query "
+                         "heads per kv head, 1 to 2^24 keys")
+    seg, segs = decode8_cut(nseq, nkv, max_ctx)
+    part = torch.empty(nseq * nq * segs * 132, dtype=torch.float32, device=device) if segs > 1 else None
+    return Decode8Plan(nseq, nq, nkv, max_ctx, seg, segs, part)
+
+
+def _want_q(q: torch.Tensor, cache: KV8Cache, out: Optional[torch.Tensor]) -> torch.Tensor:
+    dev = cache.codes.device
+    if cache.codes.dim() != 5:
+        raise ValueError("the cache must be one layer of a KV8Cache")
+    kv8.want(q, torch.bfloat16, (q.shape[0], q.shape[1], 128), dev, "q", align=16)
+    if out is None:
+        return torch.empty_like(q)
+    return kv8.want(out, torch.bfloat16, tuple(q.shape), dev, "out", align=16)
+
+
+def _want_extra(row_sq, check, rows: int, dev) -> None:
+    if row_sq is not None:
+        kv8.want(row_sq, torch.float32, (rows,), dev, "row_sq")
+    if check is not None and (check.dtype != torch.int64 or check.device != dev):
+        raise ValueError("check must be a state row (int64) on the cache's device")
+
+
+def decode8(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_req: torch.Tensor, ctx: torch.Tensor,
+            plan: Decode8Plan, out: Optional[torch.Tensor] = None, seq_idx: Optional[torch.Tensor] = None,
+            row_sq: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+            check: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per sequence over a cache of 8 bits: q (B, nq, 128) bf16, ctx[b] keys (the new token's
+    among them) in the pages of row seq_req[b] of block_table (int32). Any number of query heads per kv head up to 16.
+
+    A sequence without keys (ctx 0) gives zeros. One with more keys than its table row or the plan holds, a table row
+    that does not exist, or a page outside the cache gives NaN. seq_idx selects sequences; with `check` (a state row)
+    they are recomputed and compared with `out`. row_sq: += ||row||^2 of the output (cleared by the caller; its sum
+    over kv heads is taken in no fixed order)."""
+    b, nq = q.shape[0], q.shape[1]
+    dev, nkv = cache.codes.device, cache.nkv
+    out = _want_q(q, cache, out)
+    if (nq, nkv) != (plan.nq, plan.nkv) or b > plan.nseq:
+        raise ValueError(f"q {tuple(q.shape)} and {nkv} kv heads do not fit the plan ({plan.nseq} sequences, {plan.nq} "
+                         f"query and {plan.nkv} kv heads)")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.device != dev \
+            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be int32 (requests, pages) with contiguous rows on the cache's device")
+    kv8.want(seq_req, torch.int32, (b,), dev, "seq_req")
+    kv8.want(ctx, torch.int32, (b,), dev, "ctx")
+    if seq_idx is not None:
+        kv8.want(seq_idx, torch.int32, (seq_idx.shape[0],), dev, "seq_idx")
+    elif check is not None:
+        raise ValueError("check needs seq_idx")
+    if plan.part is not None and plan.part.device != dev:
+        raise ValueError("the plan must be on the cache's device")
+    _want_extra(row_sq, check, b, dev)
+    with kv8.on(dev):
+        _native.check(_native.lib().sdc_kv8_decode(
+            q.data_ptr(), out.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks,
+            block_table.data_ptr(), block_table.shape[0], block_table.shape[1], block_table.stride(0),
+            seq_req.data_ptr(), ctx.data_ptr(), None if seq_idx is None else seq_idx.data_ptr(),
+            b if seq_idx is None else seq_idx.shape[0], b, nq, nkv, plan.seg_pages, plan.max_segs,
+            1.0 / math.sqrt(128) if scale is None else float(scale), None if plan.part is None else plan.part.data_ptr(),
+            None if row_sq is None else row_sq.data_ptr(), None if check is None else check.data_ptr(), _s(q)),
+            "attention decode (8-bit cache)")
+    return out
+
+
+@dataclass
+class Prefill8Plan:
+    """The pages of a prefill batch in one list, and the bf16 pages they are expanded to. The same rules as for
+    `Decode8Plan`: one launch at a time, and a replay takes the plan of the call that it repeats."""
+    pages: torch.Tensor        # (P,) int32 page ids, request after request
+    table: torch.Tensor        # (R, W) int32 places in that list
+    work: torch.Tensor         # (P, 2, nkv, 16, 128) bf16
+    nkv: int
+
+
+def prefill8_plan(block_table: torch.Tensor, ctx_lens: Sequence[int], nkv: int,
+                  work: Optional[torch.Tensor] = None) -> Prefill8Plan:
+    """Plan of `prefill8` for requests of ctx_lens keys (cached and new ones) in the rows of block_table. `work`: bf16
+    memory for the expanded pages (at least 4096 nkv elements a page), kept by the caller across layers and steps."""
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != len(ctx_lens):
+        raise ValueError("block_table must be int32 with one row for each of ctx_lens")
+    dev, width = block_table.device, block_table.shape[1]
+    counts = [-(-int(n) // PAGE) for n in ctx_lens]
+    if not counts or min(int(n) for n in ctx_lens) < 1 or max(counts) > width:
+        raise ValueError(f"ctx_lens {list(ctx_lens)[:8]}: at least one key each, and no more than {width} pages")
+    total, w = sum(counts), max(counts)
+    c = torch.tensor(counts)
+    first = torch.cumsum(c, 0) - c
+    place = torch.arange(w)[None]
+    used = place < c[:, None]
+    table = torch.where(used, first[:, None] + place, 0).to(torch.int32)
+    pages = block_table[:, :w][used.to(dev)].contiguous()
+    need = total * 2 * nkv * PAGE * 128
+    if work is None:
+        work = torch.empty(need, dtype=torch.bfloat16, device=dev)
+    elif work.dtype != torch.bfloat16 or work.numel() < need or not work.is_contiguous() or work.device != dev \
+            or work.data_ptr() % 128:
+        raise ValueError(f"work must be contiguous bf16 of at least {need} elements on {dev}")
+    return Prefill8Plan(pages, table.to(dev), work.view(-1)[:need].view(total, 2, nkv, PAGE, 128), nkv)
+
+
+def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Tensor, tiles: torch.Tensor,
+             out: Optional[torch.Tensor] = None, row_idx: Optional[torch.Tensor] = None,
+             row_sq: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+             check: Optional[torch.Tensor] = None, pages_from: int = 0, pages_step: int = 64) -> torch.Tensor:
+    """`prefill` over a cache of 8 bits: the plan's pages are expanded to bf16 (exact for power-of-two scales), then the
+    tensor-core prefill reads those. q (T, nq, 128), tiles from `prefill_tiles`, requests numbered as in the plan. With
+    `check`: every pages_step-th expanded page from pages_from on and the rows of the replay tiles are compared."""
+    dev, nkv, nq = cache.codes.device, cache.nkv, q.shape[1]
+    out = _want_q(q, cache, out)
+    t = q.shape[0]
+    if nkv != plan.nkv or nq % nkv or ROWS % (nq // nkv) or nq == 0:
+        raise ValueError(f"{nq} query heads on {nkv} kv heads (plan: {plan.nkv}): a power of two up to 128 per kv head")
+    kv8.want(pos, torch.int32, (t,), dev, "pos")
+    kv8.want(tiles, torch.int32, (tiles.shape[0], 4), dev, "tiles", align=16)
+    if plan.work.device != dev:
+        raise ValueError("the plan must be on the cache's device")
+    if check is not None and (row_idx is None or pages_from < 0 or pages_step < 1):
+        raise ValueError("check needs replay tiles with row_idx, and pages_from >= 0, pages_step >= 1")
+    if row_idx is not None:
+        kv8.want(row_idx, torch.int32, (row_idx.shape[0],), dev, "row_idx")
+    _want_extra(row_sq, check, t, dev)
+    if t == 0 or tiles.shape[0] == 0:
+        return out
+    with kv8.on(dev):
+        inside = torch.empty(t, dtype=torch.int32, device=dev)      # pos, -1 where it lies outside the plan's table
+        _native.check(_native.lib().sdc_kv8_expand(
+            cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, plan.pages.data_ptr(),
+            plan.pages.shape[0], nkv, plan.work.data_ptr(), pos.data_ptr(), inside.data_ptr(), t,
+            plan.table.shape[1] * PAGE, int(pages_from), int(pages_step), None if check is None else check.data_ptr(),
+            _s(q)), "expanding 8-bit cache pages")
+        return prefill(q, plan.work, plan.table, inside, tiles, nq, nkv, out=out, row_idx=row_idx, row_sq=row_sq,
+                       scale=scale, check=check)
 
 
 def reference_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_pos: torch.Tensor) -> torch.Tensor:

@@ -8,6 +8,8 @@ from typing import Optional
 import torch
 
 from .. import _native
+from . import kv8
+from .kv8 import KV8Cache
 
 
 def _s(t: torch.Tensor) -> int:
@@ -49,6 +51,60 @@ def qk_norm_rope_kv(qkv: torch.Tensor, nq: int, nkv: int, pos: torch.Tensor, slo
         qkv.data_ptr(), qkv.stride(0), t, nq, nkv, 128, pos.data_ptr(), slots.data_ptr(), _p(q_norm), _p(k_norm),
         float(eps), cos_sin.data_ptr(), q_out.data_ptr(), cache.data_ptr(), _p(rows), _p(check), _s(qkv)),
         "qk_norm_rope_kv")
+    return q_out
+
+
+def qk_norm_rope_kv8(qkv: torch.Tensor, nq: int, nkv: int, pos: torch.Tensor, slots: torch.Tensor,
+                     q_norm: Optional[torch.Tensor], k_norm: Optional[torch.Tensor], eps: float,
+                     cos_sin: Optional[torch.Tensor], q_out: torch.Tensor, cache: KV8Cache, interleaved: bool = False,
+                     rows: Optional[torch.Tensor] = None, check: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """qk_norm_rope_kv into a cache of 8 bits (`kv8.KV8Cache`, one layer): split the fused QKV projection (T, (nq +
+    2 nkv) * 128), normalise q and k per head (where a weight is given), rotate them, q -> q_out (T, nq, 128), k and v
+    -> the cache at `slots` (int64 block * 16 + place; negative: q only). All in fp32, each output rounded once.
+
+    cos_sin: (positions, rotary / 2, 2) fp32 from `rope_table(positions, rotary, ...)`; the first `rotary` dims of a
+    head (a multiple of 8) are rotated: dim i with dim i + rotary / 2, or, `interleaved`, dims 2i and 2i + 1. None: no
+    rotation.
+
+    The tokens that a call writes to one page are adjacent rows in increasing places, as a prompt's or a step's are.
+    What the page held before the first of them is kept, at the page's new scale; what it held behind them is dead.
+    A token whose slot lies outside the cache, or whose position lies outside the table, is not stored, and its row of
+    q_out is NaN. With `check` (a state row) and `rows`: the sampled tokens are recomputed and compared with q_out and
+    the cache instead of written; this holds until a later call raises the scale of their page."""
+    t = qkv.shape[0]
+    heads = nq + 2 * nkv
+    dev = cache.codes.device
+    if cache.codes.dim() != 5 or cache.nkv != nkv:
+        raise ValueError(f"cache must be one layer with {nkv} kv heads, got {tuple(cache.codes.shape)}")
+    if qkv.dim() != 2 or qkv.shape[1] != heads * 128 or qkv.dtype != torch.bfloat16 or qkv.stride(1) != 1 \
+            or (t > 1 and qkv.stride(0) % 4) or qkv.data_ptr() % 8:
+        raise ValueError(f"qkv must be bf16 (T, {heads * 128}) with contiguous rows on 8-byte boundaries")
+    if q_out.shape != (t, nq, 128) or q_out.dtype != torch.bfloat16 or not q_out.is_contiguous() \
+            or q_out.data_ptr() % 8:
+        raise ValueError(f"q_out must be contiguous bf16 ({t}, {nq}, 128)")
+    kv8.want(pos, torch.int32, (t,), dev, "pos")
+    kv8.want(slots, torch.int64, (t,), dev, "slots")
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is not None:
+            kv8.want(w, torch.bfloat16, (128,), dev, name, align=8)
+    table_rows = rotary = 0
+    if cos_sin is not None:
+        table_rows, rotary = cos_sin.shape[0], 2 * cos_sin.shape[1]
+        kv8.want(cos_sin, torch.float32, (table_rows, rotary // 2, 2), dev, "cos_sin", align=16)
+        if rotary % 8 or not 0 < rotary <= 128:
+            raise ValueError(f"{rotary} rotated dims: a multiple of 8, at most 128")
+    if (rows is None) != (check is None):
+        raise ValueError("rows and check go together")
+    if rows is not None:
+        kv8.want(rows, torch.int32, (rows.shape[0],), dev, "rows")
+    if qkv.device != dev or q_out.device != dev:
+        raise ValueError("qkv, q_out and the cache must be on one device")
+    with kv8.on(dev):
+        _native.check(_native.lib().sdc_kv8_append(
+            qkv.data_ptr(), qkv.stride(0) if t > 1 else heads * 128, t, nq, nkv, pos.data_ptr(), slots.data_ptr(),
+            _p(q_norm), _p(k_norm), float(eps), _p(cos_sin), table_rows, rotary, int(interleaved), q_out.data_ptr(),
+            cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, _p(rows),
+            0 if rows is None else rows.shape[0], _p(check), _s(qkv)), "qk_norm_rope_kv8")
     return q_out
 
 

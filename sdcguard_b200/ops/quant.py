@@ -40,9 +40,10 @@ from typing import Optional
 import torch
 
 from .. import _native
-from . import gemm
+from . import gemm, kv8
 
 
+MATVEC_ROWS = 32
 ZERO_MODES = ("subtract", "fma", "two_roundings")
 
 
@@ -148,6 +149,48 @@ class QuantWeights:
         z = (self.zeros.cpu().double().repeat_interleave(self.group, dim=1) if self.zeros is not None
              else torch.full_like(q, float(self.center)))
         return ((q - z) * s).to(torch.bfloat16).double()
+
+    def matvec(self, x: torch.Tensor, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+               blocks: Optional[torch.Tensor] = None, check: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x W^T (+ bias) for up to 32 rows x (m, k) bf16, read from the 4-bit codes (`csrc/matvec4.cu`): W is the
+        effective weight of `zero_mode`, bit for bit, sums and bias (fp32 [n]) in fp32, one rounding to bf16. Bound by
+        the codes' bytes, a quarter of the bf16 matrix. k and the group are multiples of 32.
+
+        With `check` (a state row) and `blocks` (int32 indices of 16 outputs each): those outputs are recomputed and
+        compared with `out` (the call's result), bit for bit, instead of written."""
+        dev, m = self.codes.device, x.shape[0]
+        if self.bits != 4 or self.group % 32:
+            raise ValueError("matvec reads INT4 codes with groups of a multiple of 32")
+        if not self.codes.is_cuda or not self.codes.is_contiguous() or self.codes.data_ptr() % 16:
+            raise ValueError("the codes must be contiguous on a GPU")
+        if x.dim() != 2 or x.shape[1] != self.k or x.dtype != torch.bfloat16 or x.device != dev or x.stride(1) != 1 \
+                or (m > 1 and x.stride(0) % 8) or x.data_ptr() % 16:
+            raise ValueError(f"x must be bf16 (m, {self.k}) on {dev} with contiguous rows on 16-byte boundaries")
+        if m > MATVEC_ROWS:
+            raise ValueError(f"{m} rows: matvec takes up to {MATVEC_ROWS} (more go to the GEMM on the effective weights)")
+        ng = self.k // self.group
+        kv8.want(self.scales, torch.bfloat16, (self.n, ng), dev, "scales")
+        if self.zeros is not None:
+            kv8.want(self.zeros, torch.uint8, (self.n, ng), dev, "zeros")
+        if bias is not None:
+            kv8.want(bias, torch.float32, (self.n,), dev, "bias")
+        if out is None:
+            out = torch.empty(m, self.n, dtype=torch.bfloat16, device=dev)
+        elif out.shape != (m, self.n) or out.dtype != torch.bfloat16 or out.device != dev or out.stride(1) != 1:
+            raise ValueError(f"out must be bf16 ({m}, {self.n}) on {dev} with contiguous rows")
+        if (blocks is None) != (check is None):
+            raise ValueError("blocks and check go together")
+        if blocks is not None:
+            kv8.want(blocks, torch.int32, (blocks.shape[0],), dev, "blocks")
+        mode = 0 if self.zeros is None else ZERO_MODES.index(self.zero_mode)
+        with kv8.on(dev):
+            _native.check(_native.lib().sdc_matvec4(
+                x.data_ptr(), x.stride(0) if m > 1 else self.k, m, self.n, self.k, self.group, self.codes.data_ptr(),
+                self.scales.data_ptr(), None if self.zeros is None else self.zeros.data_ptr(), mode,
+                None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0) if m > 1 else self.n,
+                None if blocks is None else blocks.data_ptr(), 0 if blocks is None else blocks.shape[0],
+                None if check is None else check.data_ptr(), torch.cuda.current_stream(dev).cuda_stream), "matvec4")
+        return out
 
     def fingerprint(self) -> torch.Tensor:
         from .fingerprint import fingerprint

@@ -55,6 +55,7 @@ L = c_longlong
 U = c_uint
 U64 = ctypes.c_ulonglong
 F = c_float
+DBL = ctypes.c_double
 
 # name -> (restype, argtypes)
 SIGNATURES: dict[str, tuple] = {
@@ -119,7 +120,7 @@ SIGNATURES: dict[str, tuple] = {
     "sdc_dequant_weights": (I, [P, I, I, I, I, P, P, I, P, P]),
     "sdc_gemm_fp8_grouped": (I, [P, P, P, P, P, I, I, I, I, P, L, P, P, P, P, P, I, U, U, U, U, F, F, F, F, F, P, I,
                                  I, U, P]),
-    "sdc_kv8_append": (I, [P, L, I, I, I, P, P, P, P, F, P, I, I, I, P, P, P, L, P, I, P, P]),
+    "sdc_kv8_append": (I, [P, L, I, I, I, P, P, P, P, DBL, P, I, I, I, P, P, P, L, P, I, P, P]),
     "sdc_kv8_expand": (I, [P, P, L, P, I, I, P, P, P, I, I, I, I, P, P]),
     "sdc_kv8_decode": (I, [P, P, P, P, L, P, I, I, L, P, P, P, I, I, I, I, I, I, F, P, P, P, P]),
     "sdc_matvec4": (I, [P, L, I, I, I, I, P, P, P, I, P, P, L, P, I, P, P]),

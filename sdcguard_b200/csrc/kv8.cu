@@ -60,7 +60,8 @@ __device__ __forceinline__ float scale_of(float amax) {
   e = e < -60 ? -60 : e;
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
-__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+constexpr float FLOAT_MAX = 3.402823466e38f;
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= FLOAT_MAX; }
 
 struct AppendParams {
   const __nv_bfloat16* qkv;   // [T] rows of (nq + 2 nkv) x 128, `ld` apart
@@ -70,18 +71,20 @@ struct AppendParams {
   const long long* slots;     // [T] block * 16 + place; negative: not stored
   const __nv_bfloat16* qw;
   const __nv_bfloat16* kw;
-  float eps;
+  double eps;
   const float2* cs;           // [table_rows][rotary / 2] (cos, sin)
-  int table_rows, rotary, interleaved;
+  int table_rows, rotary;
   __nv_bfloat16* q_out;       // [T][nq][128]
   uint8_t* codes;
   float* scales;
   long long capacity;         // num_blocks * 16
   const int* rows;            // check mode: the sampled tokens
-  int nrows;
   unsigned long long* check;
 };
 
+__device__ __forceinline__ const float2* angles_of(const AppendParams& p, int pos) {
+  return p.cs + static_cast<long long>(pos) * (p.rotary / 2);
+}
 // The slot token t is stored at; -1: skipped; -2: its slot or position lies outside the cache or the table.
 __device__ __forceinline__ long long slot_of(const AppendParams& p, int t) {
   const long long s = p.slots[t];
@@ -93,107 +96,223 @@ __device__ __forceinline__ long long slot_of(const AppendParams& p, int t) {
   return s < 0 ? -1 : s;
 }
 
-// Lane l owns dims 4l .. 4l + 3 of the head. Norm (when w is given) and rotation, in fp32.
-__device__ __forceinline__ void norm_rotate(const AppendParams& p, float (&v)[4], const __nv_bfloat16* w, bool rotate,
-                                            int t, int lane) {
-  if (w != nullptr) {
-    const float ss = warp_sum(fmaf(v[0], v[0], fmaf(v[1], v[1], fmaf(v[2], v[2], v[3] * v[3]))));
-    const float inv = rsqrtf(ss / static_cast<float>(D) + p.eps);
-    const uint2 u = *reinterpret_cast<const uint2*>(w + 4 * lane);
-    const float2 w0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
-    const float2 w1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
-    v[0] *= inv * w0.x;
-    v[1] *= inv * w0.y;
-    v[2] *= inv * w1.x;
-    v[3] *= inv * w1.y;
-  }
-  if (!rotate || p.rotary == 0) return;
-  const int half = p.rotary / 2;
-  const float2* cs = p.cs + static_cast<long long>(p.pos[t]) * half;
-  if (p.interleaved) {
-    if (4 * lane < p.rotary) {
-      const float4 c = *reinterpret_cast<const float4*>(cs + 2 * lane);     // pairs (4l, 4l + 1), (4l + 2, 4l + 3)
-      const float a0 = v[0], b0 = v[1], a1 = v[2], b1 = v[3];
-      v[0] = a0 * c.x - b0 * c.y;
-      v[1] = b0 * c.x + a0 * c.y;
-      v[2] = a1 * c.z - b1 * c.w;
-      v[3] = b1 * c.z + a1 * c.w;
+// How the 16 lanes of a half warp share a row: a lane holds two quads of dims, v[0..3] and v[4..7], such that v[i] and
+// v[4 + i] are a rotation's pair, so no value crosses lanes. Halves: quads 4l and rotary / 2 + 4l, and behind the
+// rotated part two neighbouring quads. Interleaved (INTER): dims 8l .. 8l + 7, the even ones in v[0..3].
+template <bool INTER>
+struct RowLane {
+  int d0, d1, ci;      // dims of the two quads in memory, first (cos, sin) of the lane
+  bool rot;
+  __device__ __forceinline__ RowLane(int l, int rotary) {
+    const int half = rotary / 2;
+    ci = 4 * l;
+    if (INTER) {
+      d0 = 8 * l;
+      d1 = d0 + 4;
+      rot = d0 < rotary;
+    } else {
+      rot = 4 * l < half;
+      d0 = rot ? 4 * l : rotary + 8 * (l - half / 4);
+      d1 = rot ? half + 4 * l : d0 + 4;
     }
-    return;
   }
-  // halves: dim i pairs with i + half; half is a multiple of 4, so the partner dims are another lane's four
-  const bool low = 4 * lane < half, in = 4 * lane < p.rotary;
-  const int other = in ? (low ? lane + half / 4 : lane - half / 4) : lane;
-  float o[4];
+  __device__ __forceinline__ uint4 load(const __nv_bfloat16* row) const {
+    const uint2 a = *reinterpret_cast<const uint2*>(row + d0), b = *reinterpret_cast<const uint2*>(row + d1);
+    return make_uint4(a.x, a.y, b.x, b.y);
+  }
+  __device__ __forceinline__ void unpack(const uint4& u, float (&v)[8]) const {
+    uint4 w = u;
+    if (INTER)
+      w = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.z, u.w, 0x5410), __byte_perm(u.x, u.y, 0x7632),
+                     __byte_perm(u.z, u.w, 0x7632));
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = __shfl_sync(0xffffffffu, v[i], other);
-  if (in) {
-    const float4* c = reinterpret_cast<const float4*>(cs + (low ? 4 * lane : 4 * lane - half));
-    const float4 c0 = c[0], c1 = c[1];
-    const float co[4] = {c0.x, c0.z, c1.x, c1.z}, si[4] = {c0.y, c0.w, c1.y, c1.w};
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(x[i] << 16);
+      v[2 * i + 1] = __uint_as_float(x[i] & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ uint4 pack(const float (&v)[8]) const {
+    if (INTER)
+      return make_uint4(pack_bf16x2(v[0], v[4]), pack_bf16x2(v[1], v[5]), pack_bf16x2(v[2], v[6]), pack_bf16x2(v[3], v[7]));
+    return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  }
+  // The lane's cosines and sines from its position's row of the table.
+  __device__ __forceinline__ void angles(const float2* cs, float (&c)[8]) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = low ? v[i] * co[i] - o[i] * si[i] : v[i] * co[i] + o[i] * si[i];
+    for (int i = 0; i < 8; ++i) c[i] = i < 4 ? 1.f : 0.f;
+    if (!rot) return;
+    const float4* a = reinterpret_cast<const float4*>(cs + ci);
+    const float4 x = __ldg(a), y = __ldg(a + 1);
+    c[0] = x.x;
+    c[1] = x.z;
+    c[2] = y.x;
+    c[3] = y.z;
+    c[4] = x.y;
+    c[5] = x.w;
+    c[6] = y.y;
+    c[7] = y.w;
+  }
+  // The codes of u[8] (scaled values) as the two words at d0 and d1.
+  __device__ __forceinline__ uint2 codes(const float (&u)[8]) const {
+    if (INTER)
+      return make_uint2(e4m3x2(u[0], u[4]) | (e4m3x2(u[1], u[5]) << 16), e4m3x2(u[2], u[6]) | (e4m3x2(u[3], u[7]) << 16));
+    return make_uint2(e4m3x2(u[0], u[1]) | (e4m3x2(u[2], u[3]) << 16), e4m3x2(u[4], u[5]) | (e4m3x2(u[6], u[7]) << 16));
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ T half_warp_sum(T v) {
+#pragma unroll
+  for (int m = 8; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
+
+// 1 / sqrt(mean of squares + eps) of the row a half warp holds.
+template <typename T>
+__device__ __forceinline__ T norm_of(const T (&v)[8], double eps) {
+  T ss = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
+  return rsqrt(half_warp_sum(ss) / static_cast<T>(D) + static_cast<T>(eps));
+}
+// Rotates the pairs (v[i], v[4 + i]) by c: four cosines, four sines (1 and 0 where nothing is rotated).
+template <typename T>
+__device__ __forceinline__ void rotate(T (&v)[8], const float (&c)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const T a = v[i], b = v[4 + i], co = c[i], si = c[4 + i];
+    v[i] = a * co - b * si;
+    v[4 + i] = b * co + a * si;
   }
 }
 
-__device__ __forceinline__ void unpack4(const uint2& u, float (&v)[4]) {
-  const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
-  const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
-  v[0] = a.x;
-  v[1] = a.y;
-  v[2] = b.x;
-  v[3] = b.y;
+// d * inv as the float that rounds to the same E4M3 code: cut, with the last bit set where bits were lost, so that the
+// second rounding sees on which side of a tie the value lies. Not finite (in fp32): NaN.
+__device__ __forceinline__ float to_odd(double d, double inv) {
+  if (!(fabs(d) <= FLOAT_MAX)) return __int_as_float(0x7fffffff);
+  const double u = d * inv;
+  const float f = __double2float_rz(u);
+  return static_cast<double>(f) == u ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
-
-__device__ __forceinline__ float amax_of(const float (&v)[4], float m) {
+__device__ __forceinline__ float amax_of(const float (&v)[8], float m) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 8; ++i)
     if (finite(v[i])) m = fmaxf(m, fabsf(v[i]));
   return m;
 }
-// The four codes of a lane at scale 1 / inv.
-__device__ __forceinline__ uint32_t codes_of(const float (&v)[4], float inv) {
-  float s[4];
+
+// A key's row in double, weights `kw` (or null), angles at `cs` (of its position). Calls, not inlined: they are rare,
+// and their registers are not to be held by the loops around them. Every lane of the warp takes part.
+template <bool INTER>
+__device__ __forceinline__ void exact_key(const __nv_bfloat16* row, const __nv_bfloat16* kw, const float2* cs, int rotary,
+                                          double eps, int l, double (&d)[8]) {
+  const RowLane<INTER> L(l, rotary);
+  float v[8], c[8];
+  L.unpack(L.load(row), v);
+  L.angles(cs, c);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) s[i] = finite(v[i]) ? v[i] * inv : __int_as_float(0x7fffffff);
-  return e4m3x2(s[0], s[1]) | (e4m3x2(s[2], s[3]) << 16);
+  for (int i = 0; i < 8; ++i) d[i] = v[i];
+  if (kw != nullptr) {
+    const double inv = norm_of(d, eps);
+    L.unpack(L.load(kw), v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[i] = d[i] * inv * v[i];
+  }
+  rotate(d, c);
+}
+// Its codes at scale 1 / up.
+template <bool INTER>
+__device__ __noinline__ uint2 exact_codes(const __nv_bfloat16* row, const __nv_bfloat16* kw, const float2* cs, int rotary,
+                                          double eps, int l, float up) {
+  double d[8];
+  exact_key<INTER>(row, kw, cs, rotary, eps, l, d);
+  float u[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u[i] = to_odd(d[i], up);
+  return RowLane<INTER>(l, rotary).codes(u);
+}
+// The largest finite magnitude among the lane's values, rounded up to a float.
+template <bool INTER>
+__device__ __noinline__ float exact_amax(const __nv_bfloat16* row, const __nv_bfloat16* kw, const float2* cs, int rotary,
+                                         double eps, int l) {
+  double d[8];
+  exact_key<INTER>(row, kw, cs, rotary, eps, l, d);
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (fabs(d[i]) <= FLOAT_MAX) m = fmaxf(m, __double2float_ru(fabs(d[i])));
+  return m;
 }
 
-// One warp per (group of TG consecutive tokens, head); heads [0, nq) queries, then nkv keys, then nkv values. A query
-// warp handles its group's tokens; a key or value warp handles the runs that begin in its group, so one warp alone
-// writes a page's scale and codes. TG = 1 gives a decode step a warp for every row (latency), TG = 16 gives a prefill
-// one warp for a page (16 rows in flight, no warps that find nothing to do).
-template <int TG>
-__global__ void __launch_bounds__(256) kv8_append_kernel(const AppendParams p) {
-  const int lane = threadIdx.x & 31, h = blockIdx.y * 8 + (threadIdx.x >> 5);
-  if (h >= p.nq + 2 * p.nkv) return;
-  const int t0 = blockIdx.x * TG;
-  const __nv_bfloat16* col = p.qkv + static_cast<long long>(h) * D + 4 * lane;
-  if (h < p.nq) {
-    uint2 raw[TG];
+constexpr float KEY_MARGIN = 1.9073486328125e-06f;    // 2^-19
+
+// A CTA has one of two roles, by its index. Queries: a warp takes two tokens (a row per half warp) and eight heads, so
+// the tokens' (cos, sin) are read once for eight rows, which are all in flight together. Keys and values: a warp takes
+// one head and the runs that begin among TG consecutive tokens (up to 16 rows of one page), so one warp alone writes a
+// page's scale and codes of a head; its rows stay in registers as they were read and are computed twice, for the
+// scale and for the codes. TG = 1 gives each token of a decode step its own warps (latency); TG = 16 gives a page one
+// warp and leaves none without work.
+//
+// Scales and codes are the correctly rounded ones of the formulas, so they do not depend on the order of operations
+// here (a replay, another kernel or a CPU can compare bits). Values are exact products. Keys are computed in fp32 with
+// an error below 2^-19 of the run's largest value (rsqrt 4, the norm 8.5 and the rotation 2 units of 2^-24, times the
+// length of a pair, at most sqrt(2) of that value); where a code or the scale would differ within this margin, the row
+// is computed again in double. (The norm's sum of squares is fp32: keys stay below 2^60.)
+constexpr int QH = 8;             // heads of a query warp
+constexpr int HALF = PAGE / 2;    // rows of a run that each half warp holds
+
+template <bool INTER>
+__device__ __forceinline__ void append_queries(const AppendParams& p, int group, int h0) {
+  const int lane = threadIdx.x & 31, hw = lane >> 4;
+  const int t = group * PAGE + 2 * (threadIdx.x >> 5) + hw;
+  const RowLane<INTER> L(lane & 15, p.rotary);
+  const bool in = t < p.T;
+  const __nv_bfloat16* row = p.qkv + (in ? t : 0) * p.ld + static_cast<long long>(h0) * D;
+  uint4 raw[QH];
 #pragma unroll
-    for (int j = 0; j < TG; ++j)
-      raw[j] = t0 + j < p.T ? *reinterpret_cast<const uint2*>(col + (t0 + j) * p.ld) : make_uint2(0, 0);
+  for (int j = 0; j < QH; ++j) raw[j] = in && h0 + j < p.nq ? L.load(row + j * D) : make_uint4(0, 0, 0, 0);
+  const bool out = in && slot_of(p, t) == -2;
+  float c[8] = {1.f, 1.f, 1.f, 1.f, 0.f, 0.f, 0.f, 0.f};
+  if (in && !out) L.angles(angles_of(p, p.rotary > 0 ? p.pos[t] : 0), c);
+  float w[8];
+  if (p.qw != nullptr) L.unpack(L.load(p.qw), w);
+  __nv_bfloat16* dst = p.q_out + (static_cast<long long>(in ? t : 0) * p.nq + h0) * D;
 #pragma unroll
-    for (int j = 0; j < TG; ++j) {
-      const int t = t0 + j;
-      if (t >= p.T) return;
-      float v[4];
-      unpack4(raw[j], v);
-      uint2 o = make_uint2(0x7fff7fffu, 0x7fff7fffu);     // NaN: a slot or position outside must not pass unseen
-      if (slot_of(p, t) != -2) {
-        norm_rotate(p, v, p.qw, true, t, lane);
-        o = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-      }
-      *reinterpret_cast<uint2*>(p.q_out + (static_cast<long long>(t) * p.nq + h) * D + 4 * lane) = o;
+  for (int j = 0; j < QH; ++j) {
+    float v[8];
+    L.unpack(raw[j], v);
+    if (p.qw != nullptr) {
+      const float inv = norm_of(v, p.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
     }
-    return;
+    rotate(v, c);
+    uint4 o = L.pack(v);
+    if (out) o.x = o.y = o.z = o.w = 0x7fff7fffu;         // NaN: a slot or position outside must not pass unseen
+    if (in && h0 + j < p.nq) {
+      *reinterpret_cast<uint2*>(dst + j * D + L.d0) = make_uint2(o.x, o.y);
+      *reinterpret_cast<uint2*>(dst + j * D + L.d1) = make_uint2(o.z, o.w);
+    }
   }
-  const bool is_k = h < p.nq + p.nkv;
-  const int kvh = is_k ? h - p.nq : h - p.nq - p.nkv;
+}
+
+template <int TG, bool INTER>
+__device__ __forceinline__ void append_keys_values(const AppendParams& p, int t0, int u) {
+  const int lane = threadIdx.x & 31, hw = lane >> 4, l = lane & 15;
+  const bool is_k = u < p.nkv;
+  const int kvh = is_k ? u : u - p.nkv;
+  const __nv_bfloat16* col = p.qkv + static_cast<long long>(p.nq + u) * D;
+  const RowLane<INTER> L(l, is_k ? p.rotary : 0);
+  const RowLane<false> V(l, 0);                            // dims 8l .. 8l + 7 in order
   // lane j looks at token t0 - 1 + j: the token before the group, the group, and the tokens a run may reach behind it
   const int tl = t0 - 1 + lane;
-  const long long sl = lane <= TG + PAGE - 1 && tl >= 0 && tl < p.T ? slot_of(p, tl) : -1;
+  const bool look = lane < TG + PAGE && tl >= 0 && tl < p.T;
+  const int ps = look && is_k && p.rotary > 0 ? p.pos[tl] : 0;
+  const long long sl = look ? slot_of(p, tl) : -1;
+  const bool norm = is_k && p.kw != nullptr;
+  float w[8];
+  if (norm) L.unpack(L.load(p.kw), w);
   const long long before = __shfl_up_sync(0xffffffffu, sl, 1);
   const bool follows = lane > 0 && sl >= 0 && before >= 0 && sl == before + 1 && sl % PAGE != 0;
   const uint32_t chain = __ballot_sync(0xffffffffu, follows);
@@ -204,90 +323,197 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendParams p) {
     const uint32_t rest = ~(chain >> 1 >> first);          // bit i: token first + 1 + i does not continue the run
     const int len = 1 + (rest == 0 ? 31 : __ffs(rest) - 1);   // <= 16: a run stays in its page
     const long long slot = __shfl_sync(0xffffffffu, sl, first);
-    const int t = t0 - 1 + first;
     const long long blk = slot / PAGE;
     const int at = static_cast<int>(slot % PAGE);
-    constexpr int ROWS = PAGE;
-    uint2 raw[ROWS];
-#pragma unroll
-    for (int j = 0; j < ROWS; ++j)
-      if (j < len) raw[j] = *reinterpret_cast<const uint2*>(col + (t + j) * p.ld);
-    float v[ROWS][4];
-    float m = 0.f;
-#pragma unroll
-    for (int j = 0; j < ROWS; ++j)
-      if (j < len) {
-        unpack4(raw[j], v[j]);
-        if (is_k) norm_rotate(p, v[j], p.kw, true, t + j, lane);
-        m = amax_of(v[j], m);
-      }
+    const __nv_bfloat16* rows = col + (t0 - 1 + first) * p.ld;
     float* sp = p.scales + (blk * p.nkv + kvh) * 2 + (is_k ? 0 : 1);
     const float old = at > 0 ? *sp : 0.f;
-    const float s = fmaxf(scale_of(warp_max(m)), old);
-    const float inv = 1.f / s;
-    uint8_t* page = p.codes + ((blk * 2 + (is_k ? 0 : 1)) * p.nkv + kvh) * (PAGE * D) + 4 * lane;
-    if (old < s && at > 0) {
-      const float r = old * inv;
-      for (int j = 0; j < at; ++j) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(page + j * D);
-        const float2 a = h2_to_f2(e4m3x2_to_h2(*w)), b = h2_to_f2(e4m3x2_to_h2_hi(*w));
-        *w = e4m3x2(a.x * r, a.y * r) | (e4m3x2(b.x * r, b.y * r) << 16);
+    uint8_t* page = p.codes + ((blk * 2 + (is_k ? 0 : 1)) * p.nkv + kvh) * (PAGE * D);
+    uint4 raw[HALF];
+#pragma unroll
+    for (int j = 0; j < HALF; ++j)
+      raw[j] = 2 * j + hw < len ? (is_k ? L.load(rows + (2 * j + hw) * p.ld) : V.load(rows + (2 * j + hw) * p.ld))
+                                : make_uint4(0, 0, 0, 0);
+    float m = 0.f, s;
+    if (is_k) {
+      float inv[HALF];
+#pragma unroll
+      for (int j = 0; j < HALF; ++j) {
+        inv[j] = 1.f;
+        if (2 * j < len) {                                 // (uniform) a row of zeros pairs up with the last one
+          const int pos = __shfl_sync(0xffffffffu, ps, first + min(2 * j + hw, len - 1));
+          float v[8], c[8];
+          L.unpack(raw[j], v);
+          L.angles(angles_of(p, pos), c);
+          if (norm) {
+            inv[j] = norm_of(v, p.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = v[i] * inv[j] * w[i];
+          }
+          rotate(v, c);
+          m = amax_of(v, m);
+        }
+      }
+      m = warp_max(m);
+      s = scale_of(m);
+      const bool exact = !norm && p.rotary == 0;
+      if (!exact && scale_of(m * (1.f - KEY_MARGIN)) != scale_of(m * (1.f + KEY_MARGIN))) {
+        float top = 0.f;
+#pragma unroll 1
+        for (int j = 0; 2 * j < len; ++j) {
+          const int r = min(2 * j + hw, len - 1);
+          const int pos = __shfl_sync(0xffffffffu, ps, first + r);
+          top = fmaxf(top, exact_amax<INTER>(rows + r * p.ld, p.kw, angles_of(p, pos), p.rotary, p.eps, l));
+        }
+        s = scale_of(warp_max(top));
+      }
+      s = fmaxf(s, old);
+      const float up = 1.f / s, margin = exact ? 0.f : KEY_MARGIN * m * up;
+#pragma unroll
+      for (int j = 0; j < HALF; ++j)
+        if (2 * j < len) {
+          const int r = min(2 * j + hw, len - 1);
+          const int pos = __shfl_sync(0xffffffffu, ps, first + r);
+          float v[8], c[8], hi[8];
+          L.unpack(raw[j], v);
+          L.angles(angles_of(p, pos), c);
+          if (norm) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = v[i] * inv[j] * w[i];
+          }
+          rotate(v, c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float x = finite(v[i]) ? v[i] * up : __int_as_float(0x7fffffff);
+            v[i] = x - margin;
+            hi[i] = x + margin;
+          }
+          uint2 code = L.codes(v);
+          if (!exact) {
+            const uint2 other = L.codes(hi);
+            if (__any_sync(0xffffffffu, code.x != other.x || code.y != other.y))
+              code = exact_codes<INTER>(rows + r * p.ld, p.kw, angles_of(p, pos), p.rotary, p.eps, l, up);
+          }
+          if (2 * j + hw < len) {
+            uint8_t* dst = page + (at + 2 * j + hw) * D;
+            *reinterpret_cast<uint32_t*>(dst + L.d0) = code.x;
+            *reinterpret_cast<uint32_t*>(dst + L.d1) = code.y;
+          }
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < HALF; ++j) {
+        float v[8];
+        V.unpack(raw[j], v);
+        m = amax_of(v, m);
+      }
+      s = fmaxf(scale_of(warp_max(m)), old);
+      const float up = 1.f / s;
+#pragma unroll
+      for (int j = 0; j < HALF; ++j) {
+        float v[8];
+        V.unpack(raw[j], v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = finite(v[i]) ? v[i] * up : __int_as_float(0x7fffffff);
+        if (2 * j + hw < len) *reinterpret_cast<uint2*>(page + (at + 2 * j + hw) * D + 8 * l) = V.codes(v);
       }
     }
-#pragma unroll
-    for (int j = 0; j < ROWS; ++j)
-      if (j < len) *reinterpret_cast<uint32_t*>(page + (at + j) * D) = codes_of(v[j], inv);
+    if (old < s && at > 0) {
+      const float r = old / s;
+      for (int j = 0; j < at; ++j) {
+        uint32_t* c = reinterpret_cast<uint32_t*>(page + j * D + 4 * lane);
+        const float2 a = h2_to_f2(e4m3x2_to_h2(*c)), b = h2_to_f2(e4m3x2_to_h2_hi(*c));
+        *c = e4m3x2(a.x * r, a.y * r) | (e4m3x2(b.x * r, b.y * r) << 16);
+      }
+    }
     __syncwarp();
     if (lane == 0) *sp = s;
   }
 }
 
-// Check mode: one warp per (sampled token, head) recomputes the row and compares it with what the append stored: the
-// query's bits, or the codes at the page's scale (which must cover the row). Valid until a later append moves the page.
+template <int TG, bool INTER>
+__global__ void __launch_bounds__(256, 3) kv8_append_kernel(const AppendParams p) {
+  const int per = (2 * p.nkv + 7) / 8;                     // key / value CTAs of a token group
+  const int kv_ctas = (p.T + TG - 1) / TG * per;
+  const int i = blockIdx.x;
+  if (i < kv_ctas) {
+    const int u = i % per * 8 + (threadIdx.x >> 5);
+    if (u < 2 * p.nkv) append_keys_values<TG, INTER>(p, i / per * TG, u);
+  } else {
+    const int q = (p.nq + QH - 1) / QH;
+    append_queries<INTER>(p, (i - kv_ctas) / q, (i - kv_ctas) % q * QH);
+  }
+}
+
+// Check mode: one warp per (sampled token, head) recomputes the row (keys in double: the same bits) and compares it
+// with what the append stored: the query's bits, or the codes at the page's scale, which must cover the row. Valid
+// until a later append moves the page.
+template <bool INTER>
 __global__ void __launch_bounds__(256) kv8_append_check_kernel(const AppendParams p) {
-  const int lane = threadIdx.x & 31, h = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, l = lane & 15, h = blockIdx.y * 8 + (threadIdx.x >> 5);
   const int heads = p.nq + 2 * p.nkv;
   if (h >= heads) return;
   const int t = p.rows[blockIdx.x];
   if (blockIdx.x == 0 && h == 0 && lane == 0) atomicAdd(p.check + 2, 1ull);
   if (t < 0 || t >= p.T) return;
   const long long slot = slot_of(p, t);
-  float v[4];
-  unpack4(*reinterpret_cast<const uint2*>(p.qkv + t * p.ld + static_cast<long long>(h) * D + 4 * lane), v);
-  int bad = -1;
-  if (h < p.nq) {
-    uint2 o = make_uint2(0x7fff7fffu, 0x7fff7fffu);
-    if (slot != -2) {
-      norm_rotate(p, v, p.qw, true, t, lane);
-      o = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+  const bool is_q = h < p.nq, is_k = !is_q && h < p.nq + p.nkv;
+  if (!is_q && slot < 0) return;
+  const RowLane<INTER> L(l, p.rotary);
+  const __nv_bfloat16* row = p.qkv + t * p.ld + static_cast<long long>(h) * D;
+  const __nv_bfloat16* nw = is_q ? p.qw : is_k ? p.kw : nullptr;
+  float w[8];
+  if (nw != nullptr) L.unpack(L.load(nw), w);
+  const int pos = p.rotary > 0 && slot != -2 ? p.pos[t] : 0;
+  int bad = D;                                             // the lane's first differing dim (both halves hold the row)
+  if (is_q) {
+    float v[8];
+    L.unpack(L.load(row), v);
+    float c[8];
+    L.angles(angles_of(p, pos), c);
+    if (nw != nullptr) {
+      const float inv = norm_of(v, p.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
     }
-    const uint2 have = *reinterpret_cast<const uint2*>(p.q_out + (static_cast<long long>(t) * p.nq + h) * D + 4 * lane);
-    const int d1 = bf16x2_diff(o.y, have.y), d0 = bf16x2_diff(o.x, have.x);
-    bad = d0 >= 0 ? 4 * lane + d0 : d1 >= 0 ? 4 * lane + 2 + d1 : -1;
+    rotate(v, c);
+    uint4 o = L.pack(v);
+    if (slot == -2) o.x = o.y = o.z = o.w = 0x7fff7fffu;
+    const uint4 have = L.load(p.q_out + (static_cast<long long>(t) * p.nq + h) * D);
+    const int e3 = bf16x2_diff(o.w, have.w), e2 = bf16x2_diff(o.z, have.z), e1 = bf16x2_diff(o.y, have.y),
+              e0 = bf16x2_diff(o.x, have.x);
+    bad = e0 >= 0 ? L.d0 + e0 : e1 >= 0 ? L.d0 + 2 + e1 : e2 >= 0 ? L.d1 + e2 : e3 >= 0 ? L.d1 + 2 + e3 : D;
   } else {
-    if (slot < 0) return;
-    const bool is_k = h < p.nq + p.nkv;
     const int kvh = is_k ? h - p.nq : h - p.nq - p.nkv;
-    if (is_k) norm_rotate(p, v, p.kw, true, t, lane);
     const long long blk = slot / PAGE;
     const float s = p.scales[(blk * p.nkv + kvh) * 2 + (is_k ? 0 : 1)];
-    const float need = scale_of(warp_max(amax_of(v, 0.f)));
-    const uint32_t have = *reinterpret_cast<const uint32_t*>(
-        p.codes + ((blk * 2 + (is_k ? 0 : 1)) * p.nkv + kvh) * (PAGE * D) + (slot % PAGE) * D + 4 * lane);
-    if (!(s >= need)) {
-      bad = 4 * lane;
+    float m;
+    uint2 want;
+    if (is_k) {
+      m = exact_amax<INTER>(row, nw, angles_of(p, pos), p.rotary, p.eps, l);
+      want = exact_codes<INTER>(row, nw, angles_of(p, pos), p.rotary, p.eps, l, 1.f / s);
     } else {
-      const uint32_t want = codes_of(v, 1.f / s);
+      float v[8];
+      L.unpack(L.load(row), v);
+      m = amax_of(v, 0.f);
 #pragma unroll
-      for (int i = 3; i >= 0; --i) {
-        const uint32_t a = (want >> (8 * i)) & 0xffu, b = (have >> (8 * i)) & 0xffu;
-        const bool same = a == b || ((a | b) & 0x7fu) == 0 || ((a & 0x7fu) == 0x7fu && (b & 0x7fu) == 0x7fu);
-        if (!same) bad = 4 * lane + i;
-      }
+      for (int i = 0; i < 8; ++i) v[i] = finite(v[i]) ? v[i] * (1.f / s) : __int_as_float(0x7fffffff);
+      want = L.codes(v);
+    }
+    const bool covers = s >= scale_of(warp_max(m));
+    const uint8_t* have = p.codes + ((blk * 2 + (is_k ? 0 : 1)) * p.nkv + kvh) * (PAGE * D) + (slot % PAGE) * D;
+    const uint32_t ws[2] = {want.x, want.y};
+    const uint32_t hs[2] = {*reinterpret_cast<const uint32_t*>(have + L.d0), *reinterpret_cast<const uint32_t*>(have + L.d1)};
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {
+      const uint32_t a = (ws[i >> 2] >> (8 * (i & 3))) & 0xffu, b = (hs[i >> 2] >> (8 * (i & 3))) & 0xffu;
+      const bool same = a == b || ((a | b) & 0x7fu) == 0 || ((a & 0x7fu) == 0x7fu && (b & 0x7fu) == 0x7fu);
+      if (!same || !covers) bad = (i < 4 ? L.d0 : L.d1) + (i & 3);
     }
   }
-  const unsigned who = __ballot_sync(0xffffffffu, bad >= 0);
-  if (who && lane == __ffs(who) - 1)
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) bad = min(bad, __shfl_xor_sync(0xffffffffu, bad, k));
+  if (bad < D && lane == 0)
     report_replay_mismatch(p.check, (static_cast<unsigned long long>(t) * heads + h) * D + bad);
 }
 
@@ -791,7 +1017,7 @@ using namespace sdc::kv8;
 extern "C" {
 
 int sdc_kv8_append(const void* qkv, long long ld, int T, int nq, int nkv, const int* pos, const long long* slots,
-                   const void* qw, const void* kw, float eps, const void* cos_sin, int table_rows, int rotary,
+                   const void* qw, const void* kw, double eps, const void* cos_sin, int table_rows, int rotary,
                    int interleaved, void* q_out, void* codes, void* scales, long long num_blocks, const int* rows,
                    int nrows, void* check, void* stream) {
   if (T <= 0 || (check != nullptr && nrows <= 0)) return 0;
@@ -811,19 +1037,29 @@ int sdc_kv8_append(const void* qkv, long long ld, int T, int nq, int nkv, const 
   p.cs = static_cast<const float2*>(cos_sin);
   p.table_rows = table_rows;
   p.rotary = rotary;
-  p.interleaved = interleaved;
   p.q_out = static_cast<__nv_bfloat16*>(q_out);
   p.codes = static_cast<uint8_t*>(codes);
   p.scales = static_cast<float*>(scales);
   p.capacity = num_blocks * PAGE;
   p.rows = rows;
-  p.nrows = nrows;
   p.check = static_cast<unsigned long long*>(check);
   const int gy = (nq + 2 * nkv + 7) / 8;
   auto st = static_cast<cudaStream_t>(stream);
-  if (p.check != nullptr) kv8_append_check_kernel<<<dim3(nrows, gy), 256, 0, st>>>(p);
-  else if (T < 1024) kv8_append_kernel<1><<<dim3(T, gy), 256, 0, st>>>(p);
-  else kv8_append_kernel<16><<<dim3((T + 15) / 16, gy), 256, 0, st>>>(p);
+  const int tg = T < 1024 ? 1 : PAGE;
+  const long long ctas = static_cast<long long>((T + tg - 1) / tg) * ((2 * nkv + 7) / 8) +
+                         static_cast<long long>((T + PAGE - 1) / PAGE) * ((nq + QH - 1) / QH);
+  const unsigned grid = static_cast<unsigned>(ctas);
+  const dim3 sample(nrows, gy);
+  if (p.check != nullptr) {
+    if (interleaved) kv8_append_check_kernel<true><<<sample, 256, 0, st>>>(p);
+    else kv8_append_check_kernel<false><<<sample, 256, 0, st>>>(p);
+  } else if (tg == 1) {
+    if (interleaved) kv8_append_kernel<1, true><<<grid, 256, 0, st>>>(p);
+    else kv8_append_kernel<1, false><<<grid, 256, 0, st>>>(p);
+  } else {
+    if (interleaved) kv8_append_kernel<PAGE, true><<<grid, 256, 0, st>>>(p);
+    else kv8_append_kernel<PAGE, false><<<grid, 256, 0, st>>>(p);
+  }
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -197,13 +197,17 @@ __device__ __forceinline__ float to_odd(double d, double inv) {
 }
 __device__ __forceinline__ float amax_of(const float (&v)[8], float m) {
 #pragma unroll
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));      // passes over NaN
+  return m;
+}
+__device__ __forceinline__ float finite_amax(const float (&v)[8], float m) {
+#pragma unroll
   for (int i = 0; i < 8; ++i)
     if (finite(v[i])) m = fmaxf(m, fabsf(v[i]));
   return m;
 }
 
-// A key's row in double, weights `kw` (or null), angles at `cs` (of its position). Calls, not inlined: they are rare,
-// and their registers are not to be held by the loops around them. Every lane of the warp takes part.
+// A key's row in double, weights `kw` (or null), angles at `cs` (of its position). Every lane of the warp takes part.
 template <bool INTER>
 __device__ __forceinline__ void exact_key(const __nv_bfloat16* row, const __nv_bfloat16* kw, const float2* cs, int rotary,
                                           double eps, int l, double (&d)[8]) {
@@ -223,7 +227,7 @@ __device__ __forceinline__ void exact_key(const __nv_bfloat16* row, const __nv_b
 }
 // Its codes at scale 1 / up.
 template <bool INTER>
-__device__ __noinline__ uint2 exact_codes(const __nv_bfloat16* row, const __nv_bfloat16* kw, const float2* cs, int rotary,
+__device__ __forceinline__ uint2 exact_codes(const __nv_bfloat16* row, const __nv_bfloat16* kw, const float2* cs, int rotary,
                                           double eps, int l, float up) {
   double d[8];
   exact_key<INTER>(row, kw, cs, rotary, eps, l, d);
@@ -234,7 +238,7 @@ __device__ __noinline__ uint2 exact_codes(const __nv_bfloat16* row, const __nv_b
 }
 // The largest finite magnitude among the lane's values, rounded up to a float.
 template <bool INTER>
-__device__ __noinline__ float exact_amax(const __nv_bfloat16* row, const __nv_bfloat16* kw, const float2* cs, int rotary,
+__device__ __forceinline__ float exact_amax(const __nv_bfloat16* row, const __nv_bfloat16* kw, const float2* cs, int rotary,
                                          double eps, int l) {
   double d[8];
   exact_key<INTER>(row, kw, cs, rotary, eps, l, d);
@@ -245,27 +249,28 @@ __device__ __noinline__ float exact_amax(const __nv_bfloat16* row, const __nv_bf
   return m;
 }
 
-constexpr float KEY_MARGIN = 1.9073486328125e-06f;    // 2^-19
-
 // A CTA has one of two roles, by its index. Queries: a warp takes two tokens (a row per half warp) and eight heads, so
 // the tokens' (cos, sin) are read once for eight rows, which are all in flight together. Keys and values: a warp takes
 // one head and the runs that begin among TG consecutive tokens (up to 16 rows of one page), so one warp alone writes a
-// page's scale and codes of a head; its rows stay in registers as they were read and are computed twice, for the
-// scale and for the codes. TG = 1 gives each token of a decode step its own warps (latency); TG = 16 gives a page one
-// warp and leaves none without work.
+// page's scale and codes of a head; keys wait for the scale in shared memory, values as they were read in registers.
+// TG = 1 gives each token of a decode step its own warps (latency); TG = 16 gives a page one warp and leaves none
+// without work.
 //
 // Scales and codes are the correctly rounded ones of the formulas, so they do not depend on the order of operations
-// here (a replay, another kernel or a CPU can compare bits). Values are exact products. Keys are computed in fp32 with
-// an error below 2^-19 of the run's largest value (rsqrt 4, the norm 8.5 and the rotation 2 units of 2^-24, times the
-// length of a pair, at most sqrt(2) of that value); where a code or the scale would differ within this margin, the row
-// is computed again in double. (The norm's sum of squares is fp32: keys stay below 2^60.)
+// here (a replay, another kernel or a CPU can compare bits). Values are exact products. Keys are computed in fp32; with
+// u = 2^-24, the norm's factor errs by 10.5 u of itself (rsqrt 4, the sum of squares and its root 6.5), the products
+// with it and the rotation by 4 u of the pair's length, at most sqrt(2) of the run's largest magnitude. Where a code
+// differs within 11 u of the key plus 6 u of that magnitude, or the scale within 2^-19, the row is computed again in
+// double: one pair of rows in thirty. (The sum of squares is fp32: keys stay below 2^60.)
+constexpr float KEY_RELATIVE = 11.f / 16777216.f, KEY_ABSOLUTE = 6.f / 16777216.f, SCALE_MARGIN = 32.f / 16777216.f;
+constexpr int AW = 4;             // warps of a CTA
 constexpr int QH = 8;             // heads of a query warp
 constexpr int HALF = PAGE / 2;    // rows of a run that each half warp holds
 
 template <bool INTER>
 __device__ __forceinline__ void append_queries(const AppendParams& p, int group, int h0) {
   const int lane = threadIdx.x & 31, hw = lane >> 4;
-  const int t = group * PAGE + 2 * (threadIdx.x >> 5) + hw;
+  const int t = 2 * (group * AW + (threadIdx.x >> 5)) + hw;
   const RowLane<INTER> L(lane & 15, p.rotary);
   const bool in = t < p.T;
   const __nv_bfloat16* row = p.qkv + (in ? t : 0) * p.ld + static_cast<long long>(h0) * D;
@@ -275,11 +280,16 @@ __device__ __forceinline__ void append_queries(const AppendParams& p, int group,
   const bool out = in && slot_of(p, t) == -2;
   float c[8] = {1.f, 1.f, 1.f, 1.f, 0.f, 0.f, 0.f, 0.f};
   if (in && !out) L.angles(angles_of(p, p.rotary > 0 ? p.pos[t] : 0), c);
+  if (out) {                                              // a slot or position outside must not pass unseen
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = __int_as_float(0x7fffffff);
+  }
   float w[8];
   if (p.qw != nullptr) L.unpack(L.load(p.qw), w);
   __nv_bfloat16* dst = p.q_out + (static_cast<long long>(in ? t : 0) * p.nq + h0) * D;
 #pragma unroll
   for (int j = 0; j < QH; ++j) {
+    if (h0 + j >= p.nq) break;
     float v[8];
     L.unpack(raw[j], v);
     if (p.qw != nullptr) {
@@ -288,9 +298,8 @@ __device__ __forceinline__ void append_queries(const AppendParams& p, int group,
       for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
     }
     rotate(v, c);
-    uint4 o = L.pack(v);
-    if (out) o.x = o.y = o.z = o.w = 0x7fff7fffu;         // NaN: a slot or position outside must not pass unseen
-    if (in && h0 + j < p.nq) {
+    const uint4 o = L.pack(v);
+    if (in) {
       *reinterpret_cast<uint2*>(dst + j * D + L.d0) = make_uint2(o.x, o.y);
       *reinterpret_cast<uint2*>(dst + j * D + L.d1) = make_uint2(o.z, o.w);
     }
@@ -298,12 +307,12 @@ __device__ __forceinline__ void append_queries(const AppendParams& p, int group,
 }
 
 template <int TG, bool INTER>
-__device__ __forceinline__ void append_keys_values(const AppendParams& p, int t0, int u) {
+__device__ __forceinline__ void append_keys_values(const AppendParams& p, int t0, int u, float4 (*keep)[2][32]) {
   const int lane = threadIdx.x & 31, hw = lane >> 4, l = lane & 15;
   const bool is_k = u < p.nkv;
   const int kvh = is_k ? u : u - p.nkv;
   const __nv_bfloat16* col = p.qkv + static_cast<long long>(p.nq + u) * D;
-  const RowLane<INTER> L(l, is_k ? p.rotary : 0);
+  const RowLane<INTER> L(l, p.rotary);
   const RowLane<false> V(l, 0);                            // dims 8l .. 8l + 7 in order
   // lane j looks at token t0 - 1 + j: the token before the group, the group, and the tokens a run may reach behind it
   const int tl = t0 - 1 + lane;
@@ -329,94 +338,123 @@ __device__ __forceinline__ void append_keys_values(const AppendParams& p, int t0
     float* sp = p.scales + (blk * p.nkv + kvh) * 2 + (is_k ? 0 : 1);
     const float old = at > 0 ? *sp : 0.f;
     uint8_t* page = p.codes + ((blk * 2 + (is_k ? 0 : 1)) * p.nkv + kvh) * (PAGE * D);
-    uint4 raw[HALF];
-#pragma unroll
-    for (int j = 0; j < HALF; ++j)
-      raw[j] = 2 * j + hw < len ? (is_k ? L.load(rows + (2 * j + hw) * p.ld) : V.load(rows + (2 * j + hw) * p.ld))
-                                : make_uint4(0, 0, 0, 0);
     float m = 0.f, s;
     if (is_k) {
-      float inv[HALF];
+      const auto place = [&](int j) { return min(2 * j + hw, len - 1); };   // a row of zeros pairs up with the last one
+#pragma unroll 1
+      for (int j0 = 0; 2 * j0 < len; j0 += 4) {
+        uint4 raw[4];
 #pragma unroll
-      for (int j = 0; j < HALF; ++j) {
-        inv[j] = 1.f;
-        if (2 * j < len) {                                 // (uniform) a row of zeros pairs up with the last one
-          const int pos = __shfl_sync(0xffffffffu, ps, first + min(2 * j + hw, len - 1));
+        for (int j = 0; j < 4; ++j)
+          raw[j] = 2 * (j0 + j) + hw < len ? L.load(rows + (2 * (j0 + j) + hw) * p.ld) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (2 * (j0 + j) >= len) break;                  // (uniform)
+          const int pos = __shfl_sync(0xffffffffu, ps, first + place(j0 + j));
           float v[8], c[8];
           L.unpack(raw[j], v);
           L.angles(angles_of(p, pos), c);
           if (norm) {
-            inv[j] = norm_of(v, p.eps);
+            const float inv = norm_of(v, p.eps);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = v[i] * inv[j] * w[i];
+            for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
           }
           rotate(v, c);
           m = amax_of(v, m);
+          keep[j0 + j][0][lane] = make_float4(v[0], v[1], v[2], v[3]);
+          keep[j0 + j][1][lane] = make_float4(v[4], v[5], v[6], v[7]);
         }
       }
       m = warp_max(m);
+      const bool inf = m > FLOAT_MAX;                      // then the largest finite one
+      if (inf) {
+        m = 0.f;
+        for (int j = 0; 2 * j < len; ++j) {
+          const float4 a = keep[j][0][lane], b = keep[j][1][lane];
+          const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+          m = finite_amax(v, m);
+        }
+        m = warp_max(m);
+      }
       s = scale_of(m);
       const bool exact = !norm && p.rotary == 0;
-      if (!exact && scale_of(m * (1.f - KEY_MARGIN)) != scale_of(m * (1.f + KEY_MARGIN))) {
+      if (!exact && scale_of(m * (1.f - SCALE_MARGIN)) != scale_of(m * (1.f + SCALE_MARGIN))) {
         float top = 0.f;
-#pragma unroll 1
         for (int j = 0; 2 * j < len; ++j) {
-          const int r = min(2 * j + hw, len - 1);
-          const int pos = __shfl_sync(0xffffffffu, ps, first + r);
-          top = fmaxf(top, exact_amax<INTER>(rows + r * p.ld, p.kw, angles_of(p, pos), p.rotary, p.eps, l));
+          const int pos = __shfl_sync(0xffffffffu, ps, first + place(j));
+          top = fmaxf(top, exact_amax<INTER>(rows + place(j) * p.ld, p.kw, angles_of(p, pos), p.rotary, p.eps, l));
         }
         s = scale_of(warp_max(top));
       }
       s = fmaxf(s, old);
-      const float up = 1.f / s, margin = exact ? 0.f : KEY_MARGIN * m * up;
-#pragma unroll
-      for (int j = 0; j < HALF; ++j)
-        if (2 * j < len) {
-          const int r = min(2 * j + hw, len - 1);
-          const int pos = __shfl_sync(0xffffffffu, ps, first + r);
-          float v[8], c[8], hi[8];
-          L.unpack(raw[j], v);
-          L.angles(angles_of(p, pos), c);
-          if (norm) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = v[i] * inv[j] * w[i];
-          }
-          rotate(v, c);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float x = finite(v[i]) ? v[i] * up : __int_as_float(0x7fffffff);
-            v[i] = x - margin;
-            hi[i] = x + margin;
-          }
-          uint2 code = L.codes(v);
-          if (!exact) {
-            const uint2 other = L.codes(hi);
-            if (__any_sync(0xffffffffu, code.x != other.x || code.y != other.y))
-              code = exact_codes<INTER>(rows + r * p.ld, p.kw, angles_of(p, pos), p.rotary, p.eps, l, up);
-          }
-          if (2 * j + hw < len) {
-            uint8_t* dst = page + (at + 2 * j + hw) * D;
-            *reinterpret_cast<uint32_t*>(dst + L.d0) = code.x;
-            *reinterpret_cast<uint32_t*>(dst + L.d1) = code.y;
-          }
-        }
-    } else {
-#pragma unroll
-      for (int j = 0; j < HALF; ++j) {
-        float v[8];
-        V.unpack(raw[j], v);
-        m = amax_of(v, m);
-      }
-      s = fmaxf(scale_of(warp_max(m)), old);
       const float up = 1.f / s;
+      const float far = exact ? 0.f : KEY_ABSOLUTE * m * up;
+      const float up1 = exact ? up : up * (1.f + KEY_RELATIVE), up0 = exact ? up : up * (1.f - KEY_RELATIVE);
+#pragma unroll 2
+      for (int j = 0; 2 * j < len; ++j) {
+        const float4 a = keep[j][0][lane], b = keep[j][1][lane];
+        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        float x[8], y[8];                                // the ends of the interval around the scaled key
 #pragma unroll
-      for (int j = 0; j < HALF; ++j) {
+        for (int i = 0; i < 8; ++i) {
+          const float f = copysignf(far, v[i]);
+          x[i] = fmaf(v[i], up1, f);
+          y[i] = fmaf(v[i], up0, -f);
+        }
+        uint2 code = L.codes(x);
+        const uint2 other = L.codes(y);
+        if (__any_sync(0xffffffffu, code.x != other.x || code.y != other.y || inf)) {
+          const int pos = __shfl_sync(0xffffffffu, ps, first + place(j));
+          code = exact_codes<INTER>(rows + place(j) * p.ld, p.kw, angles_of(p, pos), p.rotary, p.eps, l, up);
+        }
+        if (2 * j + hw < len) {
+          uint8_t* dst = page + (at + 2 * j + hw) * D;
+          *reinterpret_cast<uint32_t*>(dst + L.d0) = code.x;
+          *reinterpret_cast<uint32_t*>(dst + L.d1) = code.y;
+        }
+      }
+      __syncwarp();
+    } else {
+#pragma unroll 1
+      for (int j0 = 0; 2 * j0 < len; j0 += 4) {
+        uint4 raw[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          raw[j] = 2 * (j0 + j) + hw < len ? V.load(rows + (2 * (j0 + j) + hw) * p.ld) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float v[8];
+          V.unpack(raw[j], v);
+          m = amax_of(v, m);
+          *reinterpret_cast<uint4*>(&keep[j0 + j][0][lane]) = raw[j];
+        }
+      }
+      m = warp_max(m);
+      const bool inf = m > FLOAT_MAX;                      // then the largest finite one
+      if (inf) {
+        m = 0.f;
+        for (int j = 0; 2 * j < len; ++j) {
+          float v[8];
+          V.unpack(*reinterpret_cast<const uint4*>(&keep[j][0][lane]), v);
+          m = finite_amax(v, m);
+        }
+        m = warp_max(m);
+      }
+      s = fmaxf(scale_of(m), old);
+      const float up = 1.f / s;
+#pragma unroll 2
+      for (int j = 0; 2 * j < len; ++j) {
         float v[8];
-        V.unpack(raw[j], v);
+        V.unpack(*reinterpret_cast<const uint4*>(&keep[j][0][lane]), v);
+        if (inf) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = finite(v[i]) ? v[i] * up : __int_as_float(0x7fffffff);
+          for (int i = 0; i < 8; ++i) v[i] = finite(v[i]) ? v[i] : __int_as_float(0x7fffffff);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= up;
         if (2 * j + hw < len) *reinterpret_cast<uint2*>(page + (at + 2 * j + hw) * D + 8 * l) = V.codes(v);
       }
+      __syncwarp();
     }
     if (old < s && at > 0) {
       const float r = old / s;
@@ -432,13 +470,14 @@ __device__ __forceinline__ void append_keys_values(const AppendParams& p, int t0
 }
 
 template <int TG, bool INTER>
-__global__ void __launch_bounds__(256, 3) kv8_append_kernel(const AppendParams p) {
-  const int per = (2 * p.nkv + 7) / 8;                     // key / value CTAs of a token group
+__global__ void __launch_bounds__(AW * 32, 5) kv8_append_kernel(const AppendParams p) {
+  __shared__ float4 keep[AW][HALF][2][32];
+  const int per = (2 * p.nkv + AW - 1) / AW;               // key / value CTAs of a token group
   const int kv_ctas = (p.T + TG - 1) / TG * per;
   const int i = blockIdx.x;
   if (i < kv_ctas) {
-    const int u = i % per * 8 + (threadIdx.x >> 5);
-    if (u < 2 * p.nkv) append_keys_values<TG, INTER>(p, i / per * TG, u);
+    const int u = i % per * AW + (threadIdx.x >> 5);
+    if (u < 2 * p.nkv) append_keys_values<TG, INTER>(p, i / per * TG, u, keep[threadIdx.x >> 5]);
   } else {
     const int q = (p.nq + QH - 1) / QH;
     append_queries<INTER>(p, (i - kv_ctas) / q, (i - kv_ctas) % q * QH);
@@ -495,7 +534,7 @@ __global__ void __launch_bounds__(256) kv8_append_check_kernel(const AppendParam
     } else {
       float v[8];
       L.unpack(L.load(row), v);
-      m = amax_of(v, 0.f);
+      m = finite_amax(v, 0.f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = finite(v[i]) ? v[i] * (1.f / s) : __int_as_float(0x7fffffff);
       want = L.codes(v);
@@ -1046,19 +1085,19 @@ int sdc_kv8_append(const void* qkv, long long ld, int T, int nq, int nkv, const 
   const int gy = (nq + 2 * nkv + 7) / 8;
   auto st = static_cast<cudaStream_t>(stream);
   const int tg = T < 1024 ? 1 : PAGE;
-  const long long ctas = static_cast<long long>((T + tg - 1) / tg) * ((2 * nkv + 7) / 8) +
-                         static_cast<long long>((T + PAGE - 1) / PAGE) * ((nq + QH - 1) / QH);
+  const long long ctas = static_cast<long long>((T + tg - 1) / tg) * ((2 * nkv + AW - 1) / AW) +
+                         static_cast<long long>((T + 2 * AW - 1) / (2 * AW)) * ((nq + QH - 1) / QH);
   const unsigned grid = static_cast<unsigned>(ctas);
   const dim3 sample(nrows, gy);
   if (p.check != nullptr) {
     if (interleaved) kv8_append_check_kernel<true><<<sample, 256, 0, st>>>(p);
     else kv8_append_check_kernel<false><<<sample, 256, 0, st>>>(p);
   } else if (tg == 1) {
-    if (interleaved) kv8_append_kernel<1, true><<<grid, 256, 0, st>>>(p);
-    else kv8_append_kernel<1, false><<<grid, 256, 0, st>>>(p);
+    if (interleaved) kv8_append_kernel<1, true><<<grid, AW * 32, 0, st>>>(p);
+    else kv8_append_kernel<1, false><<<grid, AW * 32, 0, st>>>(p);
   } else {
-    if (interleaved) kv8_append_kernel<PAGE, true><<<grid, 256, 0, st>>>(p);
-    else kv8_append_kernel<PAGE, false><<<grid, 256, 0, st>>>(p);
+    if (interleaved) kv8_append_kernel<PAGE, true><<<grid, AW * 32, 0, st>>>(p);
+    else kv8_append_kernel<PAGE, false><<<grid, AW * 32, 0, st>>>(p);
   }
   return static_cast<int>(cudaGetLastError());
 }

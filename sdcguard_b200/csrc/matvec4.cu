@@ -6,24 +6,24 @@
 // rnd rounds to bf16: the effective weights of csrc/quant.cu bit for bit, so the products are those of the layer's
 // arithmetic whichever kernel serves it. Sums in fp32, one rounding of y to bf16.
 //
-// Bound by the codes' bytes (N K / 2), so the work per code is what is counted. A code becomes bf16 by its bits:
-// 0x4300 | q is 128 + q exactly, less (128 + z) is q - z exactly, times s is W with its one rounding: 7.5 instructions
-// for 4 pairs of weights, then one mma.m16n8k16 (A = W: 16 outputs, B = x^T: 8 rows of x) takes 8 weights of each
-// lane. The order of k within a product is free, so a lane takes 16 bytes (32 weights) of a row as they lie in memory,
-// pairs (i, i + 4) of each word as they come out of the nibbles, and reads x in the same order.
+// Bound by the codes' bytes (N K / 2) and, next to them, by the instructions per code: codes become bf16 weights in
+// pairs without a conversion (see `weights`), then one mma.m16n8k16 (A = W: 16 outputs, B = x^T: 8 rows of x) takes 8
+// weights of each lane. The order of k within a product is free, so a lane takes 16 bytes (32 weights) of a row as they
+// lie in memory, pairs (i, i + 4) of each word as masks give them, and reads x in the same order.
 //
-// A CTA of 8 warps computes 16 MT outputs; its warps take every 8th block of 128 k and merge in warp order. Each
-// output's arithmetic depends on its codes and x's row alone (not on M, MT or the CTA), so running some blocks of 16
-// outputs again gives the same bits: check mode compares them with y.
+// The k blocks (128 each) of an output go to 8 slices in turn, which merge in order at the end; a CTA of WARPS warps
+// computes 16 MT outputs, its warp w the slices w, w + WARPS, ... Each output's arithmetic depends on its codes and x's
+// row alone (not on M, MT, WARPS or the CTA), so a row of x gives the same bits in any batch, and running some blocks of
+// 16 outputs again gives them too: check mode compares them with y.
 #include "common.cuh"
 
 namespace sdc {
 namespace matvec4 {
 
-constexpr int WARPS = 8;
-constexpr int KB = 128;       // k per warp step: 4 lanes x 32
+constexpr int SLICES = 8;
+constexpr int KB = 128;       // k per block: 4 lanes x 32
 
-enum { ZERO_SUBTRACT = 0, ZERO_FMA = 1, ZERO_TWO = 2 };
+enum { ZERO_SUBTRACT = 0, ZERO_FMA = 1, ZERO_TWO = 2, ZERO_EIGHT = 3 };   // EIGHT: subtract without zero points
 
 struct Params {
   const uint8_t* codes;            // [N][K / 2]
@@ -34,13 +34,14 @@ struct Params {
   const float* bias;               // [N] or null, added before y is rounded
   __nv_bfloat16* y;                // M rows, `ldy` apart
   long long ldy;
-  int M, N, K, group, ng;
+  int M, N, K, ng;
+  float per_group;                 // 32 / group
   const int* blocks;               // check mode: blocks of 16 outputs
   unsigned long long* check;
 };
 
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -49,112 +50,164 @@ __device__ __forceinline__ __nv_bfloat162 as_bf2(uint32_t u) { return *reinterpr
 __device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 v) { return *reinterpret_cast<uint32_t*>(&v); }
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
   uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0,%1,%2,%3}, [%4];"
+  asm("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
                : "l"(p));
   return r;
 }
 __device__ __forceinline__ uint32_t word(const uint4& u, int j) { return j == 0 ? u.x : j == 1 ? u.y : j == 2 ? u.z : u.w; }
 
-// Weights (i, i + 4) of a word of eight codes.
-template <int MODE>
-__device__ __forceinline__ uint32_t pair(uint32_t w, int i, __nv_bfloat162 zero, __nv_bfloat162 scale, __nv_bfloat162 zs) {
-  const uint32_t q = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;        // 128 + q
-  const __nv_bfloat162 v = __hsub2_rn(as_bf2(q), zero);                   // q - z, or q: exact
-  if (MODE == ZERO_SUBTRACT) return as_u32(__hmul2_rn(v, scale));
-  if (MODE == ZERO_FMA) return as_u32(__hfma2(v, scale, zs));
-  return as_u32(__hadd2_rn(__hmul2_rn(v, scale), zs));
-}
+__device__ const uint4 no_x[4] = {};     // what lanes behind K read for x
 
-// NT: groups of eight rows of x; MT: groups of 16 outputs a warp holds.
-template <int NT, int MT, int MODE>
-__global__ void __launch_bounds__(WARPS * 32) matvec4_kernel(const Params p) {
+// bf16 bits below 256 are the numbers 0 .. 255 times 2^-133: the subnormals and the first binade have one spacing. So a
+// masked word is a pair of codes as it stands (in bits 0-3 of each half q, in bits 4-7 16 q), one shift serves four
+// codes, and a scale times 2^100 (2^96) takes the exponent back, to W 2^-33. With z = 8 the product and 8 s, a power of
+// two times s, meet in one fma and its one rounding: 9 instructions for 8 weights. Scales below 2^27 fit the factor
+// (larger ones give NaN), and W is exact from 2^-93 up.
+constexpr float BACK = 8589934592.f;     // 2^33
+struct Factor {
+  __nv_bfloat162 s, z, add;              // scale 2^100, zero point (a code's form), what is added behind the product
+};
+template <int MODE>
+__device__ __forceinline__ Factor factor_of(uint32_t scale, uint32_t z) {
+  Factor f;
+  const __nv_bfloat162 s = as_bf2(scale * 0x10001u);
+  f.s = __hmul2_rn(s, as_bf2(0x71807180u));                                          // 2^100
+  f.z = as_bf2(z * 0x10001u);
+  if (MODE == ZERO_EIGHT) f.add = __hmul2_rn(s, as_bf2(0xb080b080u));                // -8 2^-33
+  if (MODE == ZERO_FMA || MODE == ZERO_TWO)
+    f.add = __hmul2_rn(__hmul2_rn(s, __float2bfloat162_rn(-static_cast<float>(z))), as_bf2(0x2f002f00u));   // rnd, 2^-33
+  return f;
+}
+// The same for codes in bits 4-7: 16 times larger.
+template <int MODE>
+__device__ __forceinline__ Factor high_factor(const Factor& f) {
+  Factor h = f;
+  h.s = __hmul2_rn(f.s, as_bf2(0x3d803d80u));                                        // 1 / 16
+  if (MODE == ZERO_SUBTRACT) h.z = __hmul2_rn(f.z, as_bf2(0x41804180u));             // 16
+  return h;
+}
+template <int MODE>
+__device__ __forceinline__ uint32_t weights(uint32_t q, const Factor& f) {
+  const __nv_bfloat162 v = as_bf2(q);
+  if (MODE == ZERO_SUBTRACT) return as_u32(__hmul2_rn(__hsub2_rn(v, f.z), f.s));
+  if (MODE == ZERO_TWO) return as_u32(__hadd2_rn(__hmul2_rn(v, f.s), f.add));
+  return as_u32(__hfma2(v, f.s, f.add));
+}
+// NT: groups of eight rows of x; MT: groups of 16 outputs; PF: k blocks in flight per warp. Outputs behind N and rows of
+// x behind M are computed from the last ones there are and not written, which costs no predicates in the loop.
+template <int NT, int MT, int WARPS, int PF, int CTAS, int MODE>
+__global__ void __launch_bounds__(WARPS * 32, CTAS) matvec4_kernel(const Params p) {
   pdl_trigger();
-  __shared__ float red[WARPS][NT * 8][MT * 16 + 1];
+  __shared__ float red[SLICES][NT * 8][MT * 16 + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int n0 = (p.blocks ? p.blocks[blockIdx.x] : static_cast<int>(blockIdx.x) * MT) * 16;
   if (p.check != nullptr && blockIdx.x == 0 && tid == 0) atomicAdd(p.check + 2, 1ull);
   if (n0 < 0 || n0 >= p.N) return;
-  float acc[MT][NT][4];
+  const int nkb = (p.K + KB - 1) / KB;
+  const uint8_t* code[MT][2];
+  int meta[MT][2];                       // of the outputs' scales and zero points
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+    for (int r = 0; r < 2; ++r) {
+      const int n = min(n0 + i * 16 + r * 8 + g, p.N - 1);
+      code[i][r] = p.codes + static_cast<long long>(n) * (p.K / 2);
+      meta[i][r] = n * p.ng;
+    }
+  const __nv_bfloat16* xrow[NT];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-  const __nv_bfloat162 magic = as_bf2(0x43004300u);
-  const int nkb = (p.K + KB - 1) / KB;
-#pragma unroll 2
-  for (int kb = warp; kb < nkb; kb += WARPS) {
-    const int k = kb * KB + 32 * t;
-    const bool in = k < p.K;             // K is a multiple of 32
-    uint4 w[MT][2];
-    __nv_bfloat162 sc[MT][2], ze[MT][2], zs[MT][2];
+  for (int j = 0; j < NT; ++j) xrow[j] = p.x + min(j * 8 + g, p.M - 1) * p.ldx;
+  uint4 w[PF][MT][2];                    // a lane's 32 codes, scale and zero point of 2 MT outputs
+  uint32_t ws[PF][MT][2], wz[PF][MT][2];
+  // the warp's blocks: slice after slice, in each every SLICES-th, a slice in whole turns of the PF buffers
+  int ls = warp, lk = warp;              // the next block to load
+  const auto load_next = [&](int f) {
+    if (lk < nkb) {
+      const int k = lk * KB + 32 * t;
+      const int kc = k < p.K ? k : 0;    // the last block may end early (K is a multiple of 32): x is 0 there
+      const int gi = static_cast<int>((static_cast<float>(kc >> 5) + 0.5f) * p.per_group);     // kc / group
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          w[f][i][r] = ld_stream(code[i][r] + (kc >> 1));
+          ws[f][i][r] = __ldg(reinterpret_cast<const unsigned short*>(p.scales) + meta[i][r] + gi);
+          if (MODE != ZERO_EIGHT) wz[f][i][r] = __ldg(p.zeros + meta[i][r] + gi);
+        }
+    }
+    lk += SLICES;
+    if (WARPS < SLICES && f == PF - 1 && lk >= nkb && ls + WARPS < SLICES) lk = ls += WARPS;
+  };
+#pragma unroll
+  for (int f = 0; f < PF; ++f) load_next(f);
+  for (int slice = warp; slice < SLICES; slice += WARPS) {
+    float acc[MT][NT][4];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int n = n0 + i * 16 + r * 8 + g;
-        const bool ok = in && n < p.N;
-        w[i][r] = ok ? ld_stream(p.codes + static_cast<long long>(n) * (p.K / 2) + k / 2) : make_uint4(0, 0, 0, 0);
-        const long long gi = static_cast<long long>(n) * p.ng + k / p.group;
-        const __nv_bfloat16 s = ok ? p.scales[gi] : __float2bfloat16(0.f);
-        const int z = p.zeros == nullptr ? 8 : ok ? p.zeros[gi] : 0;
-        sc[i][r] = __bfloat162bfloat162(s);
-        if (MODE == ZERO_SUBTRACT) {
-          ze[i][r] = __bfloat162bfloat162(__int2bfloat16_rn(128 + z));
-        } else {
-          ze[i][r] = magic;
-          zs[i][r] = __bfloat162bfloat162(__float2bfloat16_rn(-__bfloat162float(s) * static_cast<float>(z)));
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
+    for (int kb = slice; kb < nkb; kb += SLICES * PF) {
+#pragma unroll
+      for (int f = 0; f < PF; ++f) {
+        const int kc = kb + f * SLICES;
+        if (kc < nkb) {                  // (uniform)
+          const int k = kc * KB + 32 * t;
+          const uint4* xp[NT];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) xp[j] = k < p.K ? reinterpret_cast<const uint4*>(xrow[j] + k) : no_x;
+          Factor lo[MT][2];
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) lo[i][r] = factor_of<MODE>(ws[f][i][r], MODE == ZERO_EIGHT ? 8u : wz[f][i][r]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {        // word c: k + 8c .. k + 8c + 7
+            uint32_t b[NT][4];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              const uint4 x = __ldg(xp[j] + c);
+              b[j][0] = __byte_perm(x.x, x.z, 0x5410);    // x0, x4
+              b[j][1] = __byte_perm(x.x, x.z, 0x7632);    // x1, x5
+              b[j][2] = __byte_perm(x.y, x.w, 0x5410);    // x2, x6
+              b[j][3] = __byte_perm(x.y, x.w, 0x7632);    // x3, x7
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              const uint32_t w0 = word(w[f][i][0], c), w1 = word(w[f][i][1], c);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t u0 = h ? w0 >> 8 : w0, u1 = h ? w1 >> 8 : w1;
+                const uint32_t a[4] = {weights<MODE>(u0 & 0x000f000fu, lo[i][0]), weights<MODE>(u1 & 0x000f000fu, lo[i][1]),
+                                 weights<MODE>(u0 & 0x00f000f0u, high_factor<MODE>(lo[i][0])),
+                                 weights<MODE>(u1 & 0x00f000f0u, high_factor<MODE>(lo[i][1]))};
+#pragma unroll
+                for (int j = 0; j < NT; ++j) mma(acc[i][j], a, b[j][2 * h], b[j][2 * h + 1]);
+              }
+            }
+          }
         }
-      }
-    uint4 xr[NT][4];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int m = j * 8 + g;
-      const uint4* src = reinterpret_cast<const uint4*>(p.x + m * p.ldx + k);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) xr[j][c] = in && m < p.M ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {          // word c: k + 8c .. k + 8c + 7
-      uint32_t b[NT][4];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        b[j][0] = __byte_perm(xr[j][c].x, xr[j][c].z, 0x5410);    // x0, x4
-        b[j][1] = __byte_perm(xr[j][c].x, xr[j][c].z, 0x7632);    // x1, x5
-        b[j][2] = __byte_perm(xr[j][c].y, xr[j][c].w, 0x5410);    // x2, x6
-        b[j][3] = __byte_perm(xr[j][c].y, xr[j][c].w, 0x7632);    // x3, x7
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const uint32_t w0 = word(w[i][0], c), w1 = word(w[i][1], c);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t a[4] = {pair<MODE>(w0, 2 * h, ze[i][0], sc[i][0], zs[i][0]),
-                                 pair<MODE>(w1, 2 * h, ze[i][1], sc[i][1], zs[i][1]),
-                                 pair<MODE>(w0, 2 * h + 1, ze[i][0], sc[i][0], zs[i][0]),
-                                 pair<MODE>(w1, 2 * h + 1, ze[i][1], sc[i][1], zs[i][1])};
-#pragma unroll
-          for (int j = 0; j < NT; ++j) mma(acc[i][j], a, b[j][2 * h], b[j][2 * h + 1]);
-        }
+        load_next(f);
       }
     }
+    // acc[i][j]: outputs 16 i + g (+ 8), rows 8 j + 2t (+ 1)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[slice][j * 8 + 2 * t + (e & 1)][i * 16 + g + (e >> 1) * 8] = acc[i][j][e];
   }
-  // acc[i][j]: outputs 16 i + g (+ 8), rows 8 j + 2t (+ 1)
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) red[warp][j * 8 + 2 * t + (e & 1)][i * 16 + g + (e >> 1) * 8] = acc[i][j][e];
   __syncthreads();
   for (int i = tid; i < p.M * MT * 16; i += WARPS * 32) {
     const int m = i / (MT * 16), c = i % (MT * 16), n = n0 + c;
     if (n >= p.N) continue;
     float s = red[0][m][c];
 #pragma unroll
-    for (int w = 1; w < WARPS; ++w) s += red[w][m][c];
+    for (int w = 1; w < SLICES; ++w) s += red[w][m][c];
+    s *= BACK;
     if (p.bias != nullptr) s += p.bias[n];
     __nv_bfloat16* dst = p.y + m * p.ldy + n;
     const __nv_bfloat16 r = __float2bfloat16(s);
@@ -168,12 +221,15 @@ __global__ void __launch_bounds__(WARPS * 32) matvec4_kernel(const Params p) {
   }
 }
 
-template <int NT, int MT>
+template <int NT, int MT, int WARPS, int PF, int CTAS>
 static int launch(const Params& p, int mode, int grid, cudaStream_t st) {
   switch (mode) {
-    case ZERO_SUBTRACT: matvec4_kernel<NT, MT, ZERO_SUBTRACT><<<grid, WARPS * 32, 0, st>>>(p); break;
-    case ZERO_FMA: matvec4_kernel<NT, MT, ZERO_FMA><<<grid, WARPS * 32, 0, st>>>(p); break;
-    default: matvec4_kernel<NT, MT, ZERO_TWO><<<grid, WARPS * 32, 0, st>>>(p); break;
+    case ZERO_SUBTRACT:
+      if (p.zeros == nullptr) matvec4_kernel<NT, MT, WARPS, PF, CTAS, ZERO_EIGHT><<<grid, WARPS * 32, 0, st>>>(p);
+      else matvec4_kernel<NT, MT, WARPS, PF, CTAS, ZERO_SUBTRACT><<<grid, WARPS * 32, 0, st>>>(p);
+      break;
+    case ZERO_FMA: matvec4_kernel<NT, MT, WARPS, PF, CTAS, ZERO_FMA><<<grid, WARPS * 32, 0, st>>>(p); break;
+    default: matvec4_kernel<NT, MT, WARPS, PF, CTAS, ZERO_TWO><<<grid, WARPS * 32, 0, st>>>(p); break;
   }
   return static_cast<int>(cudaGetLastError());
 }
@@ -187,6 +243,8 @@ extern "C" int sdc_matvec4(const void* x, long long ldx, int M, int N, int K, in
                            const void* scales, const void* zeros, int mode, const void* bias, void* y,
                            long long ldy, const int* blocks, int nblocks, void* check, void* stream) {
   if (M <= 0 || N <= 0) return 0;
+  // scale indices fit 32 bits, and (k / 32 + 1/2) * (32 / group) in fp32 finds a k's group up to K = 2^25
+  if (static_cast<long long>(N) * (K / 32) > 0x7fffffffll || K > (1 << 25)) return -1;
   if (M > 32 || K <= 0 || K % 32 || group <= 0 || group % 32 || K % group || ldx % 8 || mode < 0 || mode > 2 ||
       (mode != ZERO_SUBTRACT && zeros == nullptr) || (check != nullptr) != (blocks != nullptr))
     return -1;
@@ -202,17 +260,17 @@ extern "C" int sdc_matvec4(const void* x, long long ldx, int M, int N, int K, in
   p.M = M;
   p.N = N;
   p.K = K;
-  p.group = group;
   p.ng = K / group;
+  p.per_group = 32.f / static_cast<float>(group);
   p.blocks = blocks;
   p.check = static_cast<unsigned long long*>(check);
   auto st = static_cast<cudaStream_t>(stream);
   if (blocks != nullptr) {
     if (nblocks <= 0) return 0;
-    return M <= 8 ? launch<1, 1>(p, mode, nblocks, st)
-                  : M <= 16 ? launch<2, 1>(p, mode, nblocks, st) : launch<4, 1>(p, mode, nblocks, st);
+    return M <= 8 ? launch<1, 1, 8, 2, 4>(p, mode, nblocks, st)
+                  : M <= 16 ? launch<2, 1, 8, 2, 3>(p, mode, nblocks, st) : launch<4, 1, 8, 2, 2>(p, mode, nblocks, st);
   }
-  if (M <= 8) return launch<1, 1>(p, mode, (N + 15) / 16, st);
-  if (M <= 16) return launch<2, 2>(p, mode, (N + 31) / 32, st);
-  return launch<4, 2>(p, mode, (N + 31) / 32, st);
+  if (M <= 8) return launch<1, 1, 8, 2, 4>(p, mode, (N + 15) / 16, st);
+  if (M <= 16) return launch<2, 2, 8, 1, 2>(p, mode, (N + 31) / 32, st);
+  return launch<4, 2, 8, 2, 1>(p, mode, (N + 31) / 32, st);
 }

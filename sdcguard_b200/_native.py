@@ -168,7 +168,7 @@ def lib():
         return _lib
 
 
-WAIT_LIMIT_UNITS = ("attention", "ep_comm", "gemm_abft", "gemm_fp8", "tp_comm")
+WAIT_LIMIT_UNITS = ("attention", "ep_comm", "gemm_abft", "gemm_fp8", "kv8", "tp_comm")
 DEFAULT_WAIT_NS = 2_000_000_000
 
 

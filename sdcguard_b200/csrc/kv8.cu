@@ -12,7 +12,10 @@
 // A value that is not finite is stored as NaN and does not raise the scale.
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
+#include "tma_host.h"
 
 namespace sdc {
 namespace kv8 {
@@ -674,16 +677,9 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-               : "l"(p));
-  return r;
-}
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -698,19 +694,14 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-struct PageRegs {
-  uint4 k[4];      // key g: dims 16t.., 64 + 16t..; key g + 8: the same
-  uint4 v[4];      // keys 2t, 2t + 1, 2t + 8, 2t + 9: dims 16g..
-};
-__device__ __forceinline__ void load_page(PageRegs& r, const uint8_t* kp, const uint8_t* vp, int g, int t) {
-  r.k[0] = ld_stream(kp + g * D + 16 * t);
-  r.k[1] = ld_stream(kp + g * D + 64 + 16 * t);
-  r.k[2] = ld_stream(kp + (g + 8) * D + 16 * t);
-  r.k[3] = ld_stream(kp + (g + 8) * D + 64 + 16 * t);
-  r.v[0] = ld_stream(vp + (2 * t) * D + 16 * g);
-  r.v[1] = ld_stream(vp + (2 * t + 1) * D + 16 * g);
-  r.v[2] = ld_stream(vp + (2 * t + 8) * D + 16 * g);
-  r.v[3] = ld_stream(vp + (2 * t + 9) * D + 16 * g);
+// A warp's pages wait in shared memory, K then V of one head, 16 rows of 128 bytes each as TMA lays them out: 16-byte
+// piece j of row r at piece j ^ (r & 7). Matrix row i stands for key key_of(i) (and 8 + i for 8 + key_of(i)); this order
+// makes both reads below free of bank conflicts: eight lanes meet eight different pieces.
+constexpr int STAGES = 4;                // pages of a warp in shared memory: one in use, the others on their way
+constexpr int PAGE_BYTES = PAGE * D;
+__device__ __forceinline__ int key_of(int i) { return i ^ ((i & 1) << 2); }
+__device__ __forceinline__ uint4 piece(const uint8_t* rows, int key, int j) {
+  return *reinterpret_cast<const uint4*>(rows + key * D + ((j ^ (key & 7)) << 4));
 }
 __device__ __forceinline__ uint32_t word(const uint4& u, int j) { return j == 0 ? u.x : j == 1 ? u.y : j == 2 ? u.z : u.w; }
 
@@ -734,12 +725,24 @@ __device__ __forceinline__ bool row_fits(const DecodeParams& p, int n, int req) 
          req < p.table_rows;
 }
 
+template <int NT>
+struct DecodeSmem {
+  union {
+    uint8_t ring[WARPS][STAGES][2 * PAGE_BYTES];
+    float o[WARPS][NT * 8][D];           // the warps' sums, once the pages are done with
+  };
+  float m[WARPS][NT * 8], l[WARPS][NT * 8];
+  uint64_t full[WARPS][STAGES];
+};
+
 // NT: groups of eight heads (1: up to 8 queries a kv head, 2: up to 16).
 template <int NT>
-__global__ void __launch_bounds__(WARPS * 32) kv8_decode_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(WARPS * 32, 3) kv8_decode_kernel(const __grid_constant__ CUtensorMap tm,
+                                                                     const DecodeParams p) {
   pdl_trigger();
-  __shared__ float osm[WARPS][NT * 8][D];
-  __shared__ float msm[WARPS][NT * 8], lsm[WARPS][NT * 8];
+  extern __shared__ unsigned char decode_smem[];
+  // the pages' swizzle counts from 1 KB boundaries
+  DecodeSmem<NT>& sm = *reinterpret_cast<DecodeSmem<NT>*>(decode_smem + ((1024 - (smem_u32(decode_smem) & 1023)) & 1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int b = p.seq_idx ? p.seq_idx[blockIdx.x] : blockIdx.x;
   if (b < 0 || b >= p.nseqs) return;
@@ -756,6 +759,49 @@ __global__ void __launch_bounds__(WARPS * 32) kv8_decode_kernel(const DecodePara
   }
   const int nseg = (pages + p.seg_pages - 1) / p.seg_pages;
   if (static_cast<int>(blockIdx.z) >= nseg) return;
+  if (lane == 0) {
+    tma_prefetch_desc(&tm);
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) mbar_init(&sm.full[warp][i], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  int fetched = 0, used = 0;             // this warp's pages so far: page i waits in stage i % STAGES
+  bool ok = true;
+  // A segment's pages of this warp. Lane i holds the place (in units of a head's page) and the scales of page 32 c + i:
+  // of the 32 pages around page k, and of the next 32.
+  const int* row = p.table + req * p.table_ld;
+  int first = 0, count = 0, unit0, unit1;
+  float2 sc0, sc1;
+  const auto look_up = [&](int k, int& unit, float2& sc) {
+    const int id = k < count ? row[first + WARPS * k] : 0;
+    const bool in = id >= 0 && id < p.num_blocks;
+    unit = (in ? id : 0) * 2 * p.nkv + kvh;
+    sc = k < count ? p.scales[static_cast<long long>(in ? id : 0) * p.nkv + kvh] : make_float2(0.f, 0.f);
+    if (!in) sc.x = sc.y = __int_as_float(0x7fffffff);
+  };
+  const auto fetch = [&](int k, int base) {                // page k, base <= k < base + 64
+    const int u0 = __shfl_sync(0xffffffffu, unit0, k & 31), u1 = __shfl_sync(0xffffffffu, unit1, k & 31);
+    if (k >= count) return;
+    if (lane == 0) {
+      const int stage = fetched % STAGES, unit = k - base < 32 ? u0 : u1;
+      uint64_t* bar = &sm.full[warp][stage];
+      mbar_arrive_expect_tx(bar, 2 * PAGE_BYTES);
+      tma_load_2d(sm.ring[warp][stage], &tm, bar, 0, unit * PAGE);
+      tma_load_2d(sm.ring[warp][stage] + PAGE_BYTES, &tm, bar, 0, (unit + p.nkv) * PAGE);
+    }
+    ++fetched;
+  };
+  const auto begin = [&](int seg) {
+    first = seg * p.seg_pages + warp;
+    const int end = min(pages, (seg + 1) * p.seg_pages);
+    count = first < end ? (end - first + WARPS - 1) / WARPS : 0;
+    look_up(lane, unit0, sc0);
+    look_up(32 + lane, unit1, sc1);
+#pragma unroll 1
+    for (int k = 0; k < STAGES - 1; ++k) fetch(k, 0);
+  };
+  begin(blockIdx.z);                     // the first pages are on their way before the queries are read
   // Q^T fragments: b0 = dims 64c + 16t + 4j + {0, 1}, b1 = + {2, 3} of head g, k step 4c + j
   uint32_t qb[NT][8][2];
   float f[NT][2];                    // heads 2t, 2t + 1: scale log2(e) / (the head's power of two)
@@ -794,11 +840,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv8_decode_kernel(const DecodePara
 #pragma unroll
     for (int c = 0; c < 2; ++c) f[nt][c] = p.scale_log2 * __shfl_sync(0xffffffffu, down, (2 * t + c) * 4);
   }
-  const int* row = p.table + req * p.table_ld;
-  const long long kv_stride = static_cast<long long>(p.nkv) * PAGE * D;
   for (int seg = blockIdx.z; seg < nseg; seg += gridDim.z) {
-    const int first = seg * p.seg_pages + warp, end = min(pages, (seg + 1) * p.seg_pages);
-    const int count = first < end ? (end - first + WARPS - 1) / WARPS : 0;
+    if (seg != static_cast<int>(blockIdx.z)) begin(seg);
     float M[NT][2], l[NT][2], o[NT][8][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -809,58 +852,45 @@ __global__ void __launch_bounds__(WARPS * 32) kv8_decode_kernel(const DecodePara
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
     }
-    long long blk = 0;
-    float2 sc = make_float2(0.f, 0.f);
-    PageRegs cur;
-    // 32 of this warp's pages at a time: lane i holds the id and the scales of page i
-    for (int k0 = 0; k0 < count; k0 += 32) {
-      {
-        const int k = k0 + lane;
-        int id = k < count ? row[first + WARPS * k] : 0;
-        const bool in = id >= 0 && id < p.num_blocks;
-        blk = in ? id : 0;
-        sc = k < count ? p.scales[blk * p.nkv + kvh] : make_float2(0.f, 0.f);
-        if (!in) sc.x = sc.y = __int_as_float(0x7fffffff);
+    for (int k = 0; k < count; ++k) {
+      if (k > 0 && (k & 31) == 0) {
+        unit0 = unit1;
+        sc0 = sc1;
+        look_up(k + 32 + lane, unit1, sc1);
       }
-      const int kn = min(32, count - k0);
-      {
-        const uint8_t* kp = p.codes + (__shfl_sync(0xffffffffu, blk, 0) * 2 * p.nkv + kvh) * (PAGE * D);
-        load_page(cur, kp, kp + kv_stride, g, t);
+      __syncwarp();                      // the stage of page k + STAGES - 1 was read in the turn before
+      fetch(k + STAGES - 1, k & ~31);
+      ok = mbar_wait(&sm.full[warp][used % STAGES], (used / STAGES) & 1, nullptr);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
       }
-      for (int k = 0; k < kn; ++k) {
-        PageRegs nxt;
-        const float ks = __shfl_sync(0xffffffffu, sc.x, k), vs = __shfl_sync(0xffffffffu, sc.y, k);
-        const long long nb = __shfl_sync(0xffffffffu, blk, (k + 1) & 31);
-        if (k + 1 < kn) {
-          const uint8_t* kp = p.codes + (nb * 2 * p.nkv + kvh) * (PAGE * D);
-          load_page(nxt, kp, kp + kv_stride, g, t);
-        }
-        const int key0 = (first + WARPS * (k0 + k)) * PAGE;
-        if (key0 + PAGE > n) {         // the sequence's last page: nothing behind its end may reach a product
-          const uint4 z = make_uint4(0, 0, 0, 0);
-          if (key0 + 2 * t >= n) cur.v[0] = z;
-          if (key0 + 2 * t + 1 >= n) cur.v[1] = z;
-          if (key0 + 2 * t + 8 >= n) cur.v[2] = z;
-          if (key0 + 2 * t + 9 >= n) cur.v[3] = z;
-        }
+      const uint8_t* kpage = sm.ring[warp][used % STAGES];
+      const uint8_t* vpage = kpage + PAGE_BYTES;
+      ++used;
+      const float ks = __shfl_sync(0xffffffffu, sc0.x, k & 31), vs = __shfl_sync(0xffffffffu, sc0.y, k & 31);
+      const int key0 = (first + WARPS * k) * PAGE;
+      {
         float s[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 2; ++c) {
+          const uint4 k0 = piece(kpage, key_of(g), 4 * c + t), k8 = piece(kpage, 8 + key_of(g), 4 * c + t);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint32_t w0 = word(cur.k[c], j), w1 = word(cur.k[2 + c], j);
+            const uint32_t w0 = word(k0, j), w1 = word(k8, j);
             const uint32_t a0 = e4m3x2_to_h2(w0), a2 = e4m3x2_to_h2_hi(w0);
             const uint32_t a1 = e4m3x2_to_h2(w1), a3 = e4m3x2_to_h2_hi(w1);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a0, a1, a2, a3, qb[nt][4 * c + j][0], qb[nt][4 * c + j][1]);
           }
+        }
         const float ev = static_cast<float>(max(static_cast<int>((__float_as_uint(vs) >> 23) & 255u) - 127, -60));
         const float vw = vs * W_SCALE;       // s_V 2^(14 - SUM_BIAS)
-        const bool in0 = key0 + g < n, in1 = key0 + g + 8 < n;
+        const bool in0 = key0 + key_of(g) < n, in1 = key0 + key_of(g) + 8 < n;
         uint32_t pb[NT][2];
         bool moved = false;
         float a[NT][2], Mn[NT][2];
@@ -910,9 +940,17 @@ __global__ void __launch_bounds__(WARPS * 32) kv8_decode_kernel(const DecodePara
           pb[nt][0] = transpose8(pack_h2(w[0], w[1]));
           pb[nt][1] = transpose8(pack_h2(w[2], w[3]));
         }
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = piece(vpage, key_of(2 * t + (i & 1)) + (i >> 1) * 8, g);
+        if (key0 + PAGE > n) {         // the sequence's last page: nothing behind its end may reach a product
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (key0 + key_of(2 * t + (i & 1)) + (i >> 1) * 8 >= n) v[i] = make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t w0 = word(cur.v[0], j), w1 = word(cur.v[1], j), w2 = word(cur.v[2], j), w3 = word(cur.v[3], j);
+          const uint32_t w0 = word(v[0], j), w1 = word(v[1], j), w2 = word(v[2], j), w3 = word(v[3], j);
           const uint32_t x01 = __byte_perm(w0, w1, 0x5140), y01 = __byte_perm(w0, w1, 0x7362);
           const uint32_t x23 = __byte_perm(w2, w3, 0x5140), y23 = __byte_perm(w2, w3, 0x7362);
           const uint32_t a0 = e4m3x2_to_h2(x01), a1 = e4m3x2_to_h2_hi(x01);
@@ -925,9 +963,14 @@ __global__ void __launch_bounds__(WARPS * 32) kv8_decode_kernel(const DecodePara
             mma_f16(o[nt][2 * j + 1], c0, c1, c2, c3, pb[nt][0], pb[nt][1]);
           }
         }
-        cur = nxt;
       }
     }
+    if (!ok) {                           // a wait ran out: the row becomes NaN, and what is on its way must land
+      for (; used < fetched; ++used) mbar_wait(&sm.full[warp][used % STAGES], (used / STAGES) & 1, nullptr);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = __int_as_float(0x7fffffff);
+    }
+    __syncthreads();                     // every warp is done with its pages
     // merge of the four warps: o[nt][i] holds dims 16g + 2i + {0, 1} of heads 2t, 2t + 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -936,28 +979,28 @@ __global__ void __launch_bounds__(WARPS * 32) kv8_decode_kernel(const DecodePara
         const int h = nt * 8 + 2 * t + c;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<float2*>(&osm[warp][h][16 * g + 2 * i]) = make_float2(o[nt][i][c], o[nt][i][2 + c]);
+          *reinterpret_cast<float2*>(&sm.o[warp][h][16 * g + 2 * i]) = make_float2(o[nt][i][c], o[nt][i][2 + c]);
         float s = l[nt][c];
         s += __shfl_xor_sync(0xffffffffu, s, 4);
         s += __shfl_xor_sync(0xffffffffu, s, 8);
         s += __shfl_xor_sync(0xffffffffu, s, 16);
         if (g == 0) {
-          msm[warp][h] = M[nt][c];
-          lsm[warp][h] = s;
+          sm.m[warp][h] = M[nt][c];
+          sm.l[warp][h] = s;
         }
       }
     }
     __syncthreads();
     float sq = 0.f;
     for (int h = 0; h < p.G; ++h) {
-      const float m = fmaxf(fmaxf(msm[0][h], msm[1][h]), fmaxf(msm[2][h], msm[3][h]));
+      const float m = fmaxf(fmaxf(sm.m[0][h], sm.m[1][h]), fmaxf(sm.m[2][h], sm.m[3][h]));
       const float ref = m == -INFINITY ? 0.f : m;
       float acc = 0.f, ls = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float e = ex2(msm[w][h] - ref);
-        acc = fmaf(osm[w][h][tid], e, acc);
-        ls = fmaf(lsm[w][h], e, ls);
+        const float e = ex2(sm.m[w][h] - ref);
+        acc = fmaf(sm.o[w][h][tid], e, acc);
+        ls = fmaf(sm.l[w][h], e, ls);
       }
       if (nseg == 1) {
         sq += put(p, b, kvh * p.G + h, tid, ls == 0.f ? 0.f : acc / ls * (1.f / W_SCALE));
@@ -974,6 +1017,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv8_decode_kernel(const DecodePara
       sq = warp_sum(sq);
       if (lane == 0) atomicAdd(p.row_sq + b, sq);
     }
+    fence_proxy_async_smem();            // the sums lay where the next segment's pages go
     __syncthreads();
   }
 }
@@ -1032,9 +1076,19 @@ __global__ void __launch_bounds__(PARTS * D) kv8_combine_kernel(const DecodePara
 }
 
 template <int NT>
-static int launch_decode(const DecodeParams& p, int nrun, int z, cudaStream_t st) {
-  kv8_decode_kernel<NT><<<dim3(nrun, p.nkv, z), WARPS * 32, 0, st>>>(p);
-  cudaError_t e = cudaGetLastError();
+static int launch_decode(const CUtensorMap& tm, const DecodeParams& p, int nrun, int z, cudaStream_t st) {
+  // the attribute belongs to a device; one bit for each that has it (setting it twice does no harm)
+  static std::atomic<unsigned long long> ready{0};
+  constexpr int smem = static_cast<int>(sizeof(DecodeSmem<NT>)) + 1024;   // + room to align the pages
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev > 63 || !(ready.load() >> dev & 1))) {
+    e = cudaFuncSetAttribute(kv8_decode_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && dev <= 63) ready.fetch_or(1ull << dev);
+  }
+  if (e != cudaSuccess) return static_cast<int>(e);
+  kv8_decode_kernel<NT><<<dim3(nrun, p.nkv, z), WARPS * 32, smem, st>>>(tm, p);
+  e = cudaGetLastError();
   if (e != cudaSuccess || p.max_segs == 1) return static_cast<int>(e);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(nrun, p.nq);
@@ -1137,8 +1191,11 @@ int sdc_kv8_decode(const void* q, void* o, const void* codes, const void* scales
   if (nrun <= 0) return 0;
   if (nkv < 1 || nq % nkv || nq / nkv < 1 || nq / nkv > 16 || seg_pages < 1 || max_segs < 1 || max_segs > MAX_SEGS ||
       (max_segs > 1 && part == nullptr) || (check != nullptr && seq_idx == nullptr) ||
-      (seq_idx == nullptr && nrun > nseqs))
+      (seq_idx == nullptr && nrun > nseqs) || num_blocks * 2 * nkv * PAGE > 0x7fffffffll)
     return -1;
+  // the layer's codes as [num_blocks * 2 * nkv * 16][128] bytes; one box is one page of K or V of a head
+  CUtensorMap tm;
+  if (!make_map_u8_sw128(&tm, codes, num_blocks * 2 * nkv * PAGE, D, D, D, PAGE)) return -2;
   DecodeParams p;
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.o = static_cast<__nv_bfloat16*>(o);
@@ -1167,7 +1224,11 @@ int sdc_kv8_decode(const void* q, void* o, const void* codes, const void* scales
   long long z = 32768 / rows;
   z = z < 1 ? 1 : z > max_segs ? max_segs : z;
   auto st = static_cast<cudaStream_t>(stream);
-  return p.G <= 8 ? launch_decode<1>(p, nrun, static_cast<int>(z), st) : launch_decode<2>(p, nrun, static_cast<int>(z), st);
+  return p.G <= 8 ? launch_decode<1>(tm, p, nrun, static_cast<int>(z), st)
+                  : launch_decode<2>(tm, p, nrun, static_cast<int>(z), st);
 }
 
 }  // extern "C"
+
+// run-time wait limit of this unit (see common.cuh)
+SDC_WAIT_LIMIT_SETTER(kv8)

@@ -697,7 +697,7 @@ __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
 // A warp's pages wait in shared memory, K then V of one head, 16 rows of 128 bytes each as TMA lays them out: 16-byte
 // piece j of row r at piece j ^ (r & 7). Matrix row i stands for key key_of(i) (and 8 + i for 8 + key_of(i)); this order
 // makes both reads below free of bank conflicts: eight lanes meet eight different pieces.
-constexpr int STAGES = 4;                // pages of a warp in shared memory: one in use, the others on their way
+constexpr int STAGES = 3;                // pages of a warp in shared memory: one in use, the others on their way
 constexpr int PAGE_BYTES = PAGE * D;
 __device__ __forceinline__ int key_of(int i) { return i ^ ((i & 1) << 2); }
 __device__ __forceinline__ uint4 piece(const uint8_t* rows, int key, int j) {
@@ -725,11 +725,15 @@ __device__ __forceinline__ bool row_fits(const DecodeParams& p, int n, int req) 
          req < p.table_rows;
 }
 
+// The dim of float i of a row of sums: dim 16g + 2i + e lies at 2 (8i + g) + e, so that the lanes of a store meet
+// different banks.
+__device__ __forceinline__ int dim_of(int i) { return 16 * ((i >> 1) & 7) + 2 * (i >> 4) + (i & 1); }
+
 template <int NT>
 struct DecodeSmem {
   union {
     uint8_t ring[WARPS][STAGES][2 * PAGE_BYTES];
-    float o[WARPS][NT * 8][D];           // the warps' sums, once the pages are done with
+    float o[WARPS][NT * 8][D + 4];       // the warps' sums (see dim_of), once the pages are done with
   };
   float m[WARPS][NT * 8], l[WARPS][NT * 8];
   uint64_t full[WARPS][STAGES];
@@ -737,7 +741,7 @@ struct DecodeSmem {
 
 // NT: groups of eight heads (1: up to 8 queries a kv head, 2: up to 16).
 template <int NT>
-__global__ void __launch_bounds__(WARPS * 32, 3) kv8_decode_kernel(const __grid_constant__ CUtensorMap tm,
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv8_decode_kernel(const __grid_constant__ CUtensorMap tm,
                                                                      const DecodeParams p) {
   pdl_trigger();
   extern __shared__ unsigned char decode_smem[];
@@ -754,7 +758,8 @@ __global__ void __launch_bounds__(WARPS * 32, 3) kv8_decode_kernel(const __grid_
   if (!fits || n == 0) {
     if (blockIdx.z != 0) return;
     const float v = fits ? 0.f : __int_as_float(0x7fffffff);
-    for (int h = 0; h < p.G; ++h) put(p, b, kvh * p.G + h, tid, v);
+    for (int h = 0; h < p.G; ++h)
+      for (int i = tid; i < D; i += WARPS * 32) put(p, b, kvh * p.G + h, i, v);
     return;
   }
   const int nseg = (pages + p.seg_pages - 1) / p.seg_pages;
@@ -971,7 +976,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) kv8_decode_kernel(const __grid_
       for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = __int_as_float(0x7fffffff);
     }
     __syncthreads();                     // every warp is done with its pages
-    // merge of the four warps: o[nt][i] holds dims 16g + 2i + {0, 1} of heads 2t, 2t + 1
+    // merge of the warps: o[nt][i] holds dims 16g + 2i + {0, 1} of heads 2t, 2t + 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -979,7 +984,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3) kv8_decode_kernel(const __grid_
         const int h = nt * 8 + 2 * t + c;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<float2*>(&sm.o[warp][h][16 * g + 2 * i]) = make_float2(o[nt][i][c], o[nt][i][2 + c]);
+          *reinterpret_cast<float2*>(&sm.o[warp][h][2 * (8 * i + g)]) = make_float2(o[nt][i][c], o[nt][i][2 + c]);
         float s = l[nt][c];
         s += __shfl_xor_sync(0xffffffffu, s, 4);
         s += __shfl_xor_sync(0xffffffffu, s, 8);
@@ -993,20 +998,27 @@ __global__ void __launch_bounds__(WARPS * 32, 3) kv8_decode_kernel(const __grid_
     __syncthreads();
     float sq = 0.f;
     for (int h = 0; h < p.G; ++h) {
-      const float m = fmaxf(fmaxf(sm.m[0][h], sm.m[1][h]), fmaxf(sm.m[2][h], sm.m[3][h]));
+      float m = sm.m[0][h];
+#pragma unroll
+      for (int w = 1; w < WARPS; ++w) m = fmaxf(m, sm.m[w][h]);
       const float ref = m == -INFINITY ? 0.f : m;
-      float acc = 0.f, ls = 0.f;
+      float acc[D / (WARPS * 32)] = {}, ls = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
         const float e = ex2(sm.m[w][h] - ref);
-        acc = fmaf(sm.o[w][h][tid], e, acc);
+#pragma unroll
+        for (int i = 0; i < D / (WARPS * 32); ++i) acc[i] = fmaf(sm.o[w][h][tid + i * WARPS * 32], e, acc[i]);
         ls = fmaf(sm.l[w][h], e, ls);
       }
       if (nseg == 1) {
-        sq += put(p, b, kvh * p.G + h, tid, ls == 0.f ? 0.f : acc / ls * (1.f / W_SCALE));
+        const float inv = ls == 0.f ? 0.f : 1.f / W_SCALE / ls;
+#pragma unroll
+        for (int i = 0; i < D / (WARPS * 32); ++i)
+          sq += put(p, b, kvh * p.G + h, dim_of(tid + i * WARPS * 32), acc[i] * inv);
       } else {
         float* rec = p.part + (((static_cast<long long>(b) * p.nkv + kvh) * p.max_segs + seg) * p.G + h) * REC;
-        rec[tid] = acc;
+#pragma unroll
+        for (int i = 0; i < D / (WARPS * 32); ++i) rec[tid + i * WARPS * 32] = acc[i];
         if (tid == 0) {
           rec[D] = m;
           rec[D + 1] = ls;
@@ -1068,7 +1080,7 @@ __global__ void __launch_bounds__(PARTS * D) kv8_combine_kernel(const DecodePara
   __syncthreads();
   if (part != 0) return;
   const float o = (osm[0][d] + osm[1][d]) + (osm[2][d] + osm[3][d]);
-  float sq = put(p, b, head, d, lsum == 0.f ? 0.f : o / lsum * (1.f / W_SCALE));
+  float sq = put(p, b, head, dim_of(d), lsum == 0.f ? 0.f : o / lsum * (1.f / W_SCALE));
   if (p.check == nullptr && p.row_sq != nullptr) {
     sq = warp_sum(sq);
     if ((tid & 31) == 0) atomicAdd(p.row_sq + b, sq);

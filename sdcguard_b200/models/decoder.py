@@ -27,6 +27,7 @@ from typing import Optional
 import torch
 
 from ..ops import attention, spot, gemm, layers
+from ..ops.kv8 import KV8Cache
 
 
 @dataclass(frozen=True)
@@ -73,6 +74,7 @@ class StepMeta:
     sample_rows: Optional[torch.Tensor] = None  # (S,) int32
     sample_tiles: Optional[torch.Tensor] = None  # prefill replay tiles
     sample_idx: Optional[torch.Tensor] = None   # prefill replay token list (same rows, tile order)
+    plan8: Optional[attention.Prefill8Plan] = None   # prefill over an 8-bit cache: its pages
 
 
 def _init_linear(n: int, k: int, gen: torch.Generator, device) -> torch.Tensor:
@@ -230,6 +232,24 @@ class CheckedDecoder:
             self._bufs["dscratch"] = torch.empty(need, dtype=torch.float32, device=self.device)
         return self._bufs["dscratch"]
 
+    def decode8_plan(self, nseq: int, max_ctx: int) -> attention.Decode8Plan:
+        """The cut and scratch of a decode step over an 8-bit cache, one for each batch size and context seen (a captured
+        decode graph keeps using its own)."""
+        plans = self.__dict__.setdefault("_plans8", {})
+        if (nseq, max_ctx) not in plans:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("no decode plan for this batch before graph capture")
+            plans[nseq, max_ctx] = attention.decode8_plan(nseq, self.nq, self.nkv, max_ctx, self.device)
+        return plans[nseq, max_ctx]
+
+    def prefill8_plan(self, block_table: torch.Tensor, ctx_lens) -> attention.Prefill8Plan:
+        """The pages of a prefill batch over an 8-bit cache; the layers share one set of expanded pages."""
+        need = sum(-(-int(n) // 16) for n in ctx_lens) * attention.expanded_page(self.nkv)
+        work = self.__dict__.get("_work8")
+        if work is None or work.numel() < need:
+            work = self._work8 = torch.empty(need, dtype=torch.bfloat16, device=self.device)
+        return attention.prefill8_plan(block_table, ctx_lens, self.nkv, work)
+
     # ---------------------------------------------------------------- ops
     def inject_next(self, name: str, row: int, col: int, xor_bits: int) -> None:
         """Fault injection: the next eager (not graph-captured) bf16 GEMM of layer `name` (e.g. "L0.down") flips
@@ -267,7 +287,7 @@ class CheckedDecoder:
     def forward(self, meta: StepMeta, cache: torch.Tensor, layer_range: Optional[tuple] = None,
                 hidden: Optional[tuple] = None, last: bool = True):
         """Runs one step; returns logits (L, vocab) bf16 for meta.logits_rows. cache: (layers, blocks, 2, nkv,
-        16, 128) bf16. Pipeline stages: layer_range=(lo, hi) runs only those layers (cache then holds hi - lo layers),
+        16, 128) bf16, or a KV8Cache of as many layers (a prefill then needs meta.plan8). Pipeline stages: layer_range=(lo, hi) runs only those layers (cache then holds hi - lo layers),
         hidden=(x, resid) enters after layer lo - 1 instead of the embedding, and last=False returns the (x, resid)
         pair after layer hi - 1 (x: the last sublayer's output, not yet added to the residual resid)."""
         cfg = self.cfg
@@ -288,6 +308,7 @@ class CheckedDecoder:
         spot_on = self.checked and st.spot and meta.mode == "prefill" and self.precision == "bf16" and T > 0
         spot_target = self._next_spot_target(lo, hi) if spot_on else None
         nq, nkv, D = self.nq, self.nkv, cfg.head_dim
+        kv8_on = isinstance(cache, KV8Cache)
         # Replay checks write nothing the forward reads, so they run on a side stream next to the main chain (filling
         # SMs the small decode kernels leave idle) and rejoin before the buffers they compare are overwritten: the
         # norm-1 / rope / attention replays before norm 2 of the same layer, the norm-2 / SwiGLU replays before the
@@ -324,14 +345,15 @@ class CheckedDecoder:
             self._linear(y, lw.qkv, lw.cw.get("qkv"), f"L{i}.qkv", qkv, rs, S)
             if spot_target == f"L{i}.qkv":
                 replay(lambda: self._spot(f"L{i}.qkv", y, lw.qkv, qkv, T))
-            layers.qk_norm_rope_kv(qkv, nq, nkv, meta.pos, meta.slots, lw.q_norm, lw.k_norm, cfg.rms_eps, self.rope,
-                                   q, lc)
+            rope_kv = layers.qk_norm_rope_kv8 if kv8_on else layers.qk_norm_rope_kv
+            rope_kv(qkv, nq, nkv, meta.pos, meta.slots, lw.q_norm, lw.k_norm, cfg.rms_eps, self.rope, q, lc)
             if chk and st.rope:
-                replay(lambda: layers.qk_norm_rope_kv(qkv, nq, nkv, meta.pos, meta.slots, lw.q_norm, lw.k_norm,
-                                                      cfg.rms_eps, self.rope, q, lc, rows=S,
-                                                      check=self._st(f"L{i}.rope_kv")))
+                replay(lambda: rope_kv(qkv, nq, nkv, meta.pos, meta.slots, lw.q_norm, lw.k_norm, cfg.rms_eps,
+                                       self.rope, q, lc, rows=S, check=self._st(f"L{i}.rope_kv")))
             ors.zero_()
-            if meta.mode == "prefill":
+            if kv8_on:
+                self._attention8(meta, q, lc, att, ors, S if chk and st.attn else None, f"L{i}.attn", replay)
+            elif meta.mode == "prefill":
                 attention.prefill(q, lc, meta.block_table, meta.pos, meta.tiles, nq, nkv, out=att, row_sq=ors)
                 if chk and st.attn:
                     replay(lambda: attention.prefill(q, lc, meta.block_table, meta.pos, meta.sample_tiles, nq, nkv,
@@ -381,6 +403,23 @@ class CheckedDecoder:
         else:
             torch.matmul(yl, self.lm_head.t(), out=logits)
         return logits
+
+    def _attention8(self, meta: StepMeta, q, cache: KV8Cache, out, row_sq, sample, name: str, replay) -> None:
+        """A layer's attention over an 8-bit cache, and the replay of its sampled rows; a prefill's replay compares
+        every 64th expanded page too, from a page that rotates with the layers and steps."""
+        if meta.mode == "prefill":
+            attention.prefill8(q, cache, meta.plan8, meta.pos, meta.tiles, out=out, row_sq=row_sq)
+            if sample is not None:
+                self._page_turn = getattr(self, "_page_turn", 0) + 1
+                turn = self._page_turn % min(64, meta.plan8.pages.shape[0])
+                replay(lambda: attention.prefill8(q, cache, meta.plan8, meta.pos, meta.sample_tiles, out=out,
+                                                  row_idx=meta.sample_idx, check=self._st(name), pages_from=turn))
+            return
+        plan = self.decode8_plan(q.shape[0], meta.max_ctx)
+        attention.decode8(q, cache, meta.block_table, meta.seq_req, meta.ctx, plan, out=out, row_sq=row_sq)
+        if sample is not None:
+            replay(lambda: attention.decode8(q, cache, meta.block_table, meta.seq_req, meta.ctx, plan, out=out,
+                                             seq_idx=sample, check=self._st(name)))
 
     def read_checks(self, reset: bool = False) -> list[dict]:
         return self.state.read(reset=reset)

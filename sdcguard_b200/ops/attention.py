@@ -222,6 +222,11 @@ def decode8(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_req
     return out
 
 
+def expanded_page(nkv: int) -> int:
+    """bf16 elements of one expanded page of a layer."""
+    return 2 * nkv * PAGE * 128
+
+
 @dataclass
 class Prefill8Plan:
     """The pages of a prefill batch in one list, and the bf16 pages they are expanded to. The same rules as for
@@ -235,7 +240,7 @@ class Prefill8Plan:
 def prefill8_plan(block_table: torch.Tensor, ctx_lens: Sequence[int], nkv: int,
                   work: Optional[torch.Tensor] = None) -> Prefill8Plan:
     """Plan of `prefill8` for requests of ctx_lens keys (cached and new ones) in the rows of block_table. `work`: bf16
-    memory for the expanded pages (at least 4096 nkv elements a page), kept by the caller across layers and steps."""
+    memory for the expanded pages (`expanded_page` elements each), kept by the caller across layers and steps."""
     if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != len(ctx_lens):
         raise ValueError("block_table must be int32 with one row for each of ctx_lens")
     dev, width = block_table.device, block_table.shape[1]
@@ -248,8 +253,9 @@ def prefill8_plan(block_table: torch.Tensor, ctx_lens: Sequence[int], nkv: int,
     place = torch.arange(w)[None]
     used = place < c[:, None]
     table = torch.where(used, first[:, None] + place, 0).to(torch.int32)
-    pages = block_table[:, :w][used.to(dev)].contiguous()
-    need = total * 2 * nkv * PAGE * 128
+    r, j = (t.to(dev, non_blocking=True) for t in used.nonzero(as_tuple=True))
+    pages = block_table[r, j]
+    need = total * expanded_page(nkv)
     if work is None:
         work = torch.empty(need, dtype=torch.bfloat16, device=dev)
     elif work.dtype != torch.bfloat16 or work.numel() < need or not work.is_contiguous() or work.device != dev \

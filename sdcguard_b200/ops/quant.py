@@ -3,14 +3,16 @@
     qw = QuantWeights.quantize(w, bits=4, group=128)     # or QuantWeights(codes, scales, zeros, bits, group)
     layer = CheckedQuantLinear(qw)
     y = layer(x, state, slot)                             # the checked GEMM on the layer's effective weights
+    y = layer(x, state, slot, decode_slot=slot2)          # up to 32 rows: read from the codes (`QuantWeights.matvec`)
+    y = qw.matvec(x)                                      # the same product alone, without checks
 
 A weight-only GEMM dequantizes each weight into bf16 before its fp32 accumulation, so the matrix it multiplies by
 is the effective weight W = rnd((q - z) s) (z: the group's zero point, or 8 / 128 for the symmetric formats), exact
 in bf16. `effective_weight()` builds W on the device (`csrc/quant.cu`, one rounding per element, the same
 arithmetic), the checksum rows come from W, and the checked tcgen05 GEMM multiplies by W: outputs and checks are
 those of the layer's arithmetic. The GEMM reads W in bf16 (built once at load and kept), so this path checks
-quantized layers but does not save their memory at run time; a main loop that expands the codes in shared memory
-is not built.
+quantized layers but does not save their memory at run time. For up to 32 rows `matvec` reads the codes instead: W is
+formed in registers, bit for bit the same, and the bytes read are a quarter.
 
 `fingerprint()` hashes the codes, scales and zero points (the tensors a quantized kernel reads), so a weight scan
 can find a change in the packed weights themselves; `reference_weight()` is the float64 CPU restatement used as the
@@ -200,15 +202,35 @@ class QuantWeights:
 
 class CheckedQuantLinear:
     """A weight-only quantized linear layer on the checked GEMM (effective weights built once, with their
-    checksum rows)."""
+    checksum rows).
+
+    With `decode_slot` (a state slot of its own, `state.add(name, 1)`), calls of up to 32 rows read the 4-bit codes
+    instead of the effective weights (`QuantWeights.matvec`: a quarter of the bytes, which is what a decode step's time
+    is made of); a rotating 1/64 of their outputs is recomputed and compared bit for bit in that slot."""
 
     def __init__(self, qw: QuantWeights, bias: Optional[torch.Tensor] = None):
         self.qw = qw
         self.cw = gemm.CheckedWeight(qw.effective_weight(), bias)
         self.codes_fp = qw.fingerprint()
+        self._samples: Optional[torch.Tensor] = None
+        self._turn = 0
 
-    def __call__(self, x: torch.Tensor, state: torch.Tensor, slot: int, **kw) -> torch.Tensor:
-        return gemm.checked_linear(x, self.cw, state, slot, **kw)
+    def __call__(self, x: torch.Tensor, state: torch.Tensor, slot: int, decode_slot: Optional[int] = None,
+                 **kw) -> torch.Tensor:
+        if decode_slot is None or not 0 < x.shape[0] <= MATVEC_ROWS:
+            return gemm.checked_linear(x, self.cw, state, slot, **kw)
+        if set(kw) - {"out", "row_sq"}:
+            raise ValueError(f"{sorted(set(kw) - {'out', 'row_sq'})}: arguments of the GEMM path")
+        y = self.qw.matvec(x, self.cw.bias, out=kw.get("out"))
+        if self._samples is None:           # row i: blocks i, i + 64, ... of 16 outputs, the sample of every 64th call
+            blocks = -(-self.qw.n // 16)
+            turns = min(64, blocks)
+            per = -(-blocks // turns)
+            self._samples = (torch.arange(turns)[:, None] + turns * torch.arange(per)[None]).to(torch.int32).to(x.device)
+        sample = self._samples[self._turn % self._samples.shape[0]]
+        self._turn += 1
+        self.qw.matvec(x, self.cw.bias, out=y, blocks=sample, check=state[decode_slot])
+        return y
 
     def weights_unchanged(self) -> bool:
         """The packed codes, scales and zero points still hash to what they did at load (one device read)."""

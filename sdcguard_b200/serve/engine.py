@@ -25,7 +25,7 @@ import torch
 
 from ..utils.trace import nvtx_range
 from ..models.decoder import CheckedDecoder, DecoderConfig, StepMeta
-from ..ops import attention
+from ..ops import attention, kv8
 from .guard import ServeGuard
 
 PAGE = 16
@@ -48,7 +48,9 @@ class BlockAllocator:
         self.free.extend(reversed(list(pages)))
 
 
-def kv_bytes_per_page(cfg: DecoderConfig, nkv: int) -> int:
+def kv_bytes_per_page(cfg: DecoderConfig, nkv: int, kv_cache: str = "bf16") -> int:
+    if kv_cache == "fp8":
+        return cfg.layers * kv8.page_bytes(nkv)
     return cfg.layers * 2 * nkv * PAGE * cfg.head_dim * 2
 
 
@@ -100,8 +102,14 @@ class LLMEngine:
     def __init__(self, cfg: DecoderConfig, device="cuda", checked: bool = True, num_blocks: Optional[int] = None,
                  max_prefill_tokens: int = 16384, max_num_seqs: int = 256, sample_every: int = 64,
                  cuda_graph: bool = True, seed: int = 0, kv_fraction: float = 0.6, model: Optional[CheckedDecoder] = None,
-                 max_model_len: int = 4096, precision: str = "bf16", cache: Optional[torch.Tensor] = None):
+                 max_model_len: int = 4096, precision: str = "bf16", cache: Optional[torch.Tensor] = None,
+                 kv_cache: str = "bf16"):
+        """kv_cache "fp8": keys and values are kept in 8 bits with a scale for each page and head (`ops.kv8`): twice the
+        tokens in the same memory, half the bytes of a decode step's attention. `cache` is then a kv8.KV8Cache."""
+        if kv_cache not in ("bf16", "fp8"):
+            raise ValueError(f"kv_cache {kv_cache!r}: bf16 or fp8")
         self.cfg = cfg
+        self.kv_cache = kv_cache
         self.device = torch.device(device)
         # a checked engine trusts this library's kernels on this device only after they reproduced their
         # references on clean and corrupted cases (once per device and process)
@@ -118,23 +126,29 @@ class LLMEngine:
         self.cuda_graph = cuda_graph
         if cache is not None:          # caller-owned KV memory (e.g. a symmetric buffer peers read from)
             want = (cfg.layers, cache.shape[1], 2, self.model.nkv, PAGE, cfg.head_dim)
-            if tuple(cache.shape) != want or cache.dtype != torch.bfloat16:
-                raise ValueError(f"cache must be bf16 {want}, got {tuple(cache.shape)} {cache.dtype}")
+            if kv_cache == "fp8" and not isinstance(cache, kv8.KV8Cache):
+                raise ValueError(f"cache must be a KV8Cache {want} with kv_cache='fp8'")
+            if tuple(cache.shape) != want or (kv_cache == "bf16" and cache.dtype != torch.bfloat16):
+                raise ValueError(f"cache must be {kv_cache} {want}, got {tuple(cache.shape)}")
             num_blocks = cache.shape[1]
             self.cache = cache
         else:
             if num_blocks is None:
                 free, _ = torch.cuda.mem_get_info(self.device)
-                num_blocks = int(free * kv_fraction) // kv_bytes_per_page(cfg, self.model.nkv)
-            self.cache = torch.zeros(cfg.layers, num_blocks, 2, self.model.nkv, PAGE, cfg.head_dim,
-                                     dtype=torch.bfloat16, device=self.device)
+                num_blocks = int(free * kv_fraction) // kv_bytes_per_page(cfg, self.model.nkv, kv_cache)
+            if kv_cache == "fp8":
+                self.cache = kv8.KV8Cache.empty(num_blocks, self.model.nkv, cfg.layers, self.device)
+            else:
+                self.cache = torch.zeros(cfg.layers, num_blocks, 2, self.model.nkv, PAGE, cfg.head_dim,
+                                         dtype=torch.bfloat16, device=self.device)
         self.alloc = BlockAllocator(num_blocks)
         settings = getattr(self.model, "settings", None)
         self.guard = ServeGuard(self.model, z_alarm=settings.z_alarm if settings is not None else 6.0)
         # every activation buffer and the GEMM workspace are sized once, before any CUDA graph is captured
         self.model.buffers(max(max_prefill_tokens, max_num_seqs))
         self.max_model_len = -(-max_model_len // 256) * 256
-        self.model.decode_scratch(max_num_seqs, self.max_model_len)
+        if kv_cache == "bf16":
+            self.model.decode_scratch(max_num_seqs, self.max_model_len)
         self._graphs: dict = {}
         self._graph_kernels: dict = {}     # graph key -> this library's kernels captured in it
         self._graph_replayed = 0           # kernels of this library executed by graph replays
@@ -148,10 +162,13 @@ class LLMEngine:
     def describe(self) -> dict:
         """The engine's configuration as the offline deployment contracts read it (`evidence/config.py`)."""
         from .. import __version__
-        return {"engine": "sdcguard_b200", "version": __version__, "model": self.cfg.name,
-                "kv_pages": int(self.alloc.num_blocks), "page_tokens": PAGE, "max_num_seqs": self.max_num_seqs,
-                "max_model_len": self.max_model_len, "checked": bool(self.checked), "sample_every": self.sample_every,
-                "kv_page_bytes": kv_bytes_per_page(self.cfg, self.model.nkv)}
+        d = {"engine": "sdcguard_b200", "version": __version__, "model": self.cfg.name,
+             "kv_pages": int(self.alloc.num_blocks), "page_tokens": PAGE, "max_num_seqs": self.max_num_seqs,
+             "max_model_len": self.max_model_len, "checked": bool(self.checked), "sample_every": self.sample_every,
+             "kv_page_bytes": kv_bytes_per_page(self.cfg, self.model.nkv, self.kv_cache)}
+        if self.kv_cache != "bf16":
+            d["kv_cache"] = self.kv_cache
+        return d
 
     def startup_line(self) -> str:
         """One line for the startup log: `sdcguard_b200 engine: key=value ...` (parsed by `evidence.config`)."""
@@ -185,6 +202,8 @@ class LLMEngine:
             slots=torch.tensor(slots, dtype=torch.int64).to(dev, non_blocking=True),
             block_table=bt_b, logits_rows=torch.tensor(last, dtype=torch.int64).to(dev, non_blocking=True),
             tiles=tiles.to(dev, non_blocking=True))
+        if self.kv_cache == "fp8":
+            meta.plan8 = self.model.prefill8_plan(bt_b, lens)
         if self.checked:
             # replay sample: per request a run of ceil(n / sample_every) consecutive tokens at an offset that
             # rotates with the step, so successive prefills of a prompt length cover all of it. One run per
@@ -374,6 +393,8 @@ class LLMEngine:
                     slots=torch.tensor([pages[p // PAGE] * PAGE + p % PAGE for p in range(n)], dtype=torch.int64).to(dev),
                     block_table=self.block_tables([pages]), logits_rows=torch.arange(n, dtype=torch.int64).to(dev),
                     tiles=attention.prefill_tiles([0], [n], group).to(dev))
+                if self.kv_cache == "fp8":
+                    meta.plan8 = self.model.prefill8_plan(meta.block_table, [n])
                 logits = self.model.forward(meta, self.cache)
                 v, i = torch.log_softmax(logits.float(), -1).topk(topk, -1)
                 out.append((v.cpu(), i.cpu()))

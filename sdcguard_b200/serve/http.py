@@ -1,7 +1,7 @@
 """HTTP front end of the checked serving engine: an OpenAI-style completions endpoint, Prometheus metrics that say
 from outside whether (and how much) the math is being checked, and a stack-identity record.
 
-    python -m sdcguard_b200.serve.http --model tiny --port 8000 [--unchecked] [--precision fp8]
+    python -m sdcguard_b200.serve.http --model tiny --port 8000 [--unchecked] [--precision fp8] [--kv-cache fp8]
 
 Endpoints
   POST /v1/completions   {"prompt": [token ids] or "text", "max_tokens": n, "stream": false}; greedy decoding. Text
@@ -344,6 +344,8 @@ def main(argv=None) -> int:
     ap.add_argument("--device", default="cuda:0")
     ap.add_argument("--unchecked", action="store_true")
     ap.add_argument("--precision", default="bf16", choices=["bf16", "fp8"])
+    ap.add_argument("--kv-cache", default="bf16", choices=["bf16", "fp8"],
+                    help="fp8: keys and values in 8 bits, a scale for each page of 16 tokens and head")
     ap.add_argument("--max-num-seqs", type=int, default=32)
     ap.add_argument("--max-model-len", type=int, default=2048)
     ap.add_argument("--batch-window-ms", type=float, default=5.0)
@@ -359,7 +361,7 @@ def main(argv=None) -> int:
     cfg = CONFIGS[a.model]
     eng = LLMEngine(cfg, device=a.device, checked=not a.unchecked, max_num_seqs=a.max_num_seqs,
                     max_prefill_tokens=a.max_num_seqs * a.max_model_len // 2, max_model_len=a.max_model_len,
-                    kv_fraction=0.3, seed=a.seed, precision=a.precision)
+                    kv_fraction=0.3, seed=a.seed, precision=a.precision, kv_cache=a.kv_cache)
     srv = Server(eng, cfg.name, a.batch_window_ms, max_prompt=a.max_model_len // 2,
                  weight_scan_mb=a.weight_scan_mb, alerts_path=a.alerts)
     uvicorn.run(make_app(srv), host=a.host, port=a.port, log_level="warning")

@@ -555,3 +555,61 @@ def test_layers_of_a_cache():
     cache = KV8Cache.empty(6, 2, layers=3, device=DEV)
     assert len(cache) == 3 and cache[1].codes.shape == (6, 2, 2, 16, 128) and cache[1] is cache[1]
     assert cache[2].codes.data_ptr() == cache.codes[2].data_ptr() and kv8.page_bytes(2) == 2 * 2 * (2048 + 4)
+
+
+def _engine(**kw):
+    from sdcguard_b200.models.decoder import TINY
+    from sdcguard_b200.serve.engine import LLMEngine
+    return LLMEngine(TINY, device="cuda:0", num_blocks=64, max_prefill_tokens=512, max_num_seqs=8, max_model_len=512,
+                     sample_every=4, kv_cache="fp8", **kw)
+
+
+def test_engine_with_an_8_bit_cache():
+    """Serving with kv_cache="fp8": the checks of append and attention run and stay clean, graph and eager steps give
+    the same tokens, and pages that were used before give them again."""
+    prompts = torch.randint(0, 1024, (5, 70), generator=torch.Generator().manual_seed(0))
+    lens = [70, 33, 16, 1, 48]
+    eng = _engine(checked=True)
+    out = eng.generate(prompts, lens, 20)
+    rows = {r["name"]: r for r in eng.model.read_checks()}
+    for i in range(2):
+        for op in ("rope_kv", "attn"):
+            r = rows[f"layers.{i}.{op} (replay)"]
+            assert r["checks"] > 0 and r["z"] == 0, r
+    assert all(r["z"] < 6 for r in rows.values())
+    assert eng.describe()["kv_cache"] == "fp8" and eng.describe()["kv_page_bytes"] == 2 * kv8.page_bytes(2)
+    eager = _engine(checked=True, cuda_graph=False)
+    assert torch.equal(eager.generate(prompts, lens, 20), out)
+    assert torch.equal(eager.generate(prompts, lens, 20), out)          # pages used before
+    scores = eng.score([prompts[0, :40].tolist()], topk=3)
+    assert scores[0][0].shape == (40, 3) and torch.isfinite(scores[0][0]).all()
+
+
+def test_engine_attention_replay_sees_a_flipped_page():
+    """A code that changes between the attention and its replay is reported in the layer's attention slot."""
+    eng = _engine(checked=True, cuda_graph=False)
+    real, hit = attention.decode8, []
+
+    def flipped(q, cache, *a, **kw):
+        if kw.get("check") is not None and not hit:
+            hit.append(1)
+            cache.codes.view(torch.uint8)[1:, 0] ^= 0x40
+        return real(q, cache, *a, **kw)
+
+    attention.decode8 = flipped
+    try:
+        eng.generate(torch.randint(0, 1024, (2, 20), generator=torch.Generator().manual_seed(0)), [20, 20], 3)
+    finally:
+        attention.decode8 = real
+    z = {r["name"]: r["z"] for r in eng.model.read_checks()}
+    assert hit and z["layers.0.attn (replay)"] == math.inf
+
+
+def test_engine_refuses():
+    from sdcguard_b200.models.decoder import TINY
+    from sdcguard_b200.serve.engine import LLMEngine
+    with pytest.raises(ValueError):
+        LLMEngine(TINY, device="cuda:0", num_blocks=8, kv_cache="int8")
+    with pytest.raises(ValueError):
+        LLMEngine(TINY, device="cuda:0", max_num_seqs=8, kv_cache="fp8",
+                  cache=torch.zeros(2, 8, 2, 2, 16, 128, dtype=torch.bfloat16, device=DEV))

@@ -6,7 +6,8 @@ import math
 import pytest
 import torch
 
-from sdcguard_b200.ops.quant import QuantWeights
+from sdcguard_b200.ops import gemm
+from sdcguard_b200.ops.quant import CheckedQuantLinear, QuantWeights
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -83,3 +84,21 @@ def test_matvec_replay_and_stream():
         a, b = (abft.decode_state_row(r) for r in st.cpu().tolist())
         assert a["z"] == 0 and a["checks"] == 1
         assert b["z"] == math.inf and b["flat"] == (m - 1) * 200 + 199 and b["checks"] == 1
+
+
+def test_checked_layer_reads_the_codes_in_small_batches():
+    qw = _weights(2000, 256, 64, True)
+    bias = torch.randn(2000, device=DEV)
+    layer = CheckedQuantLinear(qw, bias)
+    st = gemm.StateTable(DEV, 2)
+    s0, s1 = st.add("quant (ABFT GEMM)", layer.cw.nb), st.add("quant.decode (replay)", 1)
+    x = torch.randn(40, 256, device=DEV).bfloat16()
+    for _ in range(70):                                   # more turns than there are samples
+        y = layer(x[:5], st.state, s0, decode_slot=s1)
+    assert _holds(y, x[:5], qw, bias) and torch.equal(y, qw.matvec(x[:5], bias))
+    rows = st.read()
+    assert rows[0]["checks"] == 0 and rows[1]["checks"] == 70 and rows[1]["z"] == 0
+    big = layer(x, st.state, s0, decode_slot=s1)          # more rows than matvec takes: the checked GEMM
+    assert st.read()[0]["checks"] > 0 and _holds(big, x, qw, bias)
+    with pytest.raises(ValueError):
+        layer(x[:5], st.state, s0, decode_slot=s1, inject=(0, 0, 1))

@@ -117,6 +117,7 @@ def decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, seq_
 
 
 # ------------------------------------------------------------------------------------ cache in 8 bits (csrc/kv8.cu)
+_SCALE = 1.0 / math.sqrt(128)
 DECODE8_CTAS = 148 * 3      # CTAs of one long sequence: three per SM
 DECODE8_MAX_SEGS = 256
 
@@ -165,8 +166,8 @@ def decode8_plan(nseq: int, nq: int, nkv: int, max_ctx: int, device) -> Decode8P
 
 
 def _want_q(q: torch.Tensor, cache: KV8Cache, out: Optional[torch.Tensor]) -> torch.Tensor:
-    dev = cache.codes.device
-    if cache.codes.dim() != 5:
+    dev = cache.device
+    if len(cache):
         raise ValueError("the cache must be one layer of a KV8Cache")
     kv8.want(q, torch.bfloat16, (q.shape[0], q.shape[1], 128), dev, "q", align=16)
     if out is None:
@@ -193,13 +194,13 @@ def decode8(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_req
     they are recomputed and compared with `out`. row_sq: += ||row||^2 of the output (cleared by the caller; its sum
     over kv heads is taken in no fixed order)."""
     b, nq = q.shape[0], q.shape[1]
-    dev, nkv = cache.codes.device, cache.nkv
+    dev, nkv = cache.device, cache.nkv
     out = _want_q(q, cache, out)
     if (nq, nkv) != (plan.nq, plan.nkv) or b > plan.nseq:
         raise ValueError(f"q {tuple(q.shape)} and {nkv} kv heads do not fit the plan ({plan.nseq} sequences, {plan.nq} "
                          f"query and {plan.nkv} kv heads)")
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.device != dev \
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    if block_table.dtype is not torch.int32 or block_table.device != dev or block_table.dim() != 2 \
+            or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
         raise ValueError("block_table must be int32 (requests, pages) with contiguous rows on the cache's device")
     kv8.want(seq_req, torch.int32, (b,), dev, "seq_req")
     kv8.want(ctx, torch.int32, (b,), dev, "ctx")
@@ -209,16 +210,15 @@ def decode8(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_req
         raise ValueError("check needs seq_idx")
     if plan.part is not None and plan.part.device != dev:
         raise ValueError("the plan must be on the cache's device")
-    _want_extra(row_sq, check, b, dev)
-    with kv8.on(dev):
-        _native.check(_native.lib().sdc_kv8_decode(
-            q.data_ptr(), out.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks,
-            block_table.data_ptr(), block_table.shape[0], block_table.shape[1], block_table.stride(0),
-            seq_req.data_ptr(), ctx.data_ptr(), None if seq_idx is None else seq_idx.data_ptr(),
-            b if seq_idx is None else seq_idx.shape[0], b, nq, nkv, plan.seg_pages, plan.max_segs,
-            1.0 / math.sqrt(128) if scale is None else float(scale), None if plan.part is None else plan.part.data_ptr(),
-            None if row_sq is None else row_sq.data_ptr(), None if check is None else check.data_ptr(), _s(q)),
-            "attention decode (8-bit cache)")
+    if row_sq is not None or check is not None:
+        _want_extra(row_sq, check, b, dev)
+    kv8.launch("sdc_kv8_decode", dev, q.data_ptr(), out.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(),
+               cache.num_blocks, block_table.data_ptr(), block_table.shape[0], block_table.shape[1],
+               block_table.stride(0), seq_req.data_ptr(), ctx.data_ptr(),
+               None if seq_idx is None else seq_idx.data_ptr(), b if seq_idx is None else seq_idx.shape[0], b, nq, nkv,
+               plan.seg_pages, plan.max_segs, _SCALE if scale is None else scale,
+               None if plan.part is None else plan.part.data_ptr(), None if row_sq is None else row_sq.data_ptr(),
+               None if check is None else check.data_ptr())
     return out
 
 
@@ -271,7 +271,7 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
     """`prefill` over a cache of 8 bits: the plan's pages are expanded to bf16 (exact for power-of-two scales), then the
     tensor-core prefill reads those. q (T, nq, 128), tiles from `prefill_tiles`, requests numbered as in the plan. With
     `check`: every pages_step-th expanded page from pages_from on and the rows of the replay tiles are compared."""
-    dev, nkv, nq = cache.codes.device, cache.nkv, q.shape[1]
+    dev, nkv, nq = cache.device, cache.nkv, q.shape[1]
     out = _want_q(q, cache, out)
     t = q.shape[0]
     if nkv != plan.nkv or nq % nkv or ROWS % (nq // nkv) or nq == 0:
@@ -287,13 +287,12 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
     _want_extra(row_sq, check, t, dev)
     if t == 0 or tiles.shape[0] == 0:
         return out
-    with kv8.on(dev):
-        inside = torch.empty(t, dtype=torch.int32, device=dev)      # pos, -1 where it lies outside the plan's table
-        _native.check(_native.lib().sdc_kv8_expand(
-            cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, plan.pages.data_ptr(),
-            plan.pages.shape[0], nkv, plan.work.data_ptr(), pos.data_ptr(), inside.data_ptr(), t,
-            plan.table.shape[1] * PAGE, int(pages_from), int(pages_step), None if check is None else check.data_ptr(),
-            _s(q)), "expanding 8-bit cache pages")
+    inside = torch.empty(t, dtype=torch.int32, device=dev)      # pos, -1 where it lies outside the plan's table
+    kv8.launch("sdc_kv8_expand", dev, cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks,
+               plan.pages.data_ptr(), plan.pages.shape[0], nkv, plan.work.data_ptr(), pos.data_ptr(), inside.data_ptr(),
+               t, plan.table.shape[1] * PAGE, int(pages_from), int(pages_step),
+               None if check is None else check.data_ptr())
+    with torch.cuda.device(dev):
         return prefill(q, plan.work, plan.table, inside, tiles, nq, nkv, out=out, row_idx=row_idx, row_sq=row_sq,
                        scale=scale, check=check)
 

@@ -12,10 +12,11 @@ finite is stored as NaN. The layout is the bf16 cache's, [blocks][2 (K, V)][kv h
 """
 from __future__ import annotations
 
-import contextlib
 from typing import Optional
 
 import torch
+
+from .. import _native
 
 PAGE = 16
 HEAD_DIM = 128
@@ -27,20 +28,27 @@ def want(t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device
          align: int = 1) -> torch.Tensor:
     """t, if it is a contiguous `dtype` tensor of `shape` on `device` on an `align`-byte boundary (a kernel takes its
     address); ValueError otherwise."""
-    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous() or t.data_ptr() % align:
+    if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous() \
+            or (align > 1 and t.data_ptr() % align):
         raise ValueError(f"{name} must be contiguous {dtype} {tuple(shape)} on {device}, aligned to {align} bytes, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t
 
 
-_here = contextlib.nullcontext()
-
-
-def on(device: torch.device):
-    """The context in which a launch on `device` belongs (a kernel starts on the current device)."""
+def launch(entry: str, device: torch.device, *args) -> None:
+    """Calls the library's `entry` with args and `device`'s current stream; a kernel starts on the current device, so
+    another one is made current for the call. (A call of these operators takes a few microseconds on the GPU: the
+    stream is taken as the bare handle, not as an object.)"""
     if device.type != "cuda":
         raise ValueError(f"the kernels run on a CUDA device, not on {device}")
-    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    fn = getattr(_native.lib(), entry)
+    if torch._C._cuda_getDevice() == device.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc:
+        _native.check(rc, entry)
 
 
 class KV8Cache:
@@ -56,7 +64,7 @@ class KV8Cache:
         if scales.dtype != torch.float32 or tuple(scales.shape) != shape or not scales.is_contiguous() \
                 or scales.device != codes.device or scales.data_ptr() % 8:
             raise ValueError(f"scales must be contiguous float32 {shape} on {codes.device}")
-        self.codes, self.scales = codes, scales
+        self.codes, self.scales, self.device = codes, scales, codes.device
         self.num_blocks, self.nkv = codes.shape[-5], codes.shape[-3]
         self._layers = [None] * codes.shape[0] if codes.dim() == 6 else []
 
@@ -80,10 +88,6 @@ class KV8Cache:
     @property
     def shape(self) -> torch.Size:
         return self.codes.shape
-
-    @property
-    def device(self) -> torch.device:
-        return self.codes.device
 
     def values(self, pages: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The stored values in float32 (of one layer; of the given pages): [pages, 2, kv heads, 16, 128]."""

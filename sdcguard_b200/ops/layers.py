@@ -73,15 +73,13 @@ def qk_norm_rope_kv8(qkv: torch.Tensor, nq: int, nkv: int, pos: torch.Tensor, sl
     the cache instead of written; this holds until a later call raises the scale of their page."""
     t = qkv.shape[0]
     heads = nq + 2 * nkv
-    dev = cache.codes.device
-    if cache.codes.dim() != 5 or cache.nkv != nkv:
+    dev = cache.device
+    if len(cache) or cache.nkv != nkv:
         raise ValueError(f"cache must be one layer with {nkv} kv heads, got {tuple(cache.codes.shape)}")
-    if qkv.dim() != 2 or qkv.shape[1] != heads * 128 or qkv.dtype != torch.bfloat16 or qkv.stride(1) != 1 \
-            or (t > 1 and qkv.stride(0) % 4) or qkv.data_ptr() % 8:
-        raise ValueError(f"qkv must be bf16 (T, {heads * 128}) with contiguous rows on 8-byte boundaries")
-    if q_out.shape != (t, nq, 128) or q_out.dtype != torch.bfloat16 or not q_out.is_contiguous() \
-            or q_out.data_ptr() % 8:
-        raise ValueError(f"q_out must be contiguous bf16 ({t}, {nq}, 128)")
+    if qkv.shape != (t, heads * 128) or qkv.dtype is not torch.bfloat16 or qkv.device != dev or qkv.data_ptr() % 8 \
+            or qkv.stride(1) != 1 or (t > 1 and qkv.stride(0) % 4):
+        raise ValueError(f"qkv must be bf16 (T, {heads * 128}) on {dev} with contiguous rows on 8-byte boundaries")
+    kv8.want(q_out, torch.bfloat16, (t, nq, 128), dev, "q_out", align=8)
     kv8.want(pos, torch.int32, (t,), dev, "pos")
     kv8.want(slots, torch.int64, (t,), dev, "slots")
     for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
@@ -97,14 +95,10 @@ def qk_norm_rope_kv8(qkv: torch.Tensor, nq: int, nkv: int, pos: torch.Tensor, sl
         raise ValueError("rows and check go together")
     if rows is not None:
         kv8.want(rows, torch.int32, (rows.shape[0],), dev, "rows")
-    if qkv.device != dev or q_out.device != dev:
-        raise ValueError("qkv, q_out and the cache must be on one device")
-    with kv8.on(dev):
-        _native.check(_native.lib().sdc_kv8_append(
-            qkv.data_ptr(), qkv.stride(0) if t > 1 else heads * 128, t, nq, nkv, pos.data_ptr(), slots.data_ptr(),
-            _p(q_norm), _p(k_norm), float(eps), _p(cos_sin), table_rows, rotary, int(interleaved), q_out.data_ptr(),
-            cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, _p(rows),
-            0 if rows is None else rows.shape[0], _p(check), _s(qkv)), "qk_norm_rope_kv8")
+    kv8.launch("sdc_kv8_append", dev, qkv.data_ptr(), qkv.stride(0) if t > 1 else heads * 128, t, nq, nkv,
+               pos.data_ptr(), slots.data_ptr(), _p(q_norm), _p(k_norm), eps, _p(cos_sin), table_rows, rotary,
+               interleaved, q_out.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks,
+               _p(rows), 0 if rows is None else rows.shape[0], _p(check))
     return q_out
 
 

@@ -163,10 +163,9 @@ class QuantWeights:
         dev, m = self.codes.device, x.shape[0]
         if self.bits != 4 or self.group % 32:
             raise ValueError("matvec reads INT4 codes with groups of a multiple of 32")
-        if not self.codes.is_cuda or not self.codes.is_contiguous() or self.codes.data_ptr() % 16:
-            raise ValueError("the codes must be contiguous on a GPU")
-        if x.dim() != 2 or x.shape[1] != self.k or x.dtype != torch.bfloat16 or x.device != dev or x.stride(1) != 1 \
-                or (m > 1 and x.stride(0) % 8) or x.data_ptr() % 16:
+        kv8.want(self.codes, torch.uint8, (self.n, self.k // 2), dev, "codes", align=16)
+        if x.shape != (m, self.k) or x.dtype is not torch.bfloat16 or x.device != dev or x.data_ptr() % 16 \
+                or x.stride(1) != 1 or (m > 1 and x.stride(0) % 8):
             raise ValueError(f"x must be bf16 (m, {self.k}) on {dev} with contiguous rows on 16-byte boundaries")
         if m > MATVEC_ROWS:
             raise ValueError(f"{m} rows: matvec takes up to {MATVEC_ROWS} (more go to the GEMM on the effective weights)")
@@ -185,13 +184,11 @@ class QuantWeights:
         if blocks is not None:
             kv8.want(blocks, torch.int32, (blocks.shape[0],), dev, "blocks")
         mode = 0 if self.zeros is None else ZERO_MODES.index(self.zero_mode)
-        with kv8.on(dev):
-            _native.check(_native.lib().sdc_matvec4(
-                x.data_ptr(), x.stride(0) if m > 1 else self.k, m, self.n, self.k, self.group, self.codes.data_ptr(),
-                self.scales.data_ptr(), None if self.zeros is None else self.zeros.data_ptr(), mode,
-                None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0) if m > 1 else self.n,
-                None if blocks is None else blocks.data_ptr(), 0 if blocks is None else blocks.shape[0],
-                None if check is None else check.data_ptr(), torch.cuda.current_stream(dev).cuda_stream), "matvec4")
+        kv8.launch("sdc_matvec4", dev, x.data_ptr(), x.stride(0) if m > 1 else self.k, m, self.n, self.k, self.group,
+                   self.codes.data_ptr(), self.scales.data_ptr(), None if self.zeros is None else self.zeros.data_ptr(),
+                   mode, None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0) if m > 1 else self.n,
+                   None if blocks is None else blocks.data_ptr(), 0 if blocks is None else blocks.shape[0],
+                   None if check is None else check.data_ptr())
         return out
 
     def fingerprint(self) -> torch.Tensor:

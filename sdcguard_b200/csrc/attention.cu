@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
 // ---------------------------------------------------------------------------------------------- prefill, ping-pong
 // Two query tiles per CTA that share their key / value tiles (consecutive tiles of one request, so they attend to
 // the same keys), so the tensor pipe always has one tile's MMAs to run while the other tile's softmax runs:
-//   warp 0      TMA: K and V pages of each 128-key tile into one of two stages (shared by both query tiles);
+//   warps 0, 2  TMA: K and V pages of each 128-key tile into one of two stages (shared by both query tiles);
 //   warp 1      MMA, in the order PV0(j-1), S0(j), PV1(j-1), S1(j) for key tile j: S_x = Q_x K_j^T into TMEM,
 //               O_x += P_x V_{j-1} with P_x read from TMEM (the A operand of a tcgen05 MMA may live in tensor
 //               memory), so P never goes through shared memory;
@@ -443,7 +443,7 @@ constexpr int OFF_Q = 0, OFF_K = 2 * TILE_B, OFF_V = 4 * TILE_B, OFF_CTL = 6 * T
 constexpr float RESCALE_LOG2 = 8.f;
 constexpr int PG_BYTES = PAGE * D * 2;
 struct Ctl {
-  uint64_t k_full[2], v_full[2], kv_empty[2];
+  uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2];
   uint64_t s_full[2], p_full[2], o_done[2];   // per query tile
   uint64_t q_ready, drain;
   uint32_t tmem_base;
@@ -474,7 +474,8 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl->k_full[i], 1);
       mbar_init(&ctl->v_full[i], 1);
-      mbar_init(&ctl->kv_empty[i], 1);
+      mbar_init(&ctl->k_empty[i], 1);
+      mbar_init(&ctl->v_empty[i], 1);
       mbar_init(&ctl->s_full[i], 1);
       mbar_init(&ctl->p_full[i], ROWS);
       mbar_init(&ctl->o_done[i], 1);
@@ -514,50 +515,47 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
   volatile int* abort_flag = &ctl->abort_flag;
   const int* bt = p.block_table + static_cast<long long>(req) * p.max_pages;
 
-  if (warp == 0 && ntiles > 0) {
-    // ------------------------------------------------------------ TMA producer (all 32 lanes issue)
+  if ((warp == 0 || warp == 2) && ntiles > 0) {
+    // ------------------------------------------------------------ TMA producers (all 32 lanes issue): warp 0 K, warp 2 V
+    // K's stage is free once S of both query tiles is formed, a softmax and a product before V's: taken apart, the next
+    // K is on its way that much earlier (with one barrier for both, the MMAs waited for K in half of the time)
+    const int kv = warp >> 1;
+    uint64_t* full = kv ? ctl->v_full : ctl->k_full;
+    uint64_t* empty = kv ? ctl->v_empty : ctl->k_empty;
     bool ok = true;
     int last = -1;
     for (int j = 0; j < ntiles && ok; ++j) {
       const int st = j & 1;
       bool got = true;
-      if (lane == 0) got = mbar_wait(&ctl->kv_empty[st], ((j >> 1) & 1u) ^ 1u, abort_flag);
+      if (lane == 0) got = mbar_wait(&empty[st], ((j >> 1) & 1u) ^ 1u, abort_flag);
       if (!__shfl_sync(0xffffffffu, got ? 1 : 0, 0)) {
         ok = false;
         break;
       }
       const int npg = min(KT / PAGE, maxpos / PAGE - j * (KT / PAGE) + 1);
-      uint8_t* kbuf = sm + OFF_K + st * TILE_B;
-      uint8_t* vbuf = sm + OFF_V + st * TILE_B;
-      if (npg < KT / PAGE) {
+      uint8_t* buf = sm + (kv ? OFF_V : OFF_K) + st * TILE_B;
+      if (kv && npg < KT / PAGE) {
         // the weights of keys past the last page are zero, but stale shared memory could hold NaN patterns
         for (int i = lane; i < (KT - npg * PAGE) * 16; i += 32) {
           const int rr = npg * PAGE + (i >> 4), c = i & 15;
-          *reinterpret_cast<uint4*>(vbuf + (c >> 3) * HALF_B + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(buf + (c >> 3) * HALF_B + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
       }
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&ctl->k_full[st], npg * PG_BYTES);
-        mbar_arrive_expect_tx(&ctl->v_full[st], npg * PG_BYTES);
-      }
+      if (lane == 0) mbar_arrive_expect_tx(&full[st], npg * PG_BYTES);
       __syncwarp();
-      if (lane < 4 * npg) {
-        const int pg = lane >> 2, kv = (lane >> 1) & 1, half = lane & 1;
+      if (lane < 2 * npg) {
+        const int pg = lane >> 1, half = lane & 1;
         const long long blk = bt[j * (KT / PAGE) + pg];
         const int row = static_cast<int>(((blk * 2 + kv) * p.nkv + kvh) * PAGE);
-        uint8_t* dst = (kv ? vbuf : kbuf) + half * HALF_B + pg * PAGE * 128;
-        tma_load_2d(dst, &tm, kv ? &ctl->v_full[st] : &ctl->k_full[st], half * 64, row);
+        tma_load_2d(buf + half * HALF_B + pg * PAGE * 128, &tm, &full[st], half * 64, row);
       }
       last = j;
     }
     if (!ok && lane == 0) {
       *abort_flag = 1;
-      for (int j = last > 0 ? last - 1 : 0; j <= last; ++j) {
-        mbar_wait(&ctl->k_full[j & 1], (j >> 1) & 1u, nullptr);
-        mbar_wait(&ctl->v_full[j & 1], (j >> 1) & 1u, nullptr);
-      }
+      for (int j = last > 0 ? last - 1 : 0; j <= last; ++j) mbar_wait(&full[j & 1], (j >> 1) & 1u, nullptr);
     }
   } else if (warp == 1 && ntiles > 0) {
     // ------------------------------------------------------------ MMA issuer
@@ -602,7 +600,8 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
             umma_commit(&ctl->s_full[x]);
           }
         }
-        if (ok && j >= 1) umma_commit(&ctl->kv_empty[(j - 1) & 1]);
+        if (ok && j < ntiles) umma_commit(&ctl->k_empty[j & 1]);
+        if (ok && j >= 1) umma_commit(&ctl->v_empty[(j - 1) & 1]);
       }
       if (!ok) {
         record_error(nullptr, ERR_TIMEOUT_MMA);
@@ -621,13 +620,22 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
     const int head = kvh * G + (r % G);
     const int my_tiles = x ? nt1 : nt0;
     {
-      // Q row -> shared memory (128-byte swizzle, dims halves in separate 16 KB halves of the tile)
+      // the warp's 32 Q rows -> shared memory (128-byte swizzle, dims halves in separate 16 KB halves of the tile), two
+      // whole rows an instruction: a row per lane met 32 cache lines each time and took 5 us of a CTA
       uint8_t* qd = sm + OFF_Q + x * TILE_B;
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (static_cast<long long>(tok < 0 ? 0 : tok) * p.nq + head) * D);
+      const int c = lane & 15;
+      uint4 v[16];
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const uint4 v = tok >= 0 ? src[c] : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(qd + (c >> 3) * HALF_B + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+      for (int i = 0; i < 16; ++i) {
+        const int rr = (warp & 3) * 32 + 2 * i + (lane >> 4), tk = ctl->tok[x][rr];
+        v[i] = tk >= 0 ? *reinterpret_cast<const uint4*>(
+                             p.q + (static_cast<long long>(tk) * p.nq + kvh * G + rr % G) * D + c * 8)
+                       : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int rr = (warp & 3) * 32 + 2 * i + (lane >> 4);
+        *reinterpret_cast<uint4*>(qd + (c >> 3) * HALF_B + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
       }
       fence_proxy_async_smem();
       mbar_arrive(&ctl->q_ready);
@@ -651,20 +659,29 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
       // the weights of keys [64, 128) over columns [96, 128) and those of keys [0, 64) over [64, 96), each written
       // only after the S values under it were read.
       const int lim = pos - kbase;      // keys [0, lim] of this tile are visible to the row
+      // every key visible to every row of the warp (all but a prompt's last tiles): no masks, the same values
+      const bool full = __all_sync(0xffffffffu, lim >= KT - 1);
       uint32_t v[2][32];
-      float mx = -INFINITY;
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (a maximum does not depend on the order)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         tmem_ld32(s_col + h * 64, v[0]);
         tmem_ld32(s_col + h * 64 + 32, v[1]);
         tmem_wait_ld();
+        if (full) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (h * 64 + c * 32 + i <= lim) mx = fmaxf(mx, u32_as_f32(v[c][i]));
+            for (int i = 0; i < 32; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], u32_as_f32(v[c][i]));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (h * 64 + c * 32 + i <= lim) mx4[i & 3] = fmaxf(mx4[i & 3], u32_as_f32(v[c][i]));
         }
       }
+      float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
       mx *= p.scale_log2;                // scale > 0: the maximum commutes with it
       float alpha = 1.f;
       if (mx > -INFINITY && (m_use == -INFINITY || mx > m_use + RESCALE_LOG2)) {
@@ -685,6 +702,7 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
         }
       }
       const bool live = m_use > -INFINITY;
+      const bool plain = full && __all_sync(0xffffffffu, live);
       float ls = 0.f;
 #pragma unroll
       for (int h = 1; h >= 0; --h) {
@@ -696,15 +714,24 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t pk[16];
+          if (plain) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const int key = h * 64 + c * 32 + i;
-            const float p0 = (key <= lim && live) ? ex2(u32_as_f32(v[c][i]) * p.scale_log2 - m_use) : 0.f;
-            const float p1 = (key + 1 <= lim && live) ? ex2(u32_as_f32(v[c][i + 1]) * p.scale_log2 - m_use) : 0.f;
-            const uint32_t w = pack_bf16x2(p0, p1);
-            pk[i >> 1] = w;
-            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
-            ls += f.x + f.y;
+            for (int i = 0; i < 32; i += 2) {
+              const uint32_t w = pack_bf16x2(ex2(u32_as_f32(v[c][i]) * p.scale_log2 - m_use),
+                                             ex2(u32_as_f32(v[c][i + 1]) * p.scale_log2 - m_use));
+              pk[i >> 1] = w;
+              ls += u32_as_f32(w << 16) + u32_as_f32(w & 0xffff0000u);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const int key = h * 64 + c * 32 + i;
+              const float p0 = (key <= lim && live) ? ex2(u32_as_f32(v[c][i]) * p.scale_log2 - m_use) : 0.f;
+              const float p1 = (key + 1 <= lim && live) ? ex2(u32_as_f32(v[c][i + 1]) * p.scale_log2 - m_use) : 0.f;
+              const uint32_t w = pack_bf16x2(p0, p1);
+              pk[i >> 1] = w;
+              ls += u32_as_f32(w << 16) + u32_as_f32(w & 0xffff0000u);
+            }
           }
           tmem_st16(s_col + P_COL + h * 32 + c * 16, pk);
         }
@@ -739,14 +766,20 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
           const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
           sq = fmaf(f.x, f.x, fmaf(f.y, f.y, sq));
         }
-        if (tok >= 0) {
+        if (p.check == nullptr) {
+          // through the Q tile, which the MMAs are done with, to whole rows
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int ch = c * 4 + i;
+            *reinterpret_cast<uint4*>(sm + OFF_Q + x * TILE_B + (ch >> 3) * HALF_B + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) =
+                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          }
+        } else if (tok >= 0) {
           uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const uint4 nv = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-            if (p.check == nullptr) {
-              dst[i] = nv;
-            } else if (bad < 0) {
+            if (bad < 0) {
               const uint4 ov = dst[i];
               const uint32_t a[4] = {nv.x, nv.y, nv.z, nv.w}, b[4] = {ov.x, ov.y, ov.z, ov.w};
 #pragma unroll
@@ -756,6 +789,18 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
               }
             }
           }
+        }
+      }
+      if (p.check == nullptr) {
+        __syncwarp();
+        const int c = lane & 15;
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+          const int rr = (warp & 3) * 32 + 2 * i + (lane >> 4), tk = ctl->tok[x][rr];
+          const uint4 v = *reinterpret_cast<const uint4*>(sm + OFF_Q + x * TILE_B + (c >> 3) * HALF_B + rr * 128 +
+                                                          (((c & 7) ^ (rr & 7)) << 4));
+          if (tk >= 0)
+            *reinterpret_cast<uint4*>(p.o + (static_cast<long long>(tk) * p.nq + kvh * G + rr % G) * D + c * 8) = v;
         }
       }
       if (tok >= 0) {

@@ -621,7 +621,8 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
     const int my_tiles = x ? nt1 : nt0;
     {
       // the warp's 32 Q rows -> shared memory (128-byte swizzle, dims halves in separate 16 KB halves of the tile), two
-      // whole rows an instruction: a row per lane met 32 cache lines each time and took 5 us of a CTA
+      // whole rows an instruction: a row per lane met 32 cache lines each time and took 5 us of a CTA (G divides ROWS, so
+      // it is a power of two)
       uint8_t* qd = sm + OFF_Q + x * TILE_B;
       const int c = lane & 15;
       uint4 v[16];
@@ -629,7 +630,7 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
       for (int i = 0; i < 16; ++i) {
         const int rr = (warp & 3) * 32 + 2 * i + (lane >> 4), tk = ctl->tok[x][rr];
         v[i] = tk >= 0 ? *reinterpret_cast<const uint4*>(
-                             p.q + (static_cast<long long>(tk) * p.nq + kvh * G + rr % G) * D + c * 8)
+                             p.q + (static_cast<long long>(tk) * p.nq + kvh * G + (rr & (G - 1))) * D + c * 8)
                        : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
@@ -800,7 +801,7 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
           const uint4 v = *reinterpret_cast<const uint4*>(sm + OFF_Q + x * TILE_B + (c >> 3) * HALF_B + rr * 128 +
                                                           (((c & 7) ^ (rr & 7)) << 4));
           if (tk >= 0)
-            *reinterpret_cast<uint4*>(p.o + (static_cast<long long>(tk) * p.nq + kvh * G + rr % G) * D + c * 8) = v;
+            *reinterpret_cast<uint4*>(p.o + (static_cast<long long>(tk) * p.nq + kvh * G + (rr & (G - 1))) * D + c * 8) = v;
         }
       }
       if (tok >= 0) {

@@ -28,25 +28,29 @@ def want(t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device
          align: int = 1) -> torch.Tensor:
     """t, if it is a contiguous `dtype` tensor of `shape` on `device` on an `align`-byte boundary (a kernel takes its
     address); ValueError otherwise."""
-    if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous() \
-            or (align > 1 and t.data_ptr() % align):
-        raise ValueError(f"{name} must be contiguous {dtype} {tuple(shape)} on {device}, aligned to {align} bytes, got "
-                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
-    return t
+    if t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous() \
+            and (align == 1 or t.data_ptr() % align == 0):
+        return t
+    raise ValueError(f"{name} must be contiguous {dtype} {tuple(shape)} on {device}, aligned to {align} bytes, got "
+                     f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def launch(entry: str, device: torch.device, *args) -> None:
+_here, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def launch(entry: str, device: torch.device, args: tuple) -> None:
     """Calls the library's `entry` with args and `device`'s current stream; a kernel starts on the current device, so
-    another one is made current for the call. (A call of these operators takes a few microseconds on the GPU: the
-    stream is taken as the bare handle, not as an object.)"""
-    if device.type != "cuda":
+    another one is made current for the call. (These operators run for a few microseconds: the stream is taken as the
+    bare handle, not as an object.)"""
+    index = device.index
+    if index is None:
         raise ValueError(f"the kernels run on a CUDA device, not on {device}")
     fn = getattr(_native.lib(), entry)
-    if torch._C._cuda_getDevice() == device.index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if _here() == index:
+        rc = fn(*args, _stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream(index))
     if rc:
         _native.check(rc, entry)
 
@@ -65,6 +69,7 @@ class KV8Cache:
                 or scales.device != codes.device or scales.data_ptr() % 8:
             raise ValueError(f"scales must be contiguous float32 {shape} on {codes.device}")
         self.codes, self.scales, self.device = codes, scales, codes.device
+        self.one_layer = codes.dim() == 5
         self.num_blocks, self.nkv = codes.shape[-5], codes.shape[-3]
         self._layers = [None] * codes.shape[0] if codes.dim() == 6 else []
 

@@ -74,7 +74,7 @@ def qk_norm_rope_kv8(qkv: torch.Tensor, nq: int, nkv: int, pos: torch.Tensor, sl
     t = qkv.shape[0]
     heads = nq + 2 * nkv
     dev = cache.device
-    if len(cache) or cache.nkv != nkv:
+    if not cache.one_layer or cache.nkv != nkv:
         raise ValueError(f"cache must be one layer with {nkv} kv heads, got {tuple(cache.codes.shape)}")
     if qkv.shape != (t, heads * 128) or qkv.dtype is not torch.bfloat16 or qkv.device != dev or qkv.data_ptr() % 8 \
             or qkv.stride(1) != 1 or (t > 1 and qkv.stride(0) % 4):
@@ -95,10 +95,10 @@ def qk_norm_rope_kv8(qkv: torch.Tensor, nq: int, nkv: int, pos: torch.Tensor, sl
         raise ValueError("rows and check go together")
     if rows is not None:
         kv8.want(rows, torch.int32, (rows.shape[0],), dev, "rows")
-    kv8.launch("sdc_kv8_append", dev, qkv.data_ptr(), qkv.stride(0) if t > 1 else heads * 128, t, nq, nkv,
-               pos.data_ptr(), slots.data_ptr(), _p(q_norm), _p(k_norm), eps, _p(cos_sin), table_rows, rotary,
-               interleaved, q_out.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks,
-               _p(rows), 0 if rows is None else rows.shape[0], _p(check))
+    kv8.launch("sdc_kv8_append", dev, (qkv.data_ptr(), qkv.stride(0) if t > 1 else heads * 128, t, nq, nkv,
+                pos.data_ptr(), slots.data_ptr(), _p(q_norm), _p(k_norm), eps, _p(cos_sin), table_rows, rotary,
+                interleaved, q_out.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks,
+                _p(rows), 0 if rows is None else rows.shape[0], _p(check)))
     return q_out
 
 

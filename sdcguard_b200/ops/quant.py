@@ -184,11 +184,11 @@ class QuantWeights:
         if blocks is not None:
             kv8.want(blocks, torch.int32, (blocks.shape[0],), dev, "blocks")
         mode = 0 if self.zeros is None else ZERO_MODES.index(self.zero_mode)
-        kv8.launch("sdc_matvec4", dev, x.data_ptr(), x.stride(0) if m > 1 else self.k, m, self.n, self.k, self.group,
-                   self.codes.data_ptr(), self.scales.data_ptr(), None if self.zeros is None else self.zeros.data_ptr(),
-                   mode, None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0) if m > 1 else self.n,
-                   None if blocks is None else blocks.data_ptr(), 0 if blocks is None else blocks.shape[0],
-                   None if check is None else check.data_ptr())
+        kv8.launch("sdc_matvec4", dev, (x.data_ptr(), x.stride(0) if m > 1 else self.k, m, self.n, self.k, self.group,
+                    self.codes.data_ptr(), self.scales.data_ptr(), None if self.zeros is None else self.zeros.data_ptr(),
+                    mode, None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0) if m > 1 else self.n,
+                    None if blocks is None else blocks.data_ptr(), 0 if blocks is None else blocks.shape[0],
+                    None if check is None else check.data_ptr()))
         return out
 
     def fingerprint(self) -> torch.Tensor:

@@ -123,7 +123,7 @@ SIGNATURES: dict[str, tuple] = {
     "sdc_kv8_append": (I, [P, L, I, I, I, P, P, P, P, DBL, P, I, I, I, P, P, P, L, P, I, P, P]),
     "sdc_kv8_expand": (I, [P, P, L, P, I, I, P, P, P, I, I, I, I, P, P]),
     "sdc_kv8_decode": (I, [P, P, P, P, L, P, I, I, L, P, P, P, I, I, I, I, I, I, F, P, P, P, P]),
-    "sdc_matvec4": (I, [P, L, I, I, I, I, P, P, P, I, P, P, L, P, I, P, P]),
+    "sdc_matvec4": (I, [P, L, I, I, I, I, P, P, P, I, P, P, L, P, P, I, P, P]),
     "sdc_ep_receive_grouped": (I, [P, P, P, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P, P]),
 }
 

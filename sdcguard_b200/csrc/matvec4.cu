@@ -36,6 +36,7 @@ struct Params {
   long long ldy;
   int M, N, K, ng;
   float per_group;                 // 32 / group
+  uint4* packed;                   // x in the order the products take it (pack_x), or null: read from x
   const int* blocks;               // check mode: blocks of 16 outputs
   unsigned long long* check;
 };
@@ -94,9 +95,25 @@ __device__ __forceinline__ uint32_t weights(uint32_t q, const Factor& f) {
   if (MODE == ZERO_TWO) return as_u32(__hadd2_rn(__hmul2_rn(v, f.s), f.add));
   return as_u32(__hfma2(v, f.s, f.add));
 }
+// x for `PACKED` products: for each block of 128 k, word c of the codes and group j of eight rows, the four pairs of every
+// lane side by side. With more than eight rows each CTA reads more bytes of x than of codes, 16 at a time from 32 places;
+// packed once, they come in whole lines and without permutes.
+__device__ __forceinline__ uint4 pairs_of(const uint4& x) {
+  return make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632),     // (x0, x4), (x1, x5)
+                    __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));    // (x2, x6), (x3, x7)
+}
+template <int NT>
+__global__ void __launch_bounds__(256) pack_x_kernel(const Params p) {
+  pdl_trigger();
+  const int i = blockIdx.x * 256 + threadIdx.x, lane = i & 31, j = (i >> 5) % NT, kc = (i >> 5) / NT;
+  const int k = (kc >> 2) * KB + 32 * (lane & 3) + 8 * (kc & 3), m = j * 8 + (lane >> 2);
+  if ((kc >> 2) * KB >= p.K) return;
+  p.packed[i] = k < p.K && m < p.M ? pairs_of(*reinterpret_cast<const uint4*>(p.x + m * p.ldx + k)) : make_uint4(0, 0, 0, 0);
+}
+
 // NT: groups of eight rows of x; MT: groups of 16 outputs; PF: k blocks in flight per warp. Outputs behind N and rows of
 // x behind M are computed from the last ones there are and not written, which costs no predicates in the loop.
-template <int NT, int MT, int WARPS, int PF, int CTAS, int MODE>
+template <int NT, int MT, int WARPS, int PF, int CTAS, int MODE, bool PACKED>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) matvec4_kernel(const Params p) {
   pdl_trigger();
   __shared__ float red[SLICES][NT * 8][MT * 16 + 1];
@@ -116,6 +133,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) matvec4_kernel(const Params 
       meta[i][r] = n * p.ng;
     }
   const __nv_bfloat16* xrow[NT];
+  if (!PACKED)
 #pragma unroll
   for (int j = 0; j < NT; ++j) xrow[j] = p.x + min(j * 8 + g, p.M - 1) * p.ldx;
   uint4 w[PF][MT][2];                    // a lane's 32 codes, scale and zero point of 2 MT outputs
@@ -141,6 +159,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) matvec4_kernel(const Params 
   };
 #pragma unroll
   for (int f = 0; f < PF; ++f) load_next(f);
+  if (PACKED) pdl_wait();                // the codes are on their way meanwhile
   for (int slice = warp; slice < SLICES; slice += WARPS) {
     float acc[MT][NT][4];
 #pragma unroll
@@ -156,6 +175,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) matvec4_kernel(const Params 
         if (kc < nkb) {                  // (uniform)
           const int k = kc * KB + 32 * t;
           const uint4* xp[NT];
+          if (!PACKED)
 #pragma unroll
           for (int j = 0; j < NT; ++j) xp[j] = k < p.K ? reinterpret_cast<const uint4*>(xrow[j] + k) : no_x;
           Factor lo[MT][2];
@@ -168,11 +188,11 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) matvec4_kernel(const Params 
             uint32_t b[NT][4];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              const uint4 x = __ldg(xp[j] + c);
-              b[j][0] = __byte_perm(x.x, x.z, 0x5410);    // x0, x4
-              b[j][1] = __byte_perm(x.x, x.z, 0x7632);    // x1, x5
-              b[j][2] = __byte_perm(x.y, x.w, 0x5410);    // x2, x6
-              b[j][3] = __byte_perm(x.y, x.w, 0x7632);    // x3, x7
+              const uint4 x = PACKED ? p.packed[((kc * 4 + c) * NT + j) * 32 + lane] : pairs_of(__ldg(xp[j] + c));
+              b[j][0] = x.x;
+              b[j][1] = x.y;
+              b[j][2] = x.z;
+              b[j][3] = x.w;
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
@@ -221,17 +241,33 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) matvec4_kernel(const Params 
   }
 }
 
-template <int NT, int MT, int WARPS, int PF, int CTAS>
-static int launch(const Params& p, int mode, int grid, cudaStream_t st) {
-  switch (mode) {
-    case ZERO_SUBTRACT:
-      if (p.zeros == nullptr) matvec4_kernel<NT, MT, WARPS, PF, CTAS, ZERO_EIGHT><<<grid, WARPS * 32, 0, st>>>(p);
-      else matvec4_kernel<NT, MT, WARPS, PF, CTAS, ZERO_SUBTRACT><<<grid, WARPS * 32, 0, st>>>(p);
-      break;
-    case ZERO_FMA: matvec4_kernel<NT, MT, WARPS, PF, CTAS, ZERO_FMA><<<grid, WARPS * 32, 0, st>>>(p); break;
-    default: matvec4_kernel<NT, MT, WARPS, PF, CTAS, ZERO_TWO><<<grid, WARPS * 32, 0, st>>>(p); break;
+template <int NT, int MT, int WARPS, int PF, int CTAS, int MODE, bool PACKED>
+static int launch_mode(const Params& p, int grid, cudaStream_t st) {
+  if (!PACKED) {
+    matvec4_kernel<NT, MT, WARPS, PF, CTAS, MODE, false><<<grid, WARPS * 32, 0, st>>>(p);
+    return static_cast<int>(cudaGetLastError());
   }
-  return static_cast<int>(cudaGetLastError());
+  const int nkb = (p.K + KB - 1) / KB;
+  pack_x_kernel<NT><<<(nkb * 4 * NT * 32 + 255) / 256, 256, 0, st>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return static_cast<int>(e);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, matvec4_kernel<NT, MT, WARPS, PF, CTAS, MODE, PACKED>, p));
+}
+template <int NT, int MT, int WARPS, int PF, int CTAS, bool PACKED = false>
+static int launch(const Params& p, int mode, int grid, cudaStream_t st) {
+  if (mode == ZERO_FMA) return launch_mode<NT, MT, WARPS, PF, CTAS, ZERO_FMA, PACKED>(p, grid, st);
+  if (mode == ZERO_TWO) return launch_mode<NT, MT, WARPS, PF, CTAS, ZERO_TWO, PACKED>(p, grid, st);
+  if (p.zeros != nullptr) return launch_mode<NT, MT, WARPS, PF, CTAS, ZERO_SUBTRACT, PACKED>(p, grid, st);
+  return launch_mode<NT, MT, WARPS, PF, CTAS, ZERO_EIGHT, PACKED>(p, grid, st);
 }
 
 }  // namespace matvec4
@@ -241,7 +277,7 @@ using namespace sdc::matvec4;
 
 extern "C" int sdc_matvec4(const void* x, long long ldx, int M, int N, int K, int group, const void* codes,
                            const void* scales, const void* zeros, int mode, const void* bias, void* y,
-                           long long ldy, const int* blocks, int nblocks, void* check, void* stream) {
+                           long long ldy, void* packed, const int* blocks, int nblocks, void* check, void* stream) {
   if (M <= 0 || N <= 0) return 0;
   // scale indices fit 32 bits, and (k / 32 + 1/2) * (32 / group) in fp32 finds a k's group up to K = 2^25
   if (static_cast<long long>(N) * (K / 32) > 0x7fffffffll || K > (1 << 25)) return -1;
@@ -262,6 +298,7 @@ extern "C" int sdc_matvec4(const void* x, long long ldx, int M, int N, int K, in
   p.K = K;
   p.ng = K / group;
   p.per_group = 32.f / static_cast<float>(group);
+  p.packed = static_cast<uint4*>(packed);
   p.blocks = blocks;
   p.check = static_cast<unsigned long long*>(check);
   auto st = static_cast<cudaStream_t>(stream);
@@ -271,6 +308,7 @@ extern "C" int sdc_matvec4(const void* x, long long ldx, int M, int N, int K, in
                   : M <= 16 ? launch<2, 1, 8, 2, 3>(p, mode, nblocks, st) : launch<4, 1, 8, 2, 2>(p, mode, nblocks, st);
   }
   if (M <= 8) return launch<1, 1, 8, 2, 4>(p, mode, (N + 15) / 16, st);
-  if (M <= 16) return launch<2, 2, 8, 1, 2>(p, mode, (N + 31) / 32, st);
-  return launch<4, 2, 8, 2, 1>(p, mode, (N + 31) / 32, st);
+  if (M <= 16)
+    return packed ? launch<2, 2, 8, 1, 2, true>(p, mode, (N + 31) / 32, st) : launch<2, 2, 8, 1, 2>(p, mode, (N + 31) / 32, st);
+  return packed ? launch<4, 2, 8, 2, 1, true>(p, mode, (N + 31) / 32, st) : launch<4, 2, 8, 2, 1>(p, mode, (N + 31) / 32, st);
 }

@@ -74,7 +74,8 @@ struct AppendParams {
   const long long* slots;     // [T] block * 16 + place; negative: not stored
   const __nv_bfloat16* qw;
   const __nv_bfloat16* kw;
-  double eps;
+  double eps;                 // keys decided in double
+  float epsf;
   const float2* cs;           // [table_rows][rotary / 2] (cos, sin)
   int table_rows, rotary;
   __nv_bfloat16* q_out;       // [T][nq][128]
@@ -173,11 +174,11 @@ __device__ __forceinline__ T half_warp_sum(T v) {
 
 // 1 / sqrt(mean of squares + eps) of the row a half warp holds.
 template <typename T>
-__device__ __forceinline__ T norm_of(const T (&v)[8], double eps) {
+__device__ __forceinline__ T norm_of(const T (&v)[8], T eps) {
   T ss = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
-  return rsqrt(half_warp_sum(ss) / static_cast<T>(D) + static_cast<T>(eps));
+  return rsqrt(half_warp_sum(ss) * static_cast<T>(1.0 / D) + eps);
 }
 // Rotates the pairs (v[i], v[4 + i]) by c: four cosines, four sines (1 and 0 where nothing is rotated).
 template <typename T>
@@ -296,7 +297,7 @@ __device__ __forceinline__ void append_queries(const AppendParams& p, int group,
     float v[8];
     L.unpack(raw[j], v);
     if (p.qw != nullptr) {
-      const float inv = norm_of(v, p.eps);
+      const float inv = norm_of(v, p.epsf);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
     }
@@ -317,6 +318,9 @@ __device__ __forceinline__ void append_keys_values(const AppendParams& p, int t0
   const __nv_bfloat16* col = p.qkv + static_cast<long long>(p.nq + u) * D;
   const RowLane<INTER> L(l, p.rotary);
   const RowLane<false> V(l, 0);                            // dims 8l .. 8l + 7 in order
+  // the group's rows are on their way to L2 before its slots say which of them this warp stores
+  if (t0 + (lane >> 1) < p.T && lane < 2 * TG)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(col + (t0 + (lane >> 1)) * p.ld + (lane & 1) * 64));
   // lane j looks at token t0 - 1 + j: the token before the group, the group, and the tokens a run may reach behind it
   const int tl = t0 - 1 + lane;
   const bool look = lane < TG + PAGE && tl >= 0 && tl < p.T;
@@ -358,7 +362,7 @@ __device__ __forceinline__ void append_keys_values(const AppendParams& p, int t0
           L.unpack(raw[j], v);
           L.angles(angles_of(p, pos), c);
           if (norm) {
-            const float inv = norm_of(v, p.eps);
+            const float inv = norm_of(v, p.epsf);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
           }
@@ -418,6 +422,7 @@ __device__ __forceinline__ void append_keys_values(const AppendParams& p, int t0
       }
       __syncwarp();
     } else {
+      __nv_bfloat162 top = __float2bfloat162_rn(0.f);        // (the maximum passes over NaN)
 #pragma unroll 1
       for (int j0 = 0; 2 * j0 < len; j0 += 4) {
         uint4 raw[4];
@@ -426,12 +431,13 @@ __device__ __forceinline__ void append_keys_values(const AppendParams& p, int t0
           raw[j] = 2 * (j0 + j) + hw < len ? V.load(rows + (2 * (j0 + j) + hw) * p.ld) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float v[8];
-          V.unpack(raw[j], v);
-          m = amax_of(v, m);
           *reinterpret_cast<uint4*>(&keep[j0 + j][0][lane]) = raw[j];
+          const uint32_t x[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&x[i])));
         }
       }
+      m = fmaxf(__low2float(top), __high2float(top));
       m = warp_max(m);
       const bool inf = m > FLOAT_MAX;                      // then the largest finite one
       if (inf) {
@@ -514,7 +520,7 @@ __global__ void __launch_bounds__(256) kv8_append_check_kernel(const AppendParam
     float c[8];
     L.angles(angles_of(p, pos), c);
     if (nw != nullptr) {
-      const float inv = norm_of(v, p.eps);
+      const float inv = norm_of(v, p.epsf);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
     }
@@ -1139,6 +1145,7 @@ int sdc_kv8_append(const void* qkv, long long ld, int T, int nq, int nkv, const 
   p.qw = static_cast<const __nv_bfloat16*>(qw);
   p.kw = static_cast<const __nv_bfloat16*>(kw);
   p.eps = eps;
+  p.epsf = static_cast<float>(eps);
   p.cs = static_cast<const float2*>(cos_sin);
   p.table_rows = table_rows;
   p.rotary = rotary;

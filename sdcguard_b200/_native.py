@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from ctypes import c_float, c_int, c_longlong, c_uint, c_void_p
 from pathlib import Path
@@ -55,7 +56,6 @@ L = c_longlong
 U = c_uint
 U64 = ctypes.c_ulonglong
 F = c_float
-DBL = ctypes.c_double
 
 # name -> (restype, argtypes)
 SIGNATURES: dict[str, tuple] = {
@@ -120,11 +120,19 @@ SIGNATURES: dict[str, tuple] = {
     "sdc_dequant_weights": (I, [P, I, I, I, I, P, P, I, P, P]),
     "sdc_gemm_fp8_grouped": (I, [P, P, P, P, P, I, I, I, I, P, L, P, P, P, P, P, I, U, U, U, U, F, F, F, F, F, P, I,
                                  I, U, P]),
-    "sdc_kv8_append": (I, [P, L, I, I, I, P, P, P, P, DBL, P, I, I, I, P, P, P, L, P, I, P, P]),
-    "sdc_kv8_expand": (I, [P, P, L, P, I, I, P, P, P, I, I, I, I, P, P]),
-    "sdc_kv8_decode": (I, [P, P, P, P, L, P, I, I, L, P, P, P, I, I, I, I, I, I, F, P, P, P, P]),
-    "sdc_matvec4": (I, [P, L, I, I, I, I, P, P, P, I, P, P, L, P, P, I, P, P]),
+    "sdc_kv8_append": (I, [P]),
+    "sdc_kv8_expand": (I, [P]),
+    "sdc_kv8_decode": (I, [P]),
+    "sdc_matvec4": (I, [P]),
     "sdc_ep_receive_grouped": (I, [P, P, P, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P, P]),
+}
+
+# entry points that take their arguments in one struct: its layout (native alignment)
+STRUCTS: dict[str, struct.Struct] = {
+    "sdc_kv8_append": struct.Struct("@PqiiiPPPPdPiiiPPPqPiPP"),
+    "sdc_kv8_expand": struct.Struct("@PPqPiiPPPiiiiPP"),
+    "sdc_kv8_decode": struct.Struct("@PPPPqPiiqPPPiiiiiifPPPP"),
+    "sdc_matvec4": struct.Struct("@PqiiiiPPPiPPqPPiPP"),
 }
 
 

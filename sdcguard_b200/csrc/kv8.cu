@@ -1125,12 +1125,37 @@ static int launch_decode(const CUtensorMap& tm, const DecodeParams& p, int nrun,
 
 using namespace sdc::kv8;
 
+// Each entry takes its arguments in one struct, natural alignment: through ctypes a call costs microseconds less than
+// with twenty arguments, which is what the smallest calls are made of.
 extern "C" {
 
-int sdc_kv8_append(const void* qkv, long long ld, int T, int nq, int nkv, const int* pos, const long long* slots,
-                   const void* qw, const void* kw, double eps, const void* cos_sin, int table_rows, int rotary,
-                   int interleaved, void* q_out, void* codes, void* scales, long long num_blocks, const int* rows,
-                   int nrows, void* check, void* stream) {
+struct Kv8AppendArgs {
+  const void* qkv;
+  long long ld;
+  int T;
+  int nq;
+  int nkv;
+  const int* pos;
+  const long long* slots;
+  const void* qw;
+  const void* kw;
+  double eps;
+  const void* cos_sin;
+  int table_rows;
+  int rotary;
+  int interleaved;
+  void* q_out;
+  void* codes;
+  void* scales;
+  long long num_blocks;
+  const int* rows;
+  int nrows;
+  void* check;
+  void* stream;
+};
+int sdc_kv8_append(const Kv8AppendArgs* args) {
+  const auto& [qkv, ld, T, nq, nkv, pos, slots, qw, kw, eps, cos_sin, table_rows, rotary, interleaved, q_out,
+               codes, scales, num_blocks, rows, nrows, check, stream] = *args;
   if (T <= 0 || (check != nullptr && nrows <= 0)) return 0;
   if (ld % 4 || rotary < 0 || rotary > D || rotary % 8 || nq < 0 || nkv < 1 || (check != nullptr) != (rows != nullptr))
     return -1;
@@ -1175,9 +1200,26 @@ int sdc_kv8_append(const void* qkv, long long ld, int T, int nq, int nkv, const 
   return static_cast<int>(cudaGetLastError());
 }
 
-int sdc_kv8_expand(const void* codes, const void* scales, long long num_blocks, const int* pages, int npages, int nkv,
-                   void* out, const int* pos, int* pos_out, int T, int limit, int from, int step, void* check,
-                   void* stream) {
+struct Kv8ExpandArgs {
+  const void* codes;
+  const void* scales;
+  long long num_blocks;
+  const int* pages;
+  int npages;
+  int nkv;
+  void* out;
+  const int* pos;
+  int* pos_out;
+  int T;
+  int limit;
+  int from;
+  int step;
+  void* check;
+  void* stream;
+};
+int sdc_kv8_expand(const Kv8ExpandArgs* args) {
+  const auto& [codes, scales, num_blocks, pages, npages, nkv, out, pos, pos_out, T, limit, from, step, check,
+               stream] = *args;
   if (npages <= 0) return 0;
   if (nkv < 1 || num_blocks < 1 || (check != nullptr && (from < 0 || step < 1))) return -1;
   ExpandParams p;
@@ -1203,10 +1245,34 @@ int sdc_kv8_expand(const void* codes, const void* scales, long long num_blocks, 
 
 // part: nseqs * nkv * max_segs * (nq / nkv) * 132 floats (not read where max_segs is 1); rows of `nrun` sequences are
 // computed: seq_idx's, or the first nrun.
-int sdc_kv8_decode(const void* q, void* o, const void* codes, const void* scales, long long num_blocks,
-                   const int* table, int table_rows, int max_pages, long long table_ld, const int* seq_req,
-                   const int* ctx, const int* seq_idx, int nrun, int nseqs, int nq, int nkv, int seg_pages,
-                   int max_segs, float scale, void* part, void* row_sq, void* check, void* stream) {
+struct Kv8DecodeArgs {
+  const void* q;
+  void* o;
+  const void* codes;
+  const void* scales;
+  long long num_blocks;
+  const int* table;
+  int table_rows;
+  int max_pages;
+  long long table_ld;
+  const int* seq_req;
+  const int* ctx;
+  const int* seq_idx;
+  int nrun;
+  int nseqs;
+  int nq;
+  int nkv;
+  int seg_pages;
+  int max_segs;
+  float scale;
+  void* part;
+  void* row_sq;
+  void* check;
+  void* stream;
+};
+int sdc_kv8_decode(const Kv8DecodeArgs* args) {
+  const auto& [q, o, codes, scales, num_blocks, table, table_rows, max_pages, table_ld, seq_req, ctx, seq_idx,
+               nrun, nseqs, nq, nkv, seg_pages, max_segs, scale, part, row_sq, check, stream] = *args;
   if (nrun <= 0) return 0;
   if (nkv < 1 || nq % nkv || nq / nkv < 1 || nq / nkv > 16 || seg_pages < 1 || max_segs < 1 || max_segs > MAX_SEGS ||
       (max_segs > 1 && part == nullptr) || (check != nullptr && seq_idx == nullptr) ||

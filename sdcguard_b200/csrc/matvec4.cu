@@ -275,9 +275,30 @@ static int launch(const Params& p, int mode, int grid, cudaStream_t st) {
 
 using namespace sdc::matvec4;
 
-extern "C" int sdc_matvec4(const void* x, long long ldx, int M, int N, int K, int group, const void* codes,
-                           const void* scales, const void* zeros, int mode, const void* bias, void* y,
-                           long long ldy, void* packed, const int* blocks, int nblocks, void* check, void* stream) {
+// The arguments in one struct (see kv8.cu).
+struct Matvec4Args {
+  const void* x;
+  long long ldx;
+  int M;
+  int N;
+  int K;
+  int group;
+  const void* codes;
+  const void* scales;
+  const void* zeros;
+  int mode;
+  const void* bias;
+  void* y;
+  long long ldy;
+  void* packed;
+  const int* blocks;
+  int nblocks;
+  void* check;
+  void* stream;
+};
+extern "C" int sdc_matvec4(const Matvec4Args* args) {
+  const auto& [x, ldx, M, N, K, group, codes, scales, zeros, mode, bias, y, ldy, packed, blocks, nblocks,
+               check, stream] = *args;
   if (M <= 0 || N <= 0) return 0;
   // scale indices fit 32 bits, and (k / 32 + 1/2) * (32 / group) in fp32 finds a k's group up to K = 2^25
   if (static_cast<long long>(N) * (K / 32) > 0x7fffffffll || K > (1 << 25)) return -1;

@@ -212,13 +212,11 @@ def decode8(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_req
         raise ValueError("the plan must be on the cache's device")
     if row_sq is not None or check is not None:
         _want_extra(row_sq, check, b, dev)
-    kv8.launch("sdc_kv8_decode", dev, (q.data_ptr(), out.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(),
-                cache.num_blocks, block_table.data_ptr(), block_table.shape[0], block_table.shape[1],
-                block_table.stride(0), seq_req.data_ptr(), ctx.data_ptr(),
-                None if seq_idx is None else seq_idx.data_ptr(), b if seq_idx is None else seq_idx.shape[0], b, nq, nkv,
-                plan.seg_pages, plan.max_segs, _SCALE if scale is None else scale,
-                None if plan.part is None else plan.part.data_ptr(), None if row_sq is None else row_sq.data_ptr(),
-                None if check is None else check.data_ptr()))
+    kv8.launch("sdc_kv8_decode", dev, (
+        q.data_ptr(), out.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks,
+        block_table.data_ptr(), block_table.shape[0], block_table.shape[1], block_table.stride(0), seq_req.data_ptr(),
+        ctx.data_ptr(), kv8.ptr(seq_idx), b if seq_idx is None else seq_idx.shape[0], b, nq, nkv, plan.seg_pages,
+        plan.max_segs, _SCALE if scale is None else scale, kv8.ptr(plan.part), kv8.ptr(row_sq), kv8.ptr(check)))
     return out
 
 
@@ -288,11 +286,11 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
     if t == 0 or tiles.shape[0] == 0:
         return out
     inside = torch.empty(t, dtype=torch.int32, device=dev)      # pos, -1 where it lies outside the plan's table
-    kv8.launch("sdc_kv8_expand", dev, (cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks,
-                plan.pages.data_ptr(), plan.pages.shape[0], nkv, plan.work.data_ptr(), pos.data_ptr(), inside.data_ptr(),
-                t, plan.table.shape[1] * PAGE, int(pages_from), int(pages_step),
-                None if check is None else check.data_ptr()))
-    with torch.cuda.device(dev):
+    kv8.launch("sdc_kv8_expand", dev, (
+        cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, plan.pages.data_ptr(), plan.pages.shape[0],
+        nkv, plan.work.data_ptr(), pos.data_ptr(), inside.data_ptr(), t, plan.table.shape[1] * PAGE, pages_from,
+        pages_step, kv8.ptr(check)))
+    with kv8.on(dev):
         return prefill(q, plan.work, plan.table, inside, tiles, nq, nkv, out=out, row_idx=row_idx, row_sq=row_sq,
                        scale=scale, check=check)
 

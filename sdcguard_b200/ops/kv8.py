@@ -12,6 +12,7 @@ finite is stored as NaN. The layout is the bf16 cache's, [blocks][2 (K, V)][kv h
 """
 from __future__ import annotations
 
+import contextlib
 from typing import Optional
 
 import torch
@@ -38,21 +39,28 @@ def want(t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device
 _here, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-def launch(entry: str, device: torch.device, args: tuple) -> None:
-    """Calls the library's `entry` with args and `device`'s current stream; a kernel starts on the current device, so
-    another one is made current for the call. (These operators run for a few microseconds: the stream is taken as the
-    bare handle, not as an object.)"""
-    index = device.index
-    if index is None:
+_same = contextlib.nullcontext()
+
+
+def on(device: torch.device):
+    """The context in which a launch on `device` belongs: a kernel starts on the current device."""
+    if device.index is None:
         raise ValueError(f"the kernels run on a CUDA device, not on {device}")
-    fn = getattr(_native.lib(), entry)
-    if _here() == index:
-        rc = fn(*args, _stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _stream(index))
+    return _same if _here() == device.index else torch.cuda.device(device.index)
+
+
+def launch(entry: str, device: torch.device, args: tuple) -> None:
+    """Calls the library's `entry` with args (addresses as integers, 0 for none) and `device`'s current stream. (These
+    operators run for a few microseconds: the arguments cross as one struct, and the stream is taken as the bare
+    handle.)"""
+    with on(device):
+        rc = getattr(_native.lib(), entry)(_native.STRUCTS[entry].pack(*args, _stream(device.index)))
     if rc:
         _native.check(rc, entry)
+
+
+def ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 class KV8Cache:

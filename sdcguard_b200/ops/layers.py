@@ -95,10 +95,11 @@ def qk_norm_rope_kv8(qkv: torch.Tensor, nq: int, nkv: int, pos: torch.Tensor, sl
         raise ValueError("rows and check go together")
     if rows is not None:
         kv8.want(rows, torch.int32, (rows.shape[0],), dev, "rows")
-    kv8.launch("sdc_kv8_append", dev, (qkv.data_ptr(), qkv.stride(0) if t > 1 else heads * 128, t, nq, nkv,
-                pos.data_ptr(), slots.data_ptr(), _p(q_norm), _p(k_norm), eps, _p(cos_sin), table_rows, rotary,
-                interleaved, q_out.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks,
-                _p(rows), 0 if rows is None else rows.shape[0], _p(check)))
+    kv8.launch("sdc_kv8_append", dev, (
+        qkv.data_ptr(), qkv.stride(0) if t > 1 else heads * 128, t, nq, nkv, pos.data_ptr(), slots.data_ptr(),
+        kv8.ptr(q_norm), kv8.ptr(k_norm), eps, kv8.ptr(cos_sin), table_rows, rotary, interleaved, q_out.data_ptr(),
+        cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, kv8.ptr(rows),
+        0 if rows is None else rows.shape[0], kv8.ptr(check)))
     return q_out
 
 

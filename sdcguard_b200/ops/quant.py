@@ -189,11 +189,11 @@ class QuantWeights:
         packed = None
         if m > 8 and blocks is None and self.n * self.k > 1 << 24:
             packed = torch.empty(-(-self.k // 128) * 128 * (16 if m <= 16 else 32), dtype=torch.bfloat16, device=dev)
-        kv8.launch("sdc_matvec4", dev, (x.data_ptr(), x.stride(0) if m > 1 else self.k, m, self.n, self.k, self.group,
-                    self.codes.data_ptr(), self.scales.data_ptr(), None if self.zeros is None else self.zeros.data_ptr(),
-                    mode, None if bias is None else bias.data_ptr(), out.data_ptr(), out.stride(0) if m > 1 else self.n,
-                    None if packed is None else packed.data_ptr(), None if blocks is None else blocks.data_ptr(), 0 if blocks is None else blocks.shape[0],
-                    None if check is None else check.data_ptr()))
+        kv8.launch("sdc_matvec4", dev, (
+            x.data_ptr(), x.stride(0) if m > 1 else self.k, m, self.n, self.k, self.group, self.codes.data_ptr(),
+            self.scales.data_ptr(), kv8.ptr(self.zeros), mode, kv8.ptr(bias), out.data_ptr(),
+            out.stride(0) if m > 1 else self.n, kv8.ptr(packed), kv8.ptr(blocks),
+            0 if blocks is None else blocks.shape[0], kv8.ptr(check)))
         return out
 
     def fingerprint(self) -> torch.Tensor:

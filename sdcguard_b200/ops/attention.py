@@ -165,14 +165,17 @@ def decode8_plan(nseq: int, nq: int, nkv: int, max_ctx: int, device) -> Decode8P
     return Decode8Plan(nseq, nq, nkv, max_ctx, seg, segs, part)
 
 
-def _want_q(q: torch.Tensor, cache: KV8Cache, out: Optional[torch.Tensor]) -> torch.Tensor:
-    dev = cache.device
-    if not cache.one_layer:
-        raise ValueError("the cache must be one layer of a KV8Cache")
-    kv8.want(q, torch.bfloat16, (q.shape[0], q.shape[1], 128), dev, "q", align=16)
+def _want_q(q: torch.Tensor, cache: KV8Cache, out: Optional[torch.Tensor]) -> tuple:
+    """(rows, query heads, out) of queries that fit the cache."""
+    shape = q.shape
+    if not cache.one_layer or len(shape) != 3 or shape[2] != 128:
+        raise ValueError(f"q must be (rows, heads, 128), got {tuple(shape)}, and the cache one layer of a KV8Cache")
+    kv8.want(q, torch.bfloat16, shape, cache.device, "q", align=16)
     if out is None:
-        return torch.empty_like(q)
-    return kv8.want(out, torch.bfloat16, tuple(q.shape), dev, "out", align=16)
+        out = torch.empty_like(q)
+    else:
+        kv8.want(out, torch.bfloat16, shape, cache.device, "out", align=16)
+    return shape[0], shape[1], out
 
 
 def _want_extra(row_sq, check, rows: int, dev) -> None:
@@ -193,10 +196,9 @@ def decode8(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_req
     that does not exist, or a page outside the cache gives NaN. seq_idx selects sequences; with `check` (a state row)
     they are recomputed and compared with `out`. row_sq: += ||row||^2 of the output (cleared by the caller; its sum
     over kv heads is taken in no fixed order)."""
-    b, nq = q.shape[0], q.shape[1]
+    b, nq, out = _want_q(q, cache, out)
     dev, nkv = cache.device, cache.nkv
-    out = _want_q(q, cache, out)
-    if (nq, nkv) != (plan.nq, plan.nkv) or b > plan.nseq:
+    if nq != plan.nq or nkv != plan.nkv or b > plan.nseq:
         raise ValueError(f"q {tuple(q.shape)} and {nkv} kv heads do not fit the plan ({plan.nseq} sequences, {plan.nq} "
                          f"query and {plan.nkv} kv heads)")
     if block_table.dtype is not torch.int32 or block_table.device != dev or block_table.dim() != 2 \
@@ -269,9 +271,8 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
     """`prefill` over a cache of 8 bits: the plan's pages are expanded to bf16 (exact for power-of-two scales), then the
     tensor-core prefill reads those. q (T, nq, 128), tiles from `prefill_tiles`, requests numbered as in the plan. With
     `check`: every pages_step-th expanded page from pages_from on and the rows of the replay tiles are compared."""
-    dev, nkv, nq = cache.device, cache.nkv, q.shape[1]
-    out = _want_q(q, cache, out)
-    t = q.shape[0]
+    t, nq, out = _want_q(q, cache, out)
+    dev, nkv = cache.device, cache.nkv
     if nkv != plan.nkv or nq % nkv or ROWS % (nq // nkv) or nq == 0:
         raise ValueError(f"{nq} query heads on {nkv} kv heads (plan: {plan.nkv}): a power of two up to 128 per kv head")
     kv8.want(pos, torch.int32, (t,), dev, "pos")

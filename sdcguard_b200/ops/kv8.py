@@ -53,8 +53,11 @@ def launch(entry: str, device: torch.device, args: tuple) -> None:
     """Calls the library's `entry` with args (addresses as integers, 0 for none) and `device`'s current stream. (These
     operators run for a few microseconds: the arguments cross as one struct, and the stream is taken as the bare
     handle.)"""
-    with on(device):
-        rc = getattr(_native.lib(), entry)(_native.STRUCTS[entry].pack(*args, _stream(device.index)))
+    index = device.index
+    if index is None or index != _here():
+        with on(device):
+            return launch(entry, device, args)
+    rc = getattr(_native.lib(), entry)(_native.STRUCTS[entry].pack(*args, _stream(index)))
     if rc:
         _native.check(rc, entry)
 

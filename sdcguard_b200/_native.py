@@ -122,6 +122,7 @@ SIGNATURES: dict[str, tuple] = {
                                  I, U, P]),
     "sdc_kv8_append": (I, [P]),
     "sdc_kv8_expand": (I, [P]),
+    "sdc_attn_prefill_expanded": (I, [P]),
     "sdc_kv8_decode": (I, [P]),
     "sdc_matvec4": (I, [P]),
     "sdc_ep_receive_grouped": (I, [P, P, P, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P, P]),
@@ -130,7 +131,8 @@ SIGNATURES: dict[str, tuple] = {
 # entry points that take their arguments in one struct: its layout (native alignment)
 STRUCTS: dict[str, struct.Struct] = {
     "sdc_kv8_append": struct.Struct("@PqiiiPPPPdPiiiPPPqPiPP"),
-    "sdc_kv8_expand": struct.Struct("@PPqPiiPPPiiiiPP"),
+    "sdc_kv8_expand": struct.Struct("@PPqPiiPiiPP"),
+    "sdc_attn_prefill_expanded": struct.Struct("@PPPqPiPPiPiifPPP"),
     "sdc_kv8_decode": struct.Struct("@PPPPqPiiqPPPiiiiiifPPPP"),
     "sdc_matvec4": struct.Struct("@PqiiiiPPPiPPqPPiPP"),
 }

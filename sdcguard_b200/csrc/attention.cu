@@ -31,7 +31,8 @@ struct PrefillParams {
   const __nv_bfloat16* cache; // layer cache
   const int* block_table;     // [R, max_pages]
   int max_pages;
-  const int* pos;             // [T] absolute position of each token
+  const int* pos;             // [T] absolute position of each token; from `limit` on: a row without keys
+  int limit;
   const int4* tiles;          // (request, first token, tokens, offset into row_idx or -1)
   const int* row_idx;
   int nq, nkv;
@@ -142,7 +143,8 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
     int tok = -1;
     if (ti < tile.z && ti < tpc) tok = tile.w >= 0 ? p.row_idx[tile.w + ti] : tile.y + ti;
     ctl->tok[r] = tok;
-    const int ps = tok >= 0 ? p.pos[tok] : -1;
+    int ps = tok >= 0 ? p.pos[tok] : -1;
+    if (ps >= p.limit) ps = -1;
     ctl->pos[r] = ps;
     if (ps >= 0) atomicMax(&ctl->maxpos, ps);
   }
@@ -155,6 +157,7 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
 
   if (warp == 0 && ntiles > 0) {
     // ------------------------------------------------------------ TMA producer (all 32 lanes issue)
+    pdl_wait();                           // the pages may come from the kernel before (launched with overlap)
     bool ok = true;
     int last = -1;                        // last tile whose loads were issued
     for (int j = 0; j < ntiles && ok; ++j) {
@@ -502,7 +505,8 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
     int tok = -1;
     if (tl.x == req && ti < tl.z && ti < tpc) tok = tl.w >= 0 ? p.row_idx[tl.w + ti] : tl.y + ti;
     ctl->tok[x][r] = tok;
-    const int ps = tok >= 0 ? p.pos[tok] : -1;
+    int ps = tok >= 0 ? p.pos[tok] : -1;
+    if (ps >= p.limit) ps = -1;
     ctl->pos[x][r] = ps;
     if (ps >= 0) atomicMax(&ctl->maxpos[x], ps);
   }
@@ -519,6 +523,7 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
     // ------------------------------------------------------------ TMA producers (all 32 lanes issue): warp 0 K, warp 2 V
     // K's stage is free once S of both query tiles is formed, a softmax and a product before V's: taken apart, the next
     // K is on its way that much earlier (with one barrier for both, the MMAs waited for K in half of the time)
+    pdl_wait();                           // the pages may come from the kernel before (launched with overlap)
     const int kv = warp >> 1;
     uint64_t* full = kv ? ctl->v_full : ctl->k_full;
     uint64_t* empty = kv ? ctl->v_empty : ctl->k_empty;
@@ -1190,11 +1195,10 @@ static int launch_decode(const DecodeParams& p, const CUtensorMap& tm, dim3 grid
   return static_cast<int>(cudaGetLastError());
 }
 
-extern "C" {
-
-int sdc_attn_prefill(const void* q, void* o, const void* cache, long long num_blocks, const int* block_table,
-                     int max_pages, const int* pos, const void* tiles, int ntiles, const int* row_idx, int nq, int nkv,
-                     int head_dim, float scale, void* row_sq, void* check, void* stream) {
+static int launch_prefill(const void* q, void* o, const void* cache, long long num_blocks, const int* block_table,
+                          int max_pages, const int* pos, int limit, const void* tiles, int ntiles, const int* row_idx,
+                          int nq, int nkv, int head_dim, float scale, void* row_sq, void* check, bool overlap,
+                          cudaStream_t stream) {
   if (ntiles <= 0) return 0;
   if (head_dim != D || nq % nkv || (ROWS % (nq / nkv))) return -1;
   PrefillParams p;
@@ -1204,6 +1208,7 @@ int sdc_attn_prefill(const void* q, void* o, const void* cache, long long num_bl
   p.block_table = block_table;
   p.max_pages = max_pages;
   p.pos = pos;
+  p.limit = limit;
   p.tiles = static_cast<const int4*>(tiles);
   p.row_idx = row_idx;
   p.nq = nq;
@@ -1226,16 +1231,55 @@ int sdc_attn_prefill(const void* q, void* o, const void* cache, long long num_bl
     const char* v = std::getenv("SDCGUARD_PREFILL_PINGPONG");
     return v == nullptr || v[0] != '0';
   }();
-  if (pingpong) {
-    // tiles come in pairs of one request (entries 2i and 2i + 1; an odd count is padded by the caller)
-    if (ntiles % 2) return -3;
-    dim3 grid(ntiles / 2, nkv);
-    prefill_pp_kernel<<<grid, pp::THREADS, pp::SMEM, static_cast<cudaStream_t>(stream)>>>(tm, p);
-  } else {
-    dim3 grid(ntiles, nkv);
-    prefill_tc_kernel<<<grid, 128 + pf::SOFT, pf::SMEM, static_cast<cudaStream_t>(stream)>>>(tm, p);
-  }
-  return static_cast<int>(cudaGetLastError());
+  // with ping-pong, tiles come in pairs of one request (entries 2i and 2i + 1; an odd count is padded by the caller)
+  if (pingpong && ntiles % 2) return -3;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(pingpong ? ntiles / 2 : ntiles, nkv);
+  cfg.blockDim = dim3(pingpong ? pp::THREADS : 128 + pf::SOFT);
+  cfg.dynamicSmemBytes = pingpong ? pp::SMEM : pf::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = overlap ? 1 : 0;
+  return static_cast<int>(pingpong ? cudaLaunchKernelEx(&cfg, prefill_pp_kernel, tm, p)
+                                   : cudaLaunchKernelEx(&cfg, prefill_tc_kernel, tm, p));
+}
+
+extern "C" {
+
+int sdc_attn_prefill(const void* q, void* o, const void* cache, long long num_blocks, const int* block_table,
+                     int max_pages, const int* pos, const void* tiles, int ntiles, const int* row_idx, int nq, int nkv,
+                     int head_dim, float scale, void* row_sq, void* check, void* stream) {
+  return launch_prefill(q, o, cache, num_blocks, block_table, max_pages, pos, 0x7fffffff, tiles, ntiles, row_idx, nq, nkv,
+                        head_dim, scale, row_sq, check, false, static_cast<cudaStream_t>(stream));
+}
+
+// The prefill over pages that the kernel before it in the stream writes (sdc_kv8_expand): it starts while that one runs
+// and waits for it before its first page. Positions beyond the block table's rows (max_pages * 16) are rows without keys.
+struct AttnPrefillArgs {
+  const void* q;
+  void* o;
+  const void* cache;
+  long long num_blocks;
+  const int* block_table;
+  int max_pages;
+  const int* pos;
+  const void* tiles;
+  int ntiles;
+  const int* row_idx;
+  int nq;
+  int nkv;
+  float scale;
+  void* row_sq;
+  void* check;
+  void* stream;
+};
+int sdc_attn_prefill_expanded(const AttnPrefillArgs* a) {
+  return launch_prefill(a->q, a->o, a->cache, a->num_blocks, a->block_table, a->max_pages, a->pos, a->max_pages * PAGE,
+                        a->tiles, a->ntiles, a->row_idx, a->nq, a->nkv, D, a->scale, a->row_sq, a->check, true,
+                        static_cast<cudaStream_t>(a->stream));
 }
 
 int sdc_attn_decode_splits(int max_ctx) { return (max_ctx + SEG_KEYS - 1) / SEG_KEYS; }

@@ -568,9 +568,8 @@ __global__ void __launch_bounds__(256) kv8_append_check_kernel(const AppendParam
 // ------------------------------------------------------------------------------------------------ pages to bf16
 // Pages of the list in bf16 (exact while scales are powers of two), for the tensor-core prefill: a prefill reads each
 // page once for every 256 / group of its query rows, so expanding it once costs less than expanding it in every CTA.
-// One warp per (page, K / V, kv head): 2 KB in, 4 KB out. A page id outside the cache gives NaN. The first warps also
-// bring the positions into the plan's table (pos >= limit becomes -1, a row without keys). With `check`: the pages
-// every `step`-th of the list from `from` are compared instead of written.
+// One warp per (page, K / V, kv head): 2 KB in, 4 KB out. A page id outside the cache gives NaN. With `check`: every
+// `step`-th page of the list from `from` on is compared instead of written.
 struct ExpandParams {
   const uint8_t* codes;
   const float* scales;
@@ -578,53 +577,41 @@ struct ExpandParams {
   int npages, nkv;
   long long num_blocks;
   __nv_bfloat16* out;
-  const int* pos;
-  int* pos_out;
-  int T, limit;
   int from, step;
   unsigned long long* check;
 };
 
 __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
   const long long gt = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  for (long long i = gt; i < p.T; i += static_cast<long long>(gridDim.x) * 256) {
-    const int v = p.pos[i];
-    p.pos_out[i] = v >= p.limit ? -1 : v;
-  }
+  pdl_trigger();                           // the prefill may start, and waits before it reads a page
   const long long gw = gt >> 5;
   const int lane = threadIdx.x & 31, per = 2 * p.nkv;
-  const long long i = p.check == nullptr ? gw / per : p.from + gw / per * p.step;
+  const long long i = p.check == nullptr ? gw / per : p.from + gw / per * static_cast<long long>(p.step);
   if (i >= p.npages) return;
   const int unit = static_cast<int>(gw % per), kv = unit / p.nkv, h = unit % p.nkv;
   const int blk = p.pages[i];
   const bool in = blk >= 0 && blk < p.num_blocks;
   const float s = in ? p.scales[(static_cast<long long>(blk) * p.nkv + h) * 2 + kv] : __int_as_float(0x7fffffff);
-  const uint4* src = reinterpret_cast<const uint4*>(
+  const uint2* src = reinterpret_cast<const uint2*>(
       p.codes + ((static_cast<long long>(in ? blk : 0) * 2 + kv) * p.nkv + h) * (PAGE * D));
   uint4* dst = reinterpret_cast<uint4*>(p.out + ((i * 2 + kv) * p.nkv + h) * (PAGE * D));
-  uint4 c[4];
+  // eight codes to a lane and 16 bytes out, so that a store writes whole lines
+  uint2 c[8];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) c[j] = src[j * 32 + lane];
+  for (int j = 0; j < 8; ++j) c[j] = src[j * 32 + lane];
   bool bad = false;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t w[4] = {c[j].x, c[j].y, c[j].z, c[j].w};
-    uint32_t o[8];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 a = h2_to_f2(e4m3x2_to_h2(w[e])), b = h2_to_f2(e4m3x2_to_h2_hi(w[e]));
-      o[2 * e] = pack_bf16x2(a.x * s, a.y * s);
-      o[2 * e + 1] = pack_bf16x2(b.x * s, b.y * s);
-    }
-    uint4* d = dst + 2 * (j * 32 + lane);
+  for (int j = 0; j < 8; ++j) {
+    const float2 f0 = h2_to_f2(e4m3x2_to_h2(c[j].x)), f1 = h2_to_f2(e4m3x2_to_h2_hi(c[j].x));
+    const float2 f2 = h2_to_f2(e4m3x2_to_h2(c[j].y)), f3 = h2_to_f2(e4m3x2_to_h2_hi(c[j].y));
+    const uint4 o = make_uint4(pack_bf16x2(f0.x * s, f0.y * s), pack_bf16x2(f1.x * s, f1.y * s),
+                               pack_bf16x2(f2.x * s, f2.y * s), pack_bf16x2(f3.x * s, f3.y * s));
     if (p.check == nullptr) {
-      d[0] = make_uint4(o[0], o[1], o[2], o[3]);
-      d[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      dst[j * 32 + lane] = o;
     } else {
-      const uint4 a = d[0], b = d[1];
-      const uint32_t have[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) bad |= bf16x2_diff(o[e], have[e]) >= 0;
+      const uint4 d = dst[j * 32 + lane];
+      bad |= bf16x2_diff(o.x, d.x) >= 0 || bf16x2_diff(o.y, d.y) >= 0 || bf16x2_diff(o.z, d.z) >= 0 ||
+             bf16x2_diff(o.w, d.w) >= 0;
     }
   }
   if (p.check != nullptr) {
@@ -1208,18 +1195,13 @@ struct Kv8ExpandArgs {
   int npages;
   int nkv;
   void* out;
-  const int* pos;
-  int* pos_out;
-  int T;
-  int limit;
   int from;
   int step;
   void* check;
   void* stream;
 };
 int sdc_kv8_expand(const Kv8ExpandArgs* args) {
-  const auto& [codes, scales, num_blocks, pages, npages, nkv, out, pos, pos_out, T, limit, from, step, check,
-               stream] = *args;
+  const auto& [codes, scales, num_blocks, pages, npages, nkv, out, from, step, check, stream] = *args;
   if (npages <= 0) return 0;
   if (nkv < 1 || num_blocks < 1 || (check != nullptr && (from < 0 || step < 1))) return -1;
   ExpandParams p;
@@ -1230,15 +1212,12 @@ int sdc_kv8_expand(const Kv8ExpandArgs* args) {
   p.nkv = nkv;
   p.num_blocks = num_blocks;
   p.out = static_cast<__nv_bfloat16*>(out);
-  p.pos = pos;
-  p.pos_out = pos_out;
-  p.T = T;
-  p.limit = limit;
   p.from = from;
   p.step = step;
   p.check = static_cast<unsigned long long*>(check);
-  const long long n = check == nullptr ? npages : (npages - from + step - 1) / step;
-  const long long blocks = n <= 0 ? 1 : (n * 2 * nkv * 32 + 255) / 256;
+  const long long n = check == nullptr ? npages : (npages - static_cast<long long>(from) + step - 1) / step;
+  if (n <= 0) return 0;
+  const long long blocks = (n * 2 * nkv * 32 + 255) / 256;
   kv8_expand_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
   return static_cast<int>(cudaGetLastError());
 }

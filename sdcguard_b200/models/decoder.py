@@ -408,6 +408,8 @@ class CheckedDecoder:
         """A layer's attention over an 8-bit cache, and the replay of its sampled rows; a prefill's replay compares
         every 64th expanded page too, from a page that rotates with the layers and steps."""
         if meta.mode == "prefill":
+            if meta.plan8 is None:
+                raise ValueError("a prefill over an 8-bit cache needs meta.plan8 (CheckedDecoder.prefill8_plan)")
             attention.prefill8(q, cache, meta.plan8, meta.pos, meta.tiles, out=out, row_sq=row_sq)
             if sample is not None:
                 self._page_turn = getattr(self, "_page_turn", 0) + 1

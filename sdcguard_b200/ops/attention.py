@@ -193,9 +193,9 @@ def decode8(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_req
     among them) in the pages of row seq_req[b] of block_table (int32). Any number of query heads per kv head up to 16.
 
     A sequence without keys (ctx 0) gives zeros. One with more keys than its table row or the plan holds, a table row
-    that does not exist, or a page outside the cache gives NaN. seq_idx selects sequences; with `check` (a state row)
-    they are recomputed and compared with `out`. row_sq: += ||row||^2 of the output (cleared by the caller; its sum
-    over kv heads is taken in no fixed order)."""
+    that does not exist, or a page outside the cache gives NaN. seq_idx selects sequences, each once; with `check` (a
+    state row) they are recomputed and compared with `out`. row_sq: += ||row||^2 of the output (cleared by the caller;
+    its sum over kv heads is taken in no fixed order)."""
     b, nq, out = _want_q(q, cache, out)
     dev, nkv = cache.device, cache.nkv
     if nq != plan.nq or nkv != plan.nkv or b > plan.nseq:
@@ -210,6 +210,8 @@ def decode8(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_req
         kv8.want(seq_idx, torch.int32, (seq_idx.shape[0],), dev, "seq_idx")
     elif check is not None:
         raise ValueError("check needs seq_idx")
+    if cache.num_blocks * nkv >= 1 << 26 or (scale is not None and not 0 <= scale < math.inf):
+        raise ValueError(f"{cache.num_blocks} pages of {nkv} heads (below 2^26 in all) and scale {scale} (not negative)")
     if plan.part is not None and plan.part.device != dev:
         raise ValueError("the plan must be on the cache's device")
     if row_sq is not None or check is not None:
@@ -269,8 +271,8 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
              row_sq: Optional[torch.Tensor] = None, scale: Optional[float] = None,
              check: Optional[torch.Tensor] = None, pages_from: int = 0, pages_step: int = 64) -> torch.Tensor:
     """`prefill` over a cache of 8 bits: the plan's pages are expanded to bf16 (exact for power-of-two scales), then the
-    tensor-core prefill reads those. q (T, nq, 128), tiles from `prefill_tiles`, requests numbered as in the plan. With
-    `check`: every pages_step-th expanded page from pages_from on and the rows of the replay tiles are compared."""
+    tensor-core prefill reads those. q (T, nq, 128), tiles from `prefill_tiles`, requests numbered as in the plan. A
+    position outside the plan's table gives a row of zeros, a page outside the cache NaN. With `check`: every pages_step-th expanded page from pages_from on and the rows of the replay tiles are compared."""
     t, nq, out = _want_q(q, cache, out)
     dev, nkv = cache.device, cache.nkv
     if nkv != plan.nkv or nq % nkv or ROWS % (nq // nkv) or nq == 0:
@@ -279,6 +281,8 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
     kv8.want(tiles, torch.int32, (tiles.shape[0], 4), dev, "tiles", align=16)
     if plan.work.device != dev:
         raise ValueError("the plan must be on the cache's device")
+    if scale is not None and not 0 <= scale < math.inf:
+        raise ValueError(f"scale {scale}: finite and not negative")
     if check is not None and (row_idx is None or pages_from < 0 or pages_step < 1):
         raise ValueError("check needs replay tiles with row_idx, and pages_from >= 0, pages_step >= 1")
     if row_idx is not None:
@@ -286,14 +290,14 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
     _want_extra(row_sq, check, t, dev)
     if t == 0 or tiles.shape[0] == 0:
         return out
-    inside = torch.empty(t, dtype=torch.int32, device=dev)      # pos, -1 where it lies outside the plan's table
     kv8.launch("sdc_kv8_expand", dev, (
         cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, plan.pages.data_ptr(), plan.pages.shape[0],
-        nkv, plan.work.data_ptr(), pos.data_ptr(), inside.data_ptr(), t, plan.table.shape[1] * PAGE, pages_from,
-        pages_step, kv8.ptr(check)))
-    with kv8.on(dev):
-        return prefill(q, plan.work, plan.table, inside, tiles, nq, nkv, out=out, row_idx=row_idx, row_sq=row_sq,
-                       scale=scale, check=check)
+        nkv, plan.work.data_ptr(), pages_from, pages_step, kv8.ptr(check)))
+    kv8.launch("sdc_attn_prefill_expanded", dev, (
+        q.data_ptr(), out.data_ptr(), plan.work.data_ptr(), plan.work.shape[0], plan.table.data_ptr(),
+        plan.table.shape[1], pos.data_ptr(), tiles.data_ptr(), tiles.shape[0], kv8.ptr(row_idx), nq, nkv,
+        _SCALE if scale is None else scale, kv8.ptr(row_sq), kv8.ptr(check)))
+    return out
 
 
 def reference_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_pos: torch.Tensor) -> torch.Tensor:

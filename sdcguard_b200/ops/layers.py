@@ -66,7 +66,8 @@ def qk_norm_rope_kv8(qkv: torch.Tensor, nq: int, nkv: int, pos: torch.Tensor, sl
     head (a multiple of 8) are rotated: dim i with dim i + rotary / 2, or, `interleaved`, dims 2i and 2i + 1. None: no
     rotation.
 
-    The tokens that a call writes to one page are adjacent rows in increasing places, as a prompt's or a step's are.
+    The tokens that a call writes to one page are adjacent rows at places that follow one another, as a prompt's or a
+    step's are: one warp sets the page's scale (a page in two runs, or a place twice, leaves what it holds undefined).
     What the page held before the first of them is kept, at the page's new scale; what it held behind them is dead.
     A token whose slot lies outside the cache, or whose position lies outside the table, is not stored, and its row of
     q_out is NaN. With `check` (a state row) and `rows`: the sampled tokens are recomputed and compared with q_out and

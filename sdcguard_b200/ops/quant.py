@@ -155,7 +155,7 @@ class QuantWeights:
     def matvec(self, x: torch.Tensor, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
                blocks: Optional[torch.Tensor] = None, check: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x W^T (+ bias) for up to 32 rows x (m, k) bf16, read from the 4-bit codes (`csrc/matvec4.cu`): W is the
-        effective weight of `zero_mode`, bit for bit, sums and bias (fp32 [n]) in fp32, one rounding to bf16. Bound by
+        effective weight of `zero_mode`, bit for bit (scales below 2^27; larger ones give NaN), sums and bias (fp32 [n]) in fp32, one rounding to bf16. Bound by
         the codes' bytes, a quarter of the bf16 matrix. k and the group are multiples of 32.
 
         With `check` (a state row) and `blocks` (int32 indices of 16 outputs each): those outputs are recomputed and

@@ -424,9 +424,11 @@ def test_decode_offsets_beyond_32_bits():
 
 
 # ------------------------------------------------------------------------------------------------ prefill
-@pytest.mark.parametrize("nq,nkv", [(16, 8), (32, 8), (4, 1), (2, 2)])
-def test_prefill_matches_64_bits_and_replays_exactly(nq, nkv):
-    lens, prior = [200, 77, 1, 130], [0, 40, 300, 16]
+@pytest.mark.parametrize("nq,nkv,lens,prior", [
+    (16, 8, [200, 77, 1, 130], [0, 40, 300, 16]), (32, 8, [200, 77, 1, 130], [0, 40, 300, 16]),
+    (4, 1, [200, 77, 1, 130], [0, 40, 300, 16]), (2, 2, [200, 77, 1, 130], [0, 40, 300, 16]),
+    (2, 1, [1500, 77, 1, 130], [700, 40, 3000, 0])])                 # many key tiles: every barrier turns often
+def test_prefill_matches_64_bits_and_replays_exactly(nq, nkv, lens, prior):
     ctxs = [a + b for a, b in zip(lens, prior)]
     _, cache, bt, _, _, _ = _decode_case(ctxs, nq, nkv, seed=nq, spread=1.0)
     T, G = sum(lens), nq // nkv

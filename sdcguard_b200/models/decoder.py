@@ -95,6 +95,13 @@ class LayerWeights:
     cw: dict = field(default_factory=dict)   # name -> gemm.CheckedWeight
 
 
+def page_offset(calls: int, pages: int) -> int:
+    """The first of every 64th page that a replay compares after `calls` replays over all layers: a multiple of the
+    golden ratio's fraction, so that the calls of one layer, which lie its model's layer count apart, reach every page
+    (counting up would not, where that count shares a factor with 64)."""
+    return ((calls * 2654435769 & 0xffffffff) * min(64, pages)) >> 32
+
+
 class CheckedDecoder:
     """The model plus its check state. Slots of the state table name each checked op (`state.names`)."""
 
@@ -413,7 +420,7 @@ class CheckedDecoder:
             attention.prefill8(q, cache, meta.plan8, meta.pos, meta.tiles, out=out, row_sq=row_sq)
             if sample is not None:
                 self._page_turn = getattr(self, "_page_turn", 0) + 1
-                turn = self._page_turn % min(64, meta.plan8.pages.shape[0])
+                turn = page_offset(self._page_turn, meta.plan8.pages.shape[0])
                 replay(lambda: attention.prefill8(q, cache, meta.plan8, meta.pos, meta.sample_tiles, out=out,
                                                   row_idx=meta.sample_idx, check=self._st(name), pages_from=turn))
             return

@@ -181,8 +181,8 @@ def _want_q(q: torch.Tensor, cache: KV8Cache, out: Optional[torch.Tensor]) -> tu
 def _want_extra(row_sq, check, rows: int, dev) -> None:
     if row_sq is not None:
         kv8.want(row_sq, torch.float32, (rows,), dev, "row_sq")
-    if check is not None and (check.dtype != torch.int64 or check.device != dev):
-        raise ValueError("check must be a state row (int64) on the cache's device")
+    if check is not None:
+        kv8.want_state(check, dev)
 
 
 def decode8(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_req: torch.Tensor, ctx: torch.Tensor,
@@ -196,6 +196,7 @@ def decode8(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_req
     that does not exist, or a page outside the cache gives NaN. seq_idx selects sequences, each once; with `check` (a
     state row) they are recomputed and compared with `out`. row_sq: += ||row||^2 of the output (cleared by the caller;
     its sum over kv heads is taken in no fixed order)."""
+    given = out
     b, nq, out = _want_q(q, cache, out)
     dev, nkv = cache.device, cache.nkv
     if nq != plan.nq or nkv != plan.nkv or b > plan.nseq:
@@ -208,8 +209,8 @@ def decode8(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_req
     kv8.want(ctx, torch.int32, (b,), dev, "ctx")
     if seq_idx is not None:
         kv8.want(seq_idx, torch.int32, (seq_idx.shape[0],), dev, "seq_idx")
-    elif check is not None:
-        raise ValueError("check needs seq_idx")
+    if check is not None and (seq_idx is None or given is None):
+        raise ValueError("check needs seq_idx, and out, which it compares")
     if cache.num_blocks * nkv >= 1 << 26 or (scale is not None and not 0 <= scale < math.inf):
         raise ValueError(f"{cache.num_blocks} pages of {nkv} heads (below 2^26 in all) and scale {scale} (not negative)")
     if plan.part is not None and plan.part.device != dev:
@@ -272,7 +273,9 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
              check: Optional[torch.Tensor] = None, pages_from: int = 0, pages_step: int = 64) -> torch.Tensor:
     """`prefill` over a cache of 8 bits: the plan's pages are expanded to bf16 (exact for power-of-two scales), then the
     tensor-core prefill reads those. q (T, nq, 128), tiles from `prefill_tiles`, requests numbered as in the plan. A
-    position outside the plan's table gives a row of zeros, a page outside the cache NaN. With `check`: every pages_step-th expanded page from pages_from on and the rows of the replay tiles are compared."""
+    position outside the plan's table gives a row of zeros, a page outside the cache NaN. With `check`: every
+    pages_step-th expanded page from pages_from on and the rows of the replay tiles are compared."""
+    given = out
     t, nq, out = _want_q(q, cache, out)
     dev, nkv = cache.device, cache.nkv
     if nkv != plan.nkv or nq % nkv or ROWS % (nq // nkv) or nq == 0:
@@ -283,8 +286,9 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
         raise ValueError("the plan must be on the cache's device")
     if scale is not None and not 0 <= scale < math.inf:
         raise ValueError(f"scale {scale}: finite and not negative")
-    if check is not None and (row_idx is None or pages_from < 0 or pages_step < 1):
-        raise ValueError("check needs replay tiles with row_idx, and pages_from >= 0, pages_step >= 1")
+    if check is not None and (row_idx is None or given is None or pages_from < 0 or pages_step < 1):
+        raise ValueError("check needs replay tiles with row_idx, out, which it compares, pages_from >= 0 and "
+                         "pages_step >= 1")
     if row_idx is not None:
         kv8.want(row_idx, torch.int32, (row_idx.shape[0],), dev, "row_idx")
     _want_extra(row_sq, check, t, dev)

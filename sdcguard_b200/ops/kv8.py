@@ -36,6 +36,13 @@ def want(t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device
                      f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
+def want_state(check: torch.Tensor, device: torch.device) -> None:
+    """ValueError unless `check` is a state row (a check mode's kernel writes all of it)."""
+    if check.dtype is not torch.int64 or check.numel() != 4 or check.device != device or not check.is_contiguous():
+        raise ValueError(f"check must be a state row (4 contiguous int64) on {device}, got {check.dtype} "
+                         f"{tuple(check.shape)} on {check.device}")
+
+
 _here, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 

@@ -21,9 +21,18 @@ def _s(t: torch.Tensor) -> int:
 
 def _geometry(cache: torch.Tensor):
     """cache: (layers, blocks, ...) bf16 -> (layers, layer stride bytes, page bytes)."""
+    if not isinstance(cache, torch.Tensor):
+        raise ValueError(f"pages are hashed and transferred from one tensor (a bf16 cache), not from a "
+                         f"{type(cache).__name__}, which keeps their scales apart")
     L = cache.shape[0]
     page_bytes = cache[0, 0].numel() * cache.element_size()
     return L, cache.stride(0) * cache.element_size(), page_bytes
+
+
+def page_bytes(cache: torch.Tensor) -> int:
+    """Bytes of one page over every layer."""
+    layers, _, page = _geometry(cache)
+    return layers * page
 
 
 def page_checksums(cache: torch.Tensor, pages: torch.Tensor, seed: int = DEFAULT_SEED,

@@ -96,6 +96,7 @@ def qk_norm_rope_kv8(qkv: torch.Tensor, nq: int, nkv: int, pos: torch.Tensor, sl
         raise ValueError("rows and check go together")
     if rows is not None:
         kv8.want(rows, torch.int32, (rows.shape[0],), dev, "rows")
+        kv8.want_state(check, dev)
     kv8.launch("sdc_kv8_append", dev, (
         qkv.data_ptr(), qkv.stride(0) if t > 1 else heads * 128, t, nq, nkv, pos.data_ptr(), slots.data_ptr(),
         kv8.ptr(q_norm), kv8.ptr(k_norm), eps, kv8.ptr(cos_sin), table_rows, rotary, interleaved, q_out.data_ptr(),

@@ -155,12 +155,13 @@ class QuantWeights:
     def matvec(self, x: torch.Tensor, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
                blocks: Optional[torch.Tensor] = None, check: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x W^T (+ bias) for up to 32 rows x (m, k) bf16, read from the 4-bit codes (`csrc/matvec4.cu`): W is the
-        effective weight of `zero_mode`, bit for bit (scales below 2^27; larger ones give NaN), sums and bias (fp32 [n]) in fp32, one rounding to bf16. Bound by
-        the codes' bytes, a quarter of the bf16 matrix. k and the group are multiples of 32.
+        effective weight of `zero_mode`, bit for bit (scales below 2^27; larger ones give NaN), sums and bias (fp32 [n])
+        in fp32, one rounding to bf16. The codes are a quarter of the bf16 matrix's bytes. k and the group are multiples
+        of 32.
 
         With `check` (a state row) and `blocks` (int32 indices of 16 outputs each): those outputs are recomputed and
         compared with `out` (the call's result), bit for bit, instead of written."""
-        dev, m = self.codes.device, x.shape[0]
+        dev, m, given = self.codes.device, x.shape[0], out
         if self.bits != 4 or self.group % 32:
             raise ValueError("matvec reads INT4 codes with groups of a multiple of 32")
         kv8.want(self.codes, torch.uint8, (self.n, self.k // 2), dev, "codes", align=16)
@@ -179,10 +180,11 @@ class QuantWeights:
             out = torch.empty(m, self.n, dtype=torch.bfloat16, device=dev)
         elif out.shape != (m, self.n) or out.dtype != torch.bfloat16 or out.device != dev or out.stride(1) != 1:
             raise ValueError(f"out must be bf16 ({m}, {self.n}) on {dev} with contiguous rows")
-        if (blocks is None) != (check is None):
-            raise ValueError("blocks and check go together")
+        if (blocks is None) != (check is None) or (check is not None and given is None):
+            raise ValueError("blocks and check go together, with out, which they compare")
         if blocks is not None:
             kv8.want(blocks, torch.int32, (blocks.shape[0],), dev, "blocks")
+            kv8.want_state(check, dev)
         mode = 0 if self.zeros is None else ZERO_MODES.index(self.zero_mode)
         # more than eight rows of x, read by many CTAs: brought into the order of the products once (13 x 28672 x 4096:
         # 28 us against 35; 16 x 4096 x 4096 and below, where the second launch counts: alike)
@@ -214,8 +216,22 @@ class CheckedQuantLinear:
         self.qw = qw
         self.cw = gemm.CheckedWeight(qw.effective_weight(), bias)
         self.codes_fp = qw.fingerprint()
-        self._samples: Optional[torch.Tensor] = None
+        # row i: blocks i, i + turns, ... of 16 outputs, the sample of every turns-th call
+        blocks = -(-qw.n // 16)
+        turns = min(64, blocks)
+        self._samples = (torch.arange(turns)[:, None] + turns * torch.arange(-(-blocks // turns))[None]).to(
+            device=qw.codes.device, dtype=torch.int32)
         self._turn = 0
+        self._graph_turn = torch.zeros(1, dtype=torch.int64, device=qw.codes.device)
+
+    def _sample(self) -> torch.Tensor:
+        """The blocks to recompute in this call. A captured call counts its replays on the device, so that they rotate
+        too."""
+        if torch.cuda.is_current_stream_capturing():
+            self._graph_turn.add_(1)
+            return self._samples.index_select(0, self._graph_turn.remainder(self._samples.shape[0])).view(-1)
+        self._turn += 1
+        return self._samples[self._turn % self._samples.shape[0]]
 
     def __call__(self, x: torch.Tensor, state: torch.Tensor, slot: int, decode_slot: Optional[int] = None,
                  **kw) -> torch.Tensor:
@@ -224,14 +240,8 @@ class CheckedQuantLinear:
         if set(kw) - {"out", "row_sq"}:
             raise ValueError(f"{sorted(set(kw) - {'out', 'row_sq'})}: arguments of the GEMM path")
         y = self.qw.matvec(x, self.cw.bias, out=kw.get("out"))
-        if self._samples is None:           # row i: blocks i, i + 64, ... of 16 outputs, the sample of every 64th call
-            blocks = -(-self.qw.n // 16)
-            turns = min(64, blocks)
-            per = -(-blocks // turns)
-            self._samples = (torch.arange(turns)[:, None] + turns * torch.arange(per)[None]).to(torch.int32).to(x.device)
-        sample = self._samples[self._turn % self._samples.shape[0]]
-        self._turn += 1
-        self.qw.matvec(x, self.cw.bias, out=y, blocks=sample, check=state[decode_slot])
+        self._sampled = self._sample()
+        self.qw.matvec(x, self.cw.bias, out=y, blocks=self._sampled, check=state[decode_slot])
         return y
 
     def weights_unchanged(self) -> bool:

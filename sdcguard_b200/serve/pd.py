@@ -219,7 +219,7 @@ def consume(engine: LLMEngine, transfers: Sequence[Transfer], src_cache: torch.T
     device time ("pull_ms", CUDA events around each pull launch) and the bytes they moved ("pull_bytes")."""
     dev = engine.device
     N = len(transfers)
-    page_bytes = engine.cache[:, 0].numel() * engine.cache.element_size()     # one page over every layer
+    page_bytes = kvx.page_bytes(engine.cache)
     local_pages, owned = [], []
     for i, t in enumerate(transfers):
         cached = prefix.lookup(t.token_ids)

@@ -145,6 +145,59 @@ def test_matvec_refuses():
             qw.matvec(x)
 
 
+@pytest.mark.parametrize("check", [torch.zeros(4), torch.zeros(3, dtype=torch.int64), torch.zeros(8, dtype=torch.int64)[::2]])
+def test_check_takes_a_state_row(check):
+    """Check modes write the whole row: anything else is refused before a launch."""
+    idx = torch.zeros(1, dtype=torch.int32)
+    d, out = _decode_args(), torch.zeros(2, 4, 128, dtype=torch.bfloat16)
+    plan = attention.prefill8_plan(torch.tensor([[1]], dtype=torch.int32), [2], 2)
+    qw, x = QuantWeights.quantize(torch.randn(8, 64), bits=4, group=32), torch.zeros(1, 64, dtype=torch.bfloat16)
+    y = torch.zeros(1, 8, dtype=torch.bfloat16)
+    for call in (lambda c: layers.qk_norm_rope_kv8(**_append_args(), rows=idx, check=c),
+                 lambda c: attention.decode8(**d, out=out, seq_idx=idx, check=c),
+                 lambda c: attention.prefill8(d["q"], d["cache"], plan, d["ctx"], torch.zeros(1, 4, dtype=torch.int32),
+                                              out=out, row_idx=idx, check=c),
+                 lambda c: qw.matvec(x, out=y, blocks=idx, check=c)):
+        with pytest.raises(ValueError, match="state row"):
+            call(check)
+
+
+def test_check_needs_the_output():
+    """A check mode without `out` would compare with memory that nothing wrote."""
+    idx, st = torch.zeros(1, dtype=torch.int32), torch.zeros(4, dtype=torch.int64)
+    d = _decode_args()
+    plan = attention.prefill8_plan(torch.tensor([[1]], dtype=torch.int32), [2], 2)
+    qw, x = QuantWeights.quantize(torch.randn(8, 64), bits=4, group=32), torch.zeros(1, 64, dtype=torch.bfloat16)
+    for call in (lambda: attention.decode8(**d, seq_idx=idx, check=st),
+                 lambda: attention.prefill8(d["q"], d["cache"], plan, d["ctx"], torch.zeros(1, 4, dtype=torch.int32),
+                                            row_idx=idx, check=st),
+                 lambda: qw.matvec(x, blocks=idx, check=st)):
+        with pytest.raises(ValueError, match="out"):
+            call()
+
+
+def test_page_transfer_refuses_the_8_bit_cache():
+    """Its scales lie apart from the pages' bytes, so hashing or copying the codes alone would be no transfer."""
+    from sdcguard_b200.ops import kv_transfer
+    c = KV8Cache.empty(3, 1, layers=2, device="cpu")
+    for call in (lambda: kv_transfer.page_checksums(c, torch.zeros(1, dtype=torch.int32)),
+                 lambda: kv_transfer.page_bytes(c),
+                 lambda: kv_transfer.pull_pages(c, c, *[torch.zeros(1, dtype=torch.int32)] * 2,
+                                                torch.zeros(1, dtype=torch.int64))):
+        with pytest.raises(ValueError, match="KV8Cache"):
+            call()
+    assert kv_transfer.page_bytes(torch.zeros(2, 3, 2, 1, 16, 128, dtype=torch.bfloat16)) == 2 * 2 * 16 * 128 * 2
+
+
+@pytest.mark.parametrize("layers_", [1, 7, 28, 32, 36, 64])
+@pytest.mark.parametrize("pages", [1, 5, 64, 1000])
+def test_replayed_pages_reach_every_page_of_every_layer(layers_, pages):
+    from sdcguard_b200.models.decoder import page_offset
+    for layer in (0, layers_ - 1):
+        seen = {page_offset(1 + step * layers_ + layer, pages) for step in range(64 * 64)}
+        assert seen == set(range(min(64, pages)))
+
+
 def test_want():
     t = torch.zeros(4, 8)
     cpu = torch.device("cpu")

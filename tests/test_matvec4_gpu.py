@@ -102,3 +102,24 @@ def test_checked_layer_reads_the_codes_in_small_batches():
     assert st.read()[0]["checks"] > 0 and _holds(big, x, qw, bias)
     with pytest.raises(ValueError):
         layer(x[:5], st.state, s0, decode_slot=s1, inject=(0, 0, 1))
+
+
+def test_checked_layer_captured_at_its_first_call():
+    """A graph holds the layer and its replay check; the recomputed outputs rotate with the graph's replays."""
+    qw = _weights(2000, 256, 64, True)
+    layer = CheckedQuantLinear(qw)
+    st = gemm.StateTable(DEV, 2)
+    s0, s1 = st.add("quant (ABFT GEMM)", layer.cw.nb), st.add("quant.decode (replay)", 1)
+    x = torch.randn(3, 256, device=DEV).bfloat16()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = layer(x, st.state, s0, decode_slot=s1)
+    seen = set()
+    for i in range(64):
+        x.copy_(torch.randn(3, 256, device=DEV))
+        g.replay()
+        assert torch.equal(y, qw.matvec(x))
+        seen |= set(layer._sampled.tolist())
+    assert seen >= set(range(125))                        # all blocks of 16 outputs
+    row = st.read()[1]
+    assert row["checks"] == 64 and row["z"] == 0

@@ -6,21 +6,25 @@
 // rnd rounds to bf16: the effective weights of csrc/quant.cu bit for bit, so the products are those of the layer's
 // arithmetic whichever kernel serves it. Sums in fp32, one rounding of y to bf16.
 //
-// Bound by the codes' bytes (N K / 2) and, next to them, by the instructions per code: codes become bf16 weights in
-// pairs without a conversion (see `weights`), then one mma.m16n8k16 (A = W: 16 outputs, B = x^T: 8 rows of x) takes 8
-// weights of each lane. The order of k within a product is free, so a lane takes 16 bytes (32 weights) of a row as they
-// lie in memory, pairs (i, i + 4) of each word as masks give them, and reads x in the same order.
+// Codes become bf16 weights in pairs without a conversion (see `weights`), then one mma.m16n8k16 (A = W: 16 outputs, B =
+// x^T: 8 rows of x) takes 8 weights of each lane. The order of k within a product is free, so a lane takes 16 bytes (32
+// weights) of a row as they lie in memory, pairs (i, i + 4) of each word as masks give them, and reads x in the same
+// order.
 //
-// The k blocks (128 each) of an output go to 8 slices in turn, which merge in order at the end; a CTA of WARPS warps
-// computes 16 MT outputs, its warp w the slices w, w + WARPS, ... Each output's arithmetic depends on its codes and x's
-// row alone (not on M, MT, WARPS or the CTA), so a row of x gives the same bits in any batch, and running some blocks of
-// 16 outputs again gives them too: check mode compares them with y.
+// The bytes that must move are the codes' (N K / 2); what bounds is the instructions per code. Device times: 1 x 4096 x
+// 4096 4.6 us (its bytes alone 1.3), 1 x 28672 x 4096 19.2 us, 13 x 28672 x 4096 with zero points 28 us. A bare read of
+// the last matrix takes 10 us, and this kernel without forming the weights and without reading x and scales 13. Codes
+// through shared memory (TMA or cp.async rings), scales staged there and CTAs that walk over tiles gave the same times.
+//
+// A CTA computes 16 MT outputs. The k blocks (128 each) of an output go to its WARPS warps in turn, whose sums merge in
+// order at the end; WARPS follows from the matrix's shape. Each output's arithmetic depends on its codes and x's row alone
+// (not on M, MT or the CTA), so a row of x gives the same bits in any batch, and running some blocks of 16 outputs again
+// gives them too: check mode compares them with y.
 #include "common.cuh"
 
 namespace sdc {
 namespace matvec4 {
 
-constexpr int SLICES = 8;
 constexpr int KB = 128;       // k per block: 4 lanes x 32
 
 enum { ZERO_SUBTRACT = 0, ZERO_FMA = 1, ZERO_TWO = 2, ZERO_EIGHT = 3 };   // EIGHT: subtract without zero points
@@ -116,7 +120,7 @@ __global__ void __launch_bounds__(256) pack_x_kernel(const Params p) {
 template <int NT, int MT, int WARPS, int PF, int CTAS, int MODE, bool PACKED>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) matvec4_kernel(const Params p) {
   pdl_trigger();
-  __shared__ float red[SLICES][NT * 8][MT * 16 + 1];
+  __shared__ float red[WARPS][NT * 8][MT * 16 + 1];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int n0 = (p.blocks ? p.blocks[blockIdx.x] : static_cast<int>(blockIdx.x) * MT) * 16;
   if (p.check != nullptr && blockIdx.x == 0 && tid == 0) atomicAdd(p.check + 2, 1ull);
@@ -138,8 +142,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) matvec4_kernel(const Params 
   for (int j = 0; j < NT; ++j) xrow[j] = p.x + min(j * 8 + g, p.M - 1) * p.ldx;
   uint4 w[PF][MT][2];                    // a lane's 32 codes, scale and zero point of 2 MT outputs
   uint32_t ws[PF][MT][2], wz[PF][MT][2];
-  // the warp's blocks: slice after slice, in each every SLICES-th, a slice in whole turns of the PF buffers
-  int ls = warp, lk = warp;              // the next block to load
+  int lk = warp;                         // the next block to load: every WARPS-th is this warp's
   const auto load_next = [&](int f) {
     if (lk < nkb) {
       const int k = lk * KB + 32 * t;
@@ -154,79 +157,76 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) matvec4_kernel(const Params 
           if (MODE != ZERO_EIGHT) wz[f][i][r] = __ldg(p.zeros + meta[i][r] + gi);
         }
     }
-    lk += SLICES;
-    if (WARPS < SLICES && f == PF - 1 && lk >= nkb && ls + WARPS < SLICES) lk = ls += WARPS;
+    lk += WARPS;
   };
 #pragma unroll
   for (int f = 0; f < PF; ++f) load_next(f);
   if (PACKED) pdl_wait();                // the codes are on their way meanwhile
-  for (int slice = warp; slice < SLICES; slice += WARPS) {
-    float acc[MT][NT][4];
+  float acc[MT][NT][4];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
-    for (int kb = slice; kb < nkb; kb += SLICES * PF) {
+      for (int e = 0; e < 4; ++e) acc[i][j][e] = 0.f;
+  for (int kb = warp; kb < nkb; kb += WARPS * PF) {
 #pragma unroll
-      for (int f = 0; f < PF; ++f) {
-        const int kc = kb + f * SLICES;
-        if (kc < nkb) {                  // (uniform)
-          const int k = kc * KB + 32 * t;
-          const uint4* xp[NT];
-          if (!PACKED)
+    for (int f = 0; f < PF; ++f) {
+      const int kc = kb + f * WARPS;
+      if (kc < nkb) {                  // (uniform)
+        const int k = kc * KB + 32 * t;
+        const uint4* xp[NT];
+        if (!PACKED)
 #pragma unroll
-          for (int j = 0; j < NT; ++j) xp[j] = k < p.K ? reinterpret_cast<const uint4*>(xrow[j] + k) : no_x;
-          Factor lo[MT][2];
+        for (int j = 0; j < NT; ++j) xp[j] = k < p.K ? reinterpret_cast<const uint4*>(xrow[j] + k) : no_x;
+        Factor lo[MT][2];
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int r = 0; r < 2; ++r) lo[i][r] = factor_of<MODE>(ws[f][i][r], MODE == ZERO_EIGHT ? 8u : wz[f][i][r]);
+          for (int r = 0; r < 2; ++r) lo[i][r] = factor_of<MODE>(ws[f][i][r], MODE == ZERO_EIGHT ? 8u : wz[f][i][r]);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {        // word c: k + 8c .. k + 8c + 7
-            uint32_t b[NT][4];
+        for (int c = 0; c < 4; ++c) {        // word c: k + 8c .. k + 8c + 7
+          uint32_t b[NT][4];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              const uint4 x = PACKED ? p.packed[((kc * 4 + c) * NT + j) * 32 + lane] : pairs_of(__ldg(xp[j] + c));
-              b[j][0] = x.x;
-              b[j][1] = x.y;
-              b[j][2] = x.z;
-              b[j][3] = x.w;
-            }
+          for (int j = 0; j < NT; ++j) {
+            const uint4 x = PACKED ? p.packed[((kc * 4 + c) * NT + j) * 32 + lane] : pairs_of(__ldg(xp[j] + c));
+            b[j][0] = x.x;
+            b[j][1] = x.y;
+            b[j][2] = x.z;
+            b[j][3] = x.w;
+          }
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              const uint32_t w0 = word(w[f][i][0], c), w1 = word(w[f][i][1], c);
+          for (int i = 0; i < MT; ++i) {
+            const uint32_t w0 = word(w[f][i][0], c), w1 = word(w[f][i][1], c);
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t u0 = h ? w0 >> 8 : w0, u1 = h ? w1 >> 8 : w1;
-                const uint32_t a[4] = {weights<MODE>(u0 & 0x000f000fu, lo[i][0]), weights<MODE>(u1 & 0x000f000fu, lo[i][1]),
-                                 weights<MODE>(u0 & 0x00f000f0u, high_factor<MODE>(lo[i][0])),
-                                 weights<MODE>(u1 & 0x00f000f0u, high_factor<MODE>(lo[i][1]))};
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t u0 = h ? w0 >> 8 : w0, u1 = h ? w1 >> 8 : w1;
+              const uint32_t a[4] = {weights<MODE>(u0 & 0x000f000fu, lo[i][0]), weights<MODE>(u1 & 0x000f000fu, lo[i][1]),
+                               weights<MODE>(u0 & 0x00f000f0u, high_factor<MODE>(lo[i][0])),
+                               weights<MODE>(u1 & 0x00f000f0u, high_factor<MODE>(lo[i][1]))};
 #pragma unroll
-                for (int j = 0; j < NT; ++j) mma(acc[i][j], a, b[j][2 * h], b[j][2 * h + 1]);
-              }
+              for (int j = 0; j < NT; ++j) mma(acc[i][j], a, b[j][2 * h], b[j][2 * h + 1]);
             }
           }
         }
-        load_next(f);
       }
+      load_next(f);
     }
-    // acc[i][j]: outputs 16 i + g (+ 8), rows 8 j + 2t (+ 1)
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) red[slice][j * 8 + 2 * t + (e & 1)][i * 16 + g + (e >> 1) * 8] = acc[i][j][e];
   }
+  // acc[i][j]: outputs 16 i + g (+ 8), rows 8 j + 2t (+ 1)
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[warp][j * 8 + 2 * t + (e & 1)][i * 16 + g + (e >> 1) * 8] = acc[i][j][e];
   __syncthreads();
   for (int i = tid; i < p.M * MT * 16; i += WARPS * 32) {
     const int m = i / (MT * 16), c = i % (MT * 16), n = n0 + c;
     if (n >= p.N) continue;
     float s = red[0][m][c];
 #pragma unroll
-    for (int w = 1; w < SLICES; ++w) s += red[w][m][c];
+    for (int w = 1; w < WARPS; ++w) s += red[w][m][c];
     s *= BACK;
     if (p.bias != nullptr) s += p.bias[n];
     __nv_bfloat16* dst = p.y + m * p.ldy + n;
@@ -323,15 +323,27 @@ extern "C" int sdc_matvec4(const Matvec4Args* args) {
   p.blocks = blocks;
   p.check = static_cast<unsigned long long*>(check);
   auto st = static_cast<cudaStream_t>(stream);
+  // 8 warps a CTA; few outputs and a long k leave each warp much to do and the SMs with few warps, so that 16 take it
+  // (8 x 4096 x 14336: 12.4 us, with 8 17.0; 1 x 4096 x 8192: 8.4 and 9.8; 1 x 9216 x 4096 the other way: 8.8 and 7.6)
+  const bool deep = N <= 148 * 32 && K >= 8192;
   if (blocks != nullptr) {
     if (nblocks <= 0) return 0;
+    if (deep)
+      return M <= 8 ? launch<1, 1, 16, 2, 2>(p, mode, nblocks, st)
+                    : M <= 16 ? launch<2, 1, 16, 2, 1>(p, mode, nblocks, st) : launch<4, 1, 16, 2, 1>(p, mode, nblocks, st);
     return M <= 8 ? launch<1, 1, 8, 2, 4>(p, mode, nblocks, st)
                   : M <= 16 ? launch<2, 1, 8, 2, 3>(p, mode, nblocks, st) : launch<4, 1, 8, 2, 2>(p, mode, nblocks, st);
   }
-  // two groups of 16 outputs a warp share the reads of x, where two CTAs per SM remain (1 x 28672 x 4096: 19.3 us against
-  // 20.6 with one group; 16 x 4096 x 14336: 19.1 us, with one group 17.2)
-  const bool wide = N >= 2 * 148 * 32;
+  // two groups of 16 outputs a warp share the reads of x, where nearly two CTAs per SM remain (16 x 9216 x 4096: 10.2 us
+  // against 13.0 with one group, 1 x 28672 x 4096 19.2 and 20.6; the other way 1 x 9216 x 4096: 8.0 and 7.6, 16 x 6144 x
+  // 4096: 9.6 and 8.5), of 16 warps one (8 x 4096 x 14336: 12.3 us against 13.9; 8 x 1024 x 4096: 4.6 and 3.7)
+  const bool wide = N >= 8192;
   const int g1 = (N + 15) / 16, g2 = (N + 31) / 32;
+  if (deep) {
+    if (M <= 8) return N > 148 * 16 ? launch<1, 2, 16, 1, 1>(p, mode, g2, st) : launch<1, 1, 16, 2, 2>(p, mode, g1, st);
+    if (M <= 16) return packed ? launch<2, 1, 16, 1, 2, true>(p, mode, g1, st) : launch<2, 1, 16, 2, 1>(p, mode, g1, st);
+    return packed ? launch<4, 1, 16, 1, 2, true>(p, mode, g1, st) : launch<4, 1, 16, 2, 1>(p, mode, g1, st);
+  }
   if (M <= 8) return wide ? launch<1, 2, 8, 1, 3>(p, mode, g2, st) : launch<1, 1, 8, 2, 4>(p, mode, g1, st);
   if (M <= 16) {
     if (packed) return wide ? launch<2, 2, 8, 1, 2, true>(p, mode, g2, st) : launch<2, 1, 8, 2, 3, true>(p, mode, g1, st);

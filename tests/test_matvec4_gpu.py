@@ -123,3 +123,18 @@ def test_checked_layer_captured_at_its_first_call():
     assert seen >= set(range(125))                        # all blocks of 16 outputs
     row = st.read()[1]
     assert row["checks"] == 64 and row["z"] == 0
+
+
+@pytest.mark.parametrize("m", [1, 8, 13, 16, 27, 32])
+@pytest.mark.parametrize("n,k,group,zeros", [(40, 8224, 32, True), (2400, 8192, 128, False), (2049, 8224, 32, True),
+                                             (4752, 8192, 64, False)])
+def test_matvec_long_products(m, n, k, group, zeros):
+    """More warps take the products of a long k: 64 bits, the same bits in every batch and in the replay."""
+    qw = _weights(n, k, group, zeros, seed=m)
+    x = torch.randn(m, k, device=DEV).bfloat16()
+    y = qw.matvec(x)
+    assert _holds(y, x, qw)
+    assert torch.equal(qw.matvec(x[:1]), y[:1]) and torch.equal(qw.matvec(x[m - 1:]), y[m - 1:])
+    st = torch.zeros(4, dtype=torch.int64, device=DEV)
+    qw.matvec(x, out=y, blocks=torch.arange(-(-n // 16), dtype=torch.int32, device=DEV), check=st)
+    assert st.tolist()[2] == 1 and st.tolist()[0] == 0

@@ -258,7 +258,7 @@ __device__ __forceinline__ float exact_amax(const __nv_bfloat16* row, const __nv
 // one head and the runs that begin among TG consecutive tokens (up to 16 rows of one page), so one warp alone writes a
 // page's scale and codes of a head; keys wait for the scale in shared memory, values as they were read in registers.
 // TG = 1 gives each token of a decode step its own warps (latency); TG = 16 gives a page one warp and leaves none
-// without work.
+// without work; TG = 4 lies between.
 //
 // Scales and codes are the correctly rounded ones of the formulas, so they do not depend on the order of operations
 // here (a replay, another kernel or a CPU can compare bits). Values are exact products. Keys are computed in fp32; with
@@ -266,6 +266,11 @@ __device__ __forceinline__ float exact_amax(const __nv_bfloat16* row, const __nv
 // with it and the rotation by 4 u of the pair's length, at most sqrt(2) of the run's largest magnitude. Where a code
 // differs within 11 u of the key plus 6 u of that magnitude, or the scale within 2^-19, the row is computed again in
 // double: one pair of rows in thirty. (The sum of squares is fp32: keys stay below 2^60.)
+//
+// Measured (32 query, 8 kv heads, device time): 8 x 2048 tokens 60.5 us, 3.9 TB/s, bound by instructions and the latency
+// of the keys' chain (rows, norm, scale, codes), 20 warps an SM; 256 x 1 token 6.3 us, 1 x 1 3.5 us, latency. At 8 x 2048
+// one row a warp took 303 us, a row to a half warp 118, queries in warps of their own 91, keys waiting in shared memory
+// instead of registers 63.
 constexpr float KEY_RELATIVE = 11.f / 16777216.f, KEY_ABSOLUTE = 6.f / 16777216.f, SCALE_MARGIN = 32.f / 16777216.f;
 constexpr int AW = 4;             // warps of a CTA
 constexpr int QH = 8;             // heads of a query warp
@@ -625,10 +630,10 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
 // (256 a key and kv head); the queries of a kv head (<= 16) share every key that is read.
 //
 // Tensor cores on converted codes (mma.m16n8k16, f16 inputs, fp32 sums): E4M3 is exact in f16, so scales stay outside
-// the products. Both products have the cache as their A operand, whose fragments a lane fills from its own 16-byte
-// loads: S^T (16 keys x heads) = K Q^T, with the order of the dims permuted alike in K and Q so that a lane's four
-// codes of a k step are neighbours; O^T (dims x heads) += V^T P^T, with the pairs of keys put together by byte
-// permutes. Nothing passes through shared memory until the warps of a CTA merge.
+// the products. Both products have the cache as their A operand, whose fragments a lane fills from 16-byte reads of the
+// page in shared memory: S^T (16 keys x heads) = K Q^T, with the order of the dims permuted alike in K and Q so that a
+// lane's four codes of a k step are neighbours; O^T (dims x heads) += V^T P^T, with the pairs of keys put together by
+// byte permutes. Pages come by TMA into a ring of each warp (three pages deep), which no other warp waits for.
 //   q: bf16 values times a power of two per head (largest in [2^14, 2^15)), exact in f16 down to 2^-38 of the largest.
 //   x = log2(e) scale s_K q . k, and with V's page scale in the exponent y = x + log2 s_V. The running maximum M is of
 //   y, so the weights w = 2^(x - M + 14) s_V <= 2^15 are the largest f16 can hold whatever the pages' scales; the row
@@ -641,6 +646,11 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
 // kv8_combine_kernel merges them in order. Segments start at absolute multiples, so a row's arithmetic does not depend
 // on the batch around it: running a subset of rows again with the same plan gives the same bits (check mode).
 // A sequence whose length or table row does not fit gives NaN, as does a page id outside the cache.
+//
+// Measured (16 query, 8 kv heads, device time): 256 x 1600 keys 135 us, 6.2 TB/s, 0.95 of a copy's rate: DRAM bounds it.
+// 1 x 131072 keys 53 us, 5.1 TB/s, with the merge of its segments and the start of the CTAs in it; 61 ragged ones up to
+// 4100 keys 64 us, 4.2 TB/s, the longest rows' tail. 1 x 37 keys 3.8 us, latency. Loads into registers instead of the
+// ring: 162 us for the first; a ring filled by cp.async: 159; two warps a CTA: 131, but 67 and 76 us for the next two.
 constexpr int WARPS = 4;
 constexpr int REC = D + 4;               // floats a record: o[D], M, l, pad
 
@@ -1169,7 +1179,10 @@ int sdc_kv8_append(const Kv8AppendArgs* args) {
   p.check = static_cast<unsigned long long*>(check);
   const int gy = (nq + 2 * nkv + 7) / 8;
   auto st = static_cast<cudaStream_t>(stream);
-  const int tg = T < 1024 ? 1 : PAGE;
+  // one token, four or a page to a warp of keys or values: a decode step's tokens lie in as many pages, a prompt's share
+  // them, and only their number is known here. Of 1, 4, 16: 256 x 1 token 6.9, 10.4, 32.9 us; 512 x 1 10.7, 12.2, 33.3;
+  // 1 x 512 10.1, 8.7, 8.6; 1024 x 1 18.5, 17.5, 37.2; 5 x 300 16.7, 12.2, 14.2; 1 x 2048 21.8, 13.9, 11.9 us
+  const int tg = T < 512 ? 1 : T < 2048 ? 4 : PAGE;
   const long long ctas = static_cast<long long>((T + tg - 1) / tg) * ((2 * nkv + AW - 1) / AW) +
                          static_cast<long long>((T + 2 * AW - 1) / (2 * AW)) * ((nq + QH - 1) / QH);
   const unsigned grid = static_cast<unsigned>(ctas);
@@ -1180,6 +1193,9 @@ int sdc_kv8_append(const Kv8AppendArgs* args) {
   } else if (tg == 1) {
     if (interleaved) kv8_append_kernel<1, true><<<grid, AW * 32, 0, st>>>(p);
     else kv8_append_kernel<1, false><<<grid, AW * 32, 0, st>>>(p);
+  } else if (tg == 4) {
+    if (interleaved) kv8_append_kernel<4, true><<<grid, AW * 32, 0, st>>>(p);
+    else kv8_append_kernel<4, false><<<grid, AW * 32, 0, st>>>(p);
   } else {
     if (interleaved) kv8_append_kernel<PAGE, true><<<grid, AW * 32, 0, st>>>(p);
     else kv8_append_kernel<PAGE, false><<<grid, AW * 32, 0, st>>>(p);

@@ -144,6 +144,31 @@ def test_append_batch_of_sequences_padding_and_strided_rows():
     _run_append(2, 1, [-1], [3], blocks=2)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_does_not_depend_on_how_tokens_are_grouped(interleaved):
+    """How many tokens a warp looks at follows from the call's length: runs that start at every place of such a group and
+    reach over its end, between rows without a slot, give the same bits in calls of 500 to 2100 rows."""
+    g = torch.Generator().manual_seed(5)
+    slots, pos, page = [], [], 0
+    while len(slots) < 450:
+        n, start = int(torch.randint(1, 24, (1,), generator=g)), int(torch.randint(0, 16, (1,), generator=g))
+        slots += [page * 16 + start + i for i in range(n)] + [-1] * int(torch.randint(0, 3, (1,), generator=g))
+        pos += [start + i for i in range(n)] + [0] * (len(slots) - len(pos) - n)
+        page += (start + n) // 16 + 1
+    used, got = len(slots), []
+    for pad in (500, 511, 512, 2047, 2048, 2100):          # against 64 bits
+        (qkv, _, _, _, _, qn, kn, eps, table, _, _), _ = _run_append(
+            6, 2, slots + [-1] * (pad - used), pos + [0] * (pad - used), interleaved=interleaved, seed=3, blocks=page + 1)
+    slots = torch.tensor(slots + [-1] * (2100 - used), dtype=torch.int64, device=DEV)
+    pos = torch.tensor(pos + [0] * (2100 - used), dtype=torch.int32, device=DEV)
+    for pad in (500, 511, 512, 2047, 2048, 2100):          # the same rows in each call
+        cache, q = _rand_cache(page + 1, 2, 4), torch.zeros(pad, 6, 128, dtype=torch.bfloat16, device=DEV)
+        layers.qk_norm_rope_kv8(qkv[:pad], 6, 2, pos[:pad], slots[:pad], qn, kn, eps, table, q, cache, interleaved=interleaved)
+        got.append((cache.codes.view(torch.uint8), cache.scales, q[:used]))
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+
+
 @pytest.mark.parametrize("size", [2.0 ** -90, 2.0 ** -20, 300.0, 2.0 ** 60])
 def test_append_small_and_large_values(size):
     _run_append(2, 2, [5 + 16 * 3 + i for i in range(9)], list(range(5, 14)), norm=False, size=size)

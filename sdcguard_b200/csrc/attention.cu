@@ -430,10 +430,16 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
 //   warp 1      MMA, in the order PV0(j-1), S0(j), PV1(j-1), S1(j) for key tile j: S_x = Q_x K_j^T into TMEM,
 //               O_x += P_x V_{j-1} with P_x read from TMEM (the A operand of a tcgen05 MMA may live in tensor
 //               memory), so P never goes through shared memory;
-//   warps 4-7   softmax of query tile 0, warps 8-11 of query tile 1: one thread per row owns the row's whole key
-//               tile (no exchange between threads): masked maximum, conditional rescale of O (only when the
+//   warps 4-11  softmax of query tile 0, warps 12-19 of query tile 1: two threads per row, of warps w and w + 4, each
+//               with half of the key tile: masked maximum (exchanged), conditional rescale of O (only when the
 //               reference maximum moves by more than 2^8), P = exp2(S - max) rounded to bf16 and written back
-//               over the first 64 columns of S_x, the row sum of those bf16 weights; at the end O / l.
+//               over the last 64 columns of S_x, the row sum of those bf16 weights (in one order: the second thread
+//               goes on from the first's sum while the MMAs run); at the end O / l
+// Bound by the chain of one tile: its softmax (2290 cycles a 128-key tile, 1600 of them the exponentials, which the two
+// tiles share the unit for) and the MMAs behind it (1500), against 2048 cycles for the exponentials or the MMAs of both
+// tiles alone. 8 x 2048 tokens, 16 / 8 heads: 190 us, 725 TFLOP/s, 0.43 of a dense bf16 product's rate. One thread a row:
+// 193 us; 37, 517 and 1 tokens behind 301, 0 and 1000 (32 / 8 heads) 26.8 against 23.1, 1 x 4096 (8 / 8) 79 against 74,
+// the other way 16 x 512 (16 / 8) 54 against 57, where CTAs are short and start slower.
 // TMEM: S_0, S_1, O_0, O_1 (128 columns each). S_x(j + 1) overwrites P_x(j) only after PV_x(j) in the MMA order
 // (tcgen05 MMAs of one thread run in issue order), and the commit that signals S_x(j) also covers PV_x(j - 1), so
 // the softmax may rescale O_x as soon as it sees S_x(j). Every decision is per row and key tiles start at absolute
@@ -454,9 +460,30 @@ struct Ctl {
   int maxpos[2];
   int tok[2][ROWS];
   int pos[2][ROWS];
+  float part_max[2][2][ROWS];               // [query tile][thread of the row]
+  float sum[2][ROWS];                       // passed from a row's first thread to its second
+  int stop[2][2][ROWS];
 };
 constexpr int SMEM = OFF_CTL + static_cast<int>(sizeof(Ctl)) + 1024;
-constexpr int THREADS = 128 + 2 * ROWS;   // warpgroup 0: warp 0 TMA, warp 1 TMEM + MMA; warpgroups 1, 2: softmax
+constexpr int THREADS = 128 + 4 * ROWS;   // warpgroup 0: warps 0, 2 TMA, warp 1 TMEM + MMA; warpgroups 1-4: softmax
+// (a, b) * s + d in one instruction, each rounded once.
+__device__ __forceinline__ float2 fma2(uint32_t a, uint32_t b, float s, float d) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "r"(a), "r"(b), "f"(s), "f"(d));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// The two warps that share 32 rows of query tile x (warps w and w + 4).
+__device__ __forceinline__ void pair_sync(int x, int quarter) {
+  asm volatile("bar.sync %0, 64;" ::"r"(1 + x * 4 + quarter) : "memory");
+}
 constexpr int P_COL = 64;                 // P_x lives in columns [64, 128) of S_x (bf16 pairs)
 }  // namespace pp
 
@@ -480,11 +507,11 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
       mbar_init(&ctl->k_empty[i], 1);
       mbar_init(&ctl->v_empty[i], 1);
       mbar_init(&ctl->s_full[i], 1);
-      mbar_init(&ctl->p_full[i], ROWS);
+      mbar_init(&ctl->p_full[i], 2 * ROWS);
       mbar_init(&ctl->o_done[i], 1);
       ctl->maxpos[i] = -1;
     }
-    mbar_init(&ctl->q_ready, 2 * ROWS);
+    mbar_init(&ctl->q_ready, 4 * ROWS);
     mbar_init(&ctl->drain, 1);
     ctl->abort_flag = 0;
     fence_mbar_init();
@@ -497,9 +524,9 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // softmax thread: query tile x = warp / 4 - 1, row = TMEM lane it may access = (warp % 4) * 32 + lane
-  if (warp >= 4) {
-    const int x = (warp >> 2) - 1, r = (warp & 3) * 32 + lane;
+  // softmax thread: query tile x = (warp - 4) / 8, row = TMEM lane it may access = (warp % 4) * 32 + lane
+  if (warp >= 4 && ((warp >> 2) & 1)) {
+    const int x = (warp - 4) >> 3, r = (warp & 3) * 32 + lane;
     const int4 tl = x ? t1 : t0;
     const int ti = r / G;
     int tok = -1;
@@ -508,7 +535,8 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
     int ps = tok >= 0 ? p.pos[tok] : -1;
     if (ps >= p.limit) ps = -1;
     ctl->pos[x][r] = ps;
-    if (ps >= 0) atomicMax(&ctl->maxpos[x], ps);
+    const int top = __reduce_max_sync(0xffffffffu, ps);
+    if (lane == 0 && top >= 0) atomicMax(&ctl->maxpos[x], top);
   }
   __syncthreads();
   const int nt0 = ctl->maxpos[0] >= 0 ? ctl->maxpos[0] / KT + 1 : 0;
@@ -616,78 +644,79 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
       }
     }
   } else if (warp >= 4) {
-    // ------------------------------------------------------------ softmax / output: thread = one row of tile x
-    const int x = (warp >> 2) - 1;
-    const int r = (warp & 3) * 32 + lane;
-    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    // ------------------------------------------------------------ softmax / output: two threads a row of tile x
+    // part 0: keys [64, 128) of each key tile and dims [0, 64) of O; part 1: keys [0, 64), dims [64, 128). Both threads
+    // of a row go through every pair_sync, whatever fails: a wait that ran out sets the abort flag and goes on.
+    const int x = (warp - 4) >> 3, part = ((warp >> 2) & 1) ^ 1, quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const int tok = ctl->tok[x][r];
     const int pos = ctl->pos[x][r];
     const int head = kvh * G + (r % G);
     const int my_tiles = x ? nt1 : nt0;
     {
-      // the warp's 32 Q rows -> shared memory (128-byte swizzle, dims halves in separate 16 KB halves of the tile), two
-      // whole rows an instruction: a row per lane met 32 cache lines each time and took 5 us of a CTA (G divides ROWS, so
-      // it is a power of two)
+      // 16 of the pair's 32 Q rows -> shared memory (128-byte swizzle, dims halves in separate 16 KB halves of the tile),
+      // two whole rows an instruction: a row per lane met 32 cache lines each time and took 5 us of a CTA (G divides ROWS,
+      // so it is a power of two)
       uint8_t* qd = sm + OFF_Q + x * TILE_B;
       const int c = lane & 15;
-      uint4 v[16];
+      uint4 v[8];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int rr = (warp & 3) * 32 + 2 * i + (lane >> 4), tk = ctl->tok[x][rr];
+      for (int i = 0; i < 8; ++i) {
+        const int rr = quarter * 32 + part * 16 + 2 * i + (lane >> 4), tk = ctl->tok[x][rr];
         v[i] = tk >= 0 ? *reinterpret_cast<const uint4*>(
                              p.q + (static_cast<long long>(tk) * p.nq + kvh * G + (rr & (G - 1))) * D + c * 8)
                        : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int rr = (warp & 3) * 32 + 2 * i + (lane >> 4);
+      for (int i = 0; i < 8; ++i) {
+        const int rr = quarter * 32 + part * 16 + 2 * i + (lane >> 4);
         *reinterpret_cast<uint4*>(qd + (c >> 3) * HALF_B + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
       }
       fence_proxy_async_smem();
       mbar_arrive(&ctl->q_ready);
     }
     const uint32_t s_col = tmem + x * KT + lane_off, o_col = tmem + 2 * KT + x * D + lane_off;
-    float m_use = -INFINITY, l = 0.f;
-    bool stop = my_tiles == 0;
+    const int key0 = (1 - part) * 64;
+    float m_use = -INFINITY, l = 0.f;      // l: part 1's
+    bool stop = false;
     for (int j = 0; j < my_tiles; ++j) {
       if (!mbar_wait(&ctl->s_full[x], j & 1u, abort_flag)) {
         *abort_flag = 1;
         stop = true;
       }
-      if (__any_sync(0xffffffffu, stop)) {
-        stop = true;
-        break;
-      }
+      __syncwarp();
       tc_fence_after();
-      const int kbase = j * KT;
-      // S row of this key tile in two 64-column halves: the maximum over both (the second half stays in registers),
-      // then the weights of the second half, then the first half again. P (bf16 pairs) goes to columns [64, 128):
-      // the weights of keys [64, 128) over columns [96, 128) and those of keys [0, 64) over [64, 96), each written
-      // only after the S values under it were read.
-      const int lim = pos - kbase;      // keys [0, lim] of this tile are visible to the row
+      // This half of the S row, and the maximum over both. P (bf16 pairs) goes to columns [64, 128): the weights of keys
+      // [64, 128) over columns [96, 128) and those of keys [0, 64) over [64, 96), written after part 0 read the S
+      // values under them (pair_sync).
+      const int lim = pos - j * KT - key0;      // keys [0, lim] of this half are visible to the row
       // every key visible to every row of the warp (all but a prompt's last tiles): no masks, the same values
-      const bool full = __all_sync(0xffffffffu, lim >= KT - 1);
+      const bool full = __all_sync(0xffffffffu, lim >= 63);
       uint32_t v[2][32];
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (a maximum does not depend on the order)
+      tmem_ld32(s_col + key0, v[0]);
+      tmem_ld32(s_col + key0 + 32, v[1]);
+      tmem_wait_ld();
+      if (full) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        tmem_ld32(s_col + h * 64, v[0]);
-        tmem_ld32(s_col + h * 64 + 32, v[1]);
-        tmem_wait_ld();
-        if (full) {
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+          for (int i = 0; i < 32; i += 2)
+            mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], u32_as_f32(v[c][i]), u32_as_f32(v[c][i + 1]));
+      } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], u32_as_f32(v[c][i]));
-        } else {
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (h * 64 + c * 32 + i <= lim) mx4[i & 3] = fmaxf(mx4[i & 3], u32_as_f32(v[c][i]));
-        }
+          for (int i = 0; i < 32; ++i)
+            if (c * 32 + i <= lim) mx4[i & 3] = fmaxf(mx4[i & 3], u32_as_f32(v[c][i]));
       }
       float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      ctl->part_max[x][part][r] = mx;
+      tc_fence_before();
+      pair_sync(x, quarter);
+      tc_fence_after();
+      mx = fmaxf(mx, ctl->part_max[x][part ^ 1][r]);
       mx *= p.scale_log2;                // scale > 0: the maximum commutes with it
       float alpha = 1.f;
       if (mx > -INFINITY && (m_use == -INFINITY || mx > m_use + RESCALE_LOG2)) {
@@ -696,126 +725,136 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
         m_use = mx;
       }
       if (__any_sync(0xffffffffu, alpha != 1.f)) {
-        // PV_x(j-1) is complete (the commit of S_x(j) covers it): rescale this row of O_x
+        // PV_x(j-1) is complete (the commit of S_x(j) covers it): rescale this half of the row of O_x
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          tmem_ld32(o_col + c * 32, o);
+          uint32_t o[16];
+          tmem_ld16(o_col + part * 64 + c * 16, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(u32_as_f32(o[i]) * alpha);
-          tmem_st32(o_col + c * 32, o);
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(u32_as_f32(o[i]) * alpha);
+          tmem_st16(o_col + part * 64 + c * 16, o);
         }
       }
       const bool live = m_use > -INFINITY;
       const bool plain = full && __all_sync(0xffffffffu, live);
-      float ls = 0.f;
+      uint32_t pk[2][16];
 #pragma unroll
-      for (int h = 1; h >= 0; --h) {
-        if (h == 0) {
-          tmem_ld32(s_col, v[0]);
-          tmem_ld32(s_col + 32, v[1]);
-          tmem_wait_ld();
-        }
+      for (int c = 0; c < 2; ++c) {
+        if (plain) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t pk[16];
-          if (plain) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const uint32_t w = pack_bf16x2(ex2(u32_as_f32(v[c][i]) * p.scale_log2 - m_use),
-                                             ex2(u32_as_f32(v[c][i + 1]) * p.scale_log2 - m_use));
-              pk[i >> 1] = w;
-              ls += u32_as_f32(w << 16) + u32_as_f32(w & 0xffff0000u);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const int key = h * 64 + c * 32 + i;
-              const float p0 = (key <= lim && live) ? ex2(u32_as_f32(v[c][i]) * p.scale_log2 - m_use) : 0.f;
-              const float p1 = (key + 1 <= lim && live) ? ex2(u32_as_f32(v[c][i + 1]) * p.scale_log2 - m_use) : 0.f;
-              const uint32_t w = pack_bf16x2(p0, p1);
-              pk[i >> 1] = w;
-              ls += u32_as_f32(w << 16) + u32_as_f32(w & 0xffff0000u);
-            }
+          for (int i = 0; i < 32; i += 2) {
+            const float2 e = fma2(v[c][i], v[c][i + 1], p.scale_log2, -m_use);
+            pk[c][i >> 1] = pack_bf16x2(ex2(e.x), ex2(e.y));
           }
-          tmem_st16(s_col + P_COL + h * 32 + c * 16, pk);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const int key = c * 32 + i;
+            const float p0 = (key <= lim && live) ? ex2(u32_as_f32(v[c][i]) * p.scale_log2 - m_use) : 0.f;
+            const float p1 = (key + 1 <= lim && live) ? ex2(u32_as_f32(v[c][i + 1]) * p.scale_log2 - m_use) : 0.f;
+            pk[c][i >> 1] = pack_bf16x2(p0, p1);
+          }
         }
+        tmem_st16(s_col + P_COL + (1 - part) * 32 + c * 16, pk[c]);
       }
-      l += ls;
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(&ctl->p_full[x]);
+      // the row's sum over keys [64, 128), then [0, 64), one order whoever holds them
+      const auto add = [&](float s) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s += u32_as_f32(pk[c][i] << 16) + u32_as_f32(pk[c][i] & 0xffff0000u);
+        return s;
+      };
+      if (part == 0) ctl->sum[x][r] = add(0.f);
+      pair_sync(x, quarter);
+      if (part == 1) l += add(ctl->sum[x][r]);
     }
-    if (!stop && my_tiles > 0) {
-      if (!mbar_wait(&ctl->o_done[x], 0, abort_flag)) {
-        *abort_flag = 1;
-        stop = true;
-      }
-      if (__any_sync(0xffffffffu, stop)) stop = true;
+    if (my_tiles > 0 && !mbar_wait(&ctl->o_done[x], 0, abort_flag)) {
+      *abort_flag = 1;
+      stop = true;
     }
+    // both warps give up, or neither
+    ctl->stop[x][part][r] = stop;
+    if (part == 1) ctl->sum[x][r] = l;
+    pair_sync(x, quarter);
+    stop = __any_sync(0xffffffffu, stop || ctl->stop[x][part ^ 1][r]);
     if (!stop && my_tiles > 0) {
       tc_fence_after();
+      l = ctl->sum[x][r];
       const float inv = l > 0.f ? 1.f / l : 0.f;
       __nv_bfloat16* orow = p.o + (static_cast<long long>(tok < 0 ? 0 : tok) * p.nq + head) * D;
-      float sq = 0.f;
       int bad = -1;
+      uint32_t w[2][16];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t v[32];
-        tmem_ld32(o_col + c * 32, v);
+        tmem_ld32(o_col + part * 64 + c * 32, v);
         tmem_wait_ld();
-        uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          w[i] = pack_bf16x2(u32_as_f32(v[2 * i]) * inv, u32_as_f32(v[2 * i + 1]) * inv);
-          const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-          sq = fmaf(f.x, f.x, fmaf(f.y, f.y, sq));
-        }
+        for (int i = 0; i < 16; ++i) w[c][i] = pack_bf16x2(u32_as_f32(v[2 * i]) * inv, u32_as_f32(v[2 * i + 1]) * inv);
         if (p.check == nullptr) {
           // through the Q tile, which the MMAs are done with, to whole rows
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int ch = c * 4 + i;
-            *reinterpret_cast<uint4*>(sm + OFF_Q + x * TILE_B + (ch >> 3) * HALF_B + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) =
-                make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            *reinterpret_cast<uint4*>(sm + OFF_Q + x * TILE_B + part * HALF_B + r * 128 + ((ch ^ (r & 7)) << 4)) =
+                make_uint4(w[c][4 * i], w[c][4 * i + 1], w[c][4 * i + 2], w[c][4 * i + 3]);
           }
         } else if (tok >= 0) {
-          uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
+          uint4* dst = reinterpret_cast<uint4*>(orow + part * 64 + c * 32);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint4 nv = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            const uint4 nv = make_uint4(w[c][4 * i], w[c][4 * i + 1], w[c][4 * i + 2], w[c][4 * i + 3]);
             if (bad < 0) {
               const uint4 ov = dst[i];
               const uint32_t a[4] = {nv.x, nv.y, nv.z, nv.w}, b[4] = {ov.x, ov.y, ov.z, ov.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int dd = bf16x2_diff(a[e], b[e]);
-                if (bad < 0 && dd >= 0) bad = c * 32 + i * 8 + e * 2 + dd;
+                if (bad < 0 && dd >= 0) bad = part * 64 + c * 32 + i * 8 + e * 2 + dd;
               }
             }
           }
         }
       }
+      const auto squares = [&](float sq) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[c][i]));
+            sq = fmaf(f.x, f.x, fmaf(f.y, f.y, sq));
+          }
+        return sq;
+      };
+      pair_sync(x, quarter);             // (l was read, both halves of the rows wait in shared memory)
       if (p.check == nullptr) {
-        __syncwarp();
         const int c = lane & 15;
 #pragma unroll 4
-        for (int i = 0; i < 16; ++i) {
-          const int rr = (warp & 3) * 32 + 2 * i + (lane >> 4), tk = ctl->tok[x][rr];
+        for (int i = 0; i < 8; ++i) {
+          const int rr = quarter * 32 + part * 16 + 2 * i + (lane >> 4), tk = ctl->tok[x][rr];
           const uint4 v = *reinterpret_cast<const uint4*>(sm + OFF_Q + x * TILE_B + (c >> 3) * HALF_B + rr * 128 +
                                                           (((c & 7) ^ (rr & 7)) << 4));
           if (tk >= 0)
             *reinterpret_cast<uint4*>(p.o + (static_cast<long long>(tk) * p.nq + kvh * G + (rr & (G - 1))) * D + c * 8) = v;
         }
       }
+      if (part == 0) {
+        ctl->sum[x][r] = squares(0.f);
+        ctl->stop[x][0][r] = bad;
+      }
+      pair_sync(x, quarter);
       if (tok >= 0) {
-        if (p.check != nullptr && bad >= 0)
+        if (p.check != nullptr && bad >= 0 && (part == 0 || ctl->stop[x][0][r] < 0))      // the row's first difference
           report_replay_mismatch(p.check, static_cast<unsigned long long>(tok) * p.nq * D + head * D + bad);
-        if (p.check == nullptr && p.row_sq != nullptr) atomicAdd(p.row_sq + tok, sq);
+        if (part == 1 && p.check == nullptr && p.row_sq != nullptr) atomicAdd(p.row_sq + tok, squares(ctl->sum[x][r]));
       }
     }
-    if (p.check != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && r == 0 && x == 0) atomicAdd(p.check + 2, 1ull);
+    if (p.check != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && r == 0 && x == 0 && part == 0) atomicAdd(p.check + 2, 1ull);
   }
   tc_fence_before();
   __syncthreads();

@@ -272,7 +272,8 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
              row_sq: Optional[torch.Tensor] = None, scale: Optional[float] = None,
              check: Optional[torch.Tensor] = None, pages_from: int = 0, pages_step: int = 64) -> torch.Tensor:
     """`prefill` over a cache of 8 bits: the plan's pages are expanded to bf16 (exact for power-of-two scales), then the
-    tensor-core prefill reads those. q (T, nq, 128), tiles from `prefill_tiles`, requests numbered as in the plan. A
+    tensor-core prefill reads those. A CTA walks over all keys of its rows, so a few new tokens behind many keys are faster
+    through `decode8`, a sequence for each token (seq_req its request, ctx its position + 1). q (T, nq, 128), tiles from `prefill_tiles`, requests numbered as in the plan. A
     position outside the plan's table gives a row of zeros, a page outside the cache NaN. With `check`: every
     pages_step-th expanded page from pages_from on and the rows of the replay tiles are compared."""
     given = out

@@ -428,6 +428,19 @@ def test_decode_table_views_requests_and_scale():
             (2 ** -11 + 2 ** -18) * cache.values().abs().max().double()).all()
 
 
+@pytest.mark.parametrize("nq,nkv", [(4, 4), (16, 2)])
+def test_decode_of_several_tokens_of_a_request(nq, nkv):
+    """A sequence for each new token, its request's pages and its own length: what a prefill of those tokens gives."""
+    lens, prior = [9, 4, 1], [394, 1317, 0]
+    ctxs = [a + b for a, b in zip(lens, prior)]
+    _, cache, bt, _, _, _ = _decode_case(ctxs, nq, nkv, seed=2)
+    q = torch.randn(14, nq, 128, device=DEV).bfloat16()
+    pos = torch.cat([torch.arange(p, p + n) for p, n in zip(prior, lens)]).int().to(DEV)
+    req = torch.repeat_interleave(torch.arange(3), torch.tensor(lens)).int().to(DEV)
+    args = (q, cache, bt, req, pos + 1, attention.decode8_plan(14, nq, nkv, max(ctxs), DEV))
+    _check_decode(args, attention.decode8(*args))
+
+
 def test_decode_offsets_beyond_32_bits():
     """Pages more than 2^31 bytes into the codes, and a long sequence."""
     nkv, blocks = 8, 150000                       # 4.9 GB of codes

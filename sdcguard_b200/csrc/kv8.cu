@@ -752,12 +752,12 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv8_decode_kernel
   DecodeSmem<NT>& sm = *reinterpret_cast<DecodeSmem<NT>*>(decode_smem + ((1024 - (smem_u32(decode_smem) & 1023)) & 1023));
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int b = p.seq_idx ? p.seq_idx[blockIdx.x] : blockIdx.x;
-  if (b < 0 || b >= p.nseqs) return;
   const int kvh = blockIdx.y;
+  if (p.check != nullptr && blockIdx.x == 0 && kvh == 0 && blockIdx.z == 0 && tid == 0) atomicAdd(p.check + 2, 1ull);
+  if (b < 0 || b >= p.nseqs) return;
   const int n = p.ctx[b], req = p.seq_req[b];
   const int pages = pages_of(n);
   const bool fits = row_fits(p, n, req);
-  if (p.check != nullptr && blockIdx.x == 0 && kvh == 0 && blockIdx.z == 0 && tid == 0) atomicAdd(p.check + 2, 1ull);
   if (!fits || n == 0) {
     if (blockIdx.z != 0) return;
     const float v = fits ? 0.f : __int_as_float(0x7fffffff);
@@ -1090,6 +1090,40 @@ __global__ void __launch_bounds__(PARTS * D) kv8_combine_kernel(const DecodePara
   }
 }
 
+// The tokens of prefill tiles (request, first token or place in row_idx, tokens, -1 or that place) as sequences of the
+// decode kernel: request and keys (position + 1) of token t, and the list of the tokens to run: a prefill's token t at
+// place t, a replay's behind them as row_idx lists it; -1 elsewhere. A position outside the table has no keys. One CTA: a
+// few hundred tokens, 2 us.
+struct TokensParams {
+  const int4* tiles;
+  int ntiles, tile_tokens;
+  const int* row_idx;
+  int nrows;
+  const int* pos;
+  int limit;                 // keys that a row of the table has room for
+  int T;
+  int* req;                  // [T]
+  int* ctx;                  // [T]
+  int* idx;                  // [T + nrows]
+};
+__global__ void __launch_bounds__(1024) kv8_tokens_kernel(const TokensParams p) {
+  for (int i = threadIdx.x; i < p.T + p.nrows; i += 1024) p.idx[i] = -1;
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (int i = threadIdx.x >> 5; i < p.ntiles; i += 32) {
+    const int4 tl = p.tiles[i];
+    for (int j = lane; j < min(tl.z, p.tile_tokens); j += 32) {
+      if (tl.w >= 0 && tl.w + j >= p.nrows) break;
+      const int t = tl.w >= 0 ? p.row_idx[tl.w + j] : tl.y + j;
+      if (t < 0 || t >= p.T) continue;
+      const int ps = p.pos[t];
+      p.req[t] = tl.x;
+      p.ctx[t] = ps >= 0 && ps < p.limit ? ps + 1 : 0;
+      p.idx[tl.w >= 0 ? p.T + tl.w + j : t] = t;
+    }
+  }
+}
+
 template <int NT>
 static int launch_decode(const CUtensorMap& tm, const DecodeParams& p, int nrun, int z, cudaStream_t st) {
   // the attribute belongs to a device; one bit for each that has it (setting it twice does no harm)
@@ -1235,6 +1269,30 @@ int sdc_kv8_expand(const Kv8ExpandArgs* args) {
   if (n <= 0) return 0;
   const long long blocks = (n * 2 * nkv * 32 + 255) / 256;
   kv8_expand_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+
+struct Kv8TokensArgs {
+  const void* tiles;
+  int ntiles;
+  int tile_tokens;
+  const int* row_idx;
+  int nrows;
+  const int* pos;
+  int limit;
+  int T;
+  void* req;
+  void* ctx;
+  void* idx;
+  void* stream;
+};
+int sdc_kv8_tokens(const Kv8TokensArgs* args) {
+  const auto& [tiles, ntiles, tile_tokens, row_idx, nrows, pos, limit, T, req, ctx, idx, stream] = *args;
+  if (T <= 0) return 0;
+  if (ntiles < 0 || nrows < 0 || (nrows > 0 && row_idx == nullptr)) return -1;
+  const TokensParams p{static_cast<const int4*>(tiles), ntiles, tile_tokens, row_idx, nrows, pos, limit, T,
+                       static_cast<int*>(req), static_cast<int*>(ctx), static_cast<int*>(idx)};
+  kv8_tokens_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -238,6 +238,7 @@ class Prefill8Plan:
     table: torch.Tensor        # (R, W) int32 places in that list
     work: torch.Tensor         # (P, 2, nkv, 16, 128) bf16
     nkv: int
+    block_table: torch.Tensor  # (R, W) int32 page ids (a copy)
 
 
 def prefill8_plan(block_table: torch.Tensor, ctx_lens: Sequence[int], nkv: int,
@@ -264,7 +265,34 @@ def prefill8_plan(block_table: torch.Tensor, ctx_lens: Sequence[int], nkv: int,
     elif work.dtype != torch.bfloat16 or work.numel() < need or not work.is_contiguous() or work.device != dev \
             or work.data_ptr() % 128:
         raise ValueError(f"work must be contiguous bf16 of at least {need} elements on {dev}")
-    return Prefill8Plan(pages, table.to(dev), work.view(-1)[:need].view(total, 2, nkv, PAGE, 128), nkv)
+    return Prefill8Plan(pages, table.to(dev), work.view(-1)[:need].view(total, 2, nkv, PAGE, 128), nkv,
+                        block_table[:, :w].clone(memory_format=torch.contiguous_format))
+
+
+# A prefill's CTA walks over all keys of its rows, 2 us for 128 of them; the decode kernel cuts the keys but reads them for
+# every token. So few rows (tokens x kv heads) go there: 54 tokens x 4 heads behind 3945 keys 36 us against 78, 23 x 2 behind
+# 1682 11 against 36, 64 x 8 behind 4000 (above the line) 73 against 84, 128 x 8 behind 8000 252 against 142.
+FEW_ROWS = 400
+
+
+def _prefill8_few(q, cache, plan, pos, tiles, out, row_idx, row_sq, scale, check):
+    t, nq, nkv, dev, keys = q.shape[0], q.shape[1], plan.nkv, cache.device, plan.table.shape[1] * PAGE
+    if cache.num_blocks * nkv >= 1 << 26:
+        raise ValueError(f"{cache.num_blocks} pages of {nkv} heads (below 2^26 in all)")
+    rows = 0 if row_idx is None else row_idx.shape[0]
+    seg, segs = decode8_cut(t, nkv, keys)
+    lists = torch.empty(3 * t + rows, dtype=torch.int32, device=dev)
+    part = torch.empty(t * nq * segs * 132, dtype=torch.float32, device=dev) if segs > 1 else None
+    at = lists.data_ptr()
+    kv8.launch("sdc_kv8_tokens", dev, (
+        tiles.data_ptr(), tiles.shape[0], ROWS // (nq // nkv), kv8.ptr(row_idx), rows, pos.data_ptr(), keys, t, at,
+        at + 4 * t, at + 8 * t))
+    bt = plan.block_table
+    kv8.launch("sdc_kv8_decode", dev, (
+        q.data_ptr(), out.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, bt.data_ptr(),
+        bt.shape[0], bt.shape[1], bt.stride(0), at, at + 4 * t, at + 8 * t, t + rows, t, nq, nkv, seg, segs,
+        _SCALE if scale is None else scale, kv8.ptr(part), kv8.ptr(row_sq), kv8.ptr(check)))
+    return out
 
 
 def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Tensor, tiles: torch.Tensor,
@@ -272,10 +300,10 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
              row_sq: Optional[torch.Tensor] = None, scale: Optional[float] = None,
              check: Optional[torch.Tensor] = None, pages_from: int = 0, pages_step: int = 64) -> torch.Tensor:
     """`prefill` over a cache of 8 bits: the plan's pages are expanded to bf16 (exact for power-of-two scales), then the
-    tensor-core prefill reads those. A CTA walks over all keys of its rows, so a few new tokens behind many keys are faster
-    through `decode8`, a sequence for each token (seq_req its request, ctx its position + 1). q (T, nq, 128), tiles from `prefill_tiles`, requests numbered as in the plan. A
-    position outside the plan's table gives a row of zeros, a page outside the cache NaN. With `check`: every
-    pages_step-th expanded page from pages_from on and the rows of the replay tiles are compared."""
+    tensor-core prefill reads those; a call of few tokens (T kv heads <= FEW_ROWS) runs through the decode kernel instead, a
+    sequence for each token, so a row's last bits depend on which of the two its call takes. q (T, nq, 128), tiles from `prefill_tiles`, requests numbered as in the plan. A
+    position outside the plan's table gives a row of zeros, a page outside the cache NaN. With `check`: the rows of the
+    replay tiles are compared, and every pages_step-th expanded page (where there are such) from pages_from on."""
     given = out
     t, nq, out = _want_q(q, cache, out)
     dev, nkv = cache.device, cache.nkv
@@ -295,6 +323,8 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
     _want_extra(row_sq, check, t, dev)
     if t == 0 or tiles.shape[0] == 0:
         return out
+    if t * nkv <= FEW_ROWS and nq // nkv <= 16 and plan.table.shape[1] <= (1 << 24) // PAGE:
+        return _prefill8_few(q, cache, plan, pos, tiles, out, row_idx, row_sq, scale, check)
     kv8.launch("sdc_kv8_expand", dev, (
         cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, plan.pages.data_ptr(), plan.pages.shape[0],
         nkv, plan.work.data_ptr(), pages_from, pages_step, kv8.ptr(check)))

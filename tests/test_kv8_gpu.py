@@ -506,6 +506,44 @@ def test_prefill_matches_64_bits_and_replays_exactly(nq, nkv, lens, prior):
     assert _flat(st[2])[:2] == (math.inf, (n - 1) * 2 * nkv + nkv)
 
 
+@pytest.mark.parametrize("nq,nkv,lens,prior", [
+    (4, 4, [9, 9, 1], [3945, 0, 700]), (16, 2, [23, 4], [1682, 16]), (8, 8, [1], [0]), (16, 1, [160, 200], [40, 3]),
+    (2, 2, [40, 33, 1], [0, 7, 5000])])
+def test_prefill_of_few_tokens(nq, nkv, lens, prior):
+    """The decode kernel's path: 64 bits, replays, rows that no tile names, positions and pages outside."""
+    ctxs = [a + b for a, b in zip(lens, prior)]
+    _, cache, bt, _, _, _ = _decode_case(ctxs, nq, nkv, seed=nq, spread=1.0)
+    T, G = sum(lens), nq // nkv
+    assert (T + 3) * nkv <= attention.FEW_ROWS
+    q = torch.randn(T + 3, nq, 128, device=DEV).bfloat16()
+    starts = [sum(lens[:i]) for i in range(len(lens))]
+    pos = torch.cat([torch.arange(p, p + n) for p, n in zip(prior, lens)] + [torch.zeros(3)]).int().to(DEV)
+    tiles = attention.prefill_tiles(starts, lens, G).to(DEV)
+    plan = attention.prefill8_plan(bt, ctxs, nkv)
+    rs, out = torch.zeros(T + 3, device=DEV), torch.full_like(q, 7.0)
+    attention.prefill8(q, cache, plan, pos, tiles, out=out, row_sq=rs)
+    assert (out[T:] == 7).all() and (rs[T:] == 0).all()
+    assert torch.allclose(rs[:T], out[:T].float().square().sum((1, 2)), rtol=2e-5)
+    req = torch.repeat_interleave(torch.arange(len(lens)), torch.tensor(lens)).int().to(DEV)
+    _check_decode((q[:T], cache, bt, req, pos[:T] + 1, None), out[:T])
+    rt, ridx = attention.replay_tiles([[s + n - 1] for s, n in zip(starts, lens)], G)
+    rt, ridx = rt.to(DEV), ridx.to(DEV)
+    st = _state(2)
+    attention.prefill8(q, cache, plan, pos, rt, out=out, row_idx=ridx, check=st[0])
+    out.view(torch.int16)[T - 1, nq - 1, 9] ^= 1
+    attention.prefill8(q, cache, plan, pos, rt, out=out, row_idx=ridx, check=st[1])
+    assert _flat(st[0])[0] == 0 and st[:, 2].tolist() == [1, 1]
+    assert _flat(st[1])[:2] == (math.inf, ((T - 1) * nq + nq - 1) * 128 + 9)
+    want = attention.prefill8(q, cache, plan, pos, tiles)[:T]
+    pos[0] = 1 << 20
+    out = attention.prefill8(q, cache, plan, pos, tiles)[:T]
+    assert (out[0] == 0).all() and torch.equal(out[1:], want[1:])
+    pos[0] = prior[0]
+    bt[-1, 0] = 1 << 20
+    out = attention.prefill8(q, cache, attention.prefill8_plan(bt, ctxs, nkv), pos, tiles)[:T]
+    assert out[starts[-1]:].isnan().all() and torch.equal(out[:starts[-1]], want[:starts[-1]])
+
+
 def test_prefill_pages_and_positions_outside():
     """A page outside the cache gives NaN to its request alone; a position outside the plan's table gives zeros."""
     lens = [40, 33]

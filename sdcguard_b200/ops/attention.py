@@ -13,6 +13,7 @@ import math
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
+import numpy as np
 import torch
 
 from .. import _native
@@ -252,21 +253,20 @@ def prefill8_plan(block_table: torch.Tensor, ctx_lens: Sequence[int], nkv: int,
     if not counts or min(int(n) for n in ctx_lens) < 1 or max(counts) > width:
         raise ValueError(f"ctx_lens {list(ctx_lens)[:8]}: at least one key each, and no more than {width} pages")
     total, w = sum(counts), max(counts)
-    c = torch.tensor(counts)
-    first = torch.cumsum(c, 0) - c
-    place = torch.arange(w)[None]
+    c = np.array(counts)
+    place = np.arange(w)
     used = place < c[:, None]
-    table = torch.where(used, first[:, None] + place, 0).to(torch.int32)
-    r, j = (t.to(dev, non_blocking=True) for t in used.nonzero(as_tuple=True))
-    pages = block_table[r, j]
+    table = np.where(used, (np.cumsum(c) - c)[:, None] + place, 0)
+    both = torch.from_numpy(np.concatenate([np.flatnonzero(used), table.ravel()]).astype(np.int32)).to(dev)   # one copy
+    bt = block_table[:, :w].clone(memory_format=torch.contiguous_format)
+    pages, table = bt.view(-1).index_select(0, both[:total]), both[total:].view(-1, w)
     need = total * expanded_page(nkv)
     if work is None:
         work = torch.empty(need, dtype=torch.bfloat16, device=dev)
     elif work.dtype != torch.bfloat16 or work.numel() < need or not work.is_contiguous() or work.device != dev \
             or work.data_ptr() % 128:
         raise ValueError(f"work must be contiguous bf16 of at least {need} elements on {dev}")
-    return Prefill8Plan(pages, table.to(dev), work.view(-1)[:need].view(total, 2, nkv, PAGE, 128), nkv,
-                        block_table[:, :w].clone(memory_format=torch.contiguous_format))
+    return Prefill8Plan(pages, table, work.view(-1)[:need].view(total, 2, nkv, PAGE, 128), nkv, bt)
 
 
 # A prefill's CTA walks over all keys of its rows, 2 us for 128 of them; the decode kernel cuts the keys but reads them for

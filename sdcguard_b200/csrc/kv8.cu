@@ -573,8 +573,8 @@ __global__ void __launch_bounds__(256) kv8_append_check_kernel(const AppendParam
 // ------------------------------------------------------------------------------------------------ pages to bf16
 // Pages of the list in bf16 (exact while scales are powers of two), for the tensor-core prefill: a prefill reads each
 // page once for every 256 / group of its query rows, so expanding it once costs less than expanding it in every CTA.
-// One warp per (page, K / V, kv head): 2 KB in, 4 KB out; 1024 pages of 8 heads 15 us, 6.7 TB/s. A page id outside the cache gives NaN. With `check`: every
-// `step`-th page of the list from `from` on is compared instead of written.
+// One warp per (page, K / V, kv head): 2 KB in, 4 KB out; 1024 pages of 8 heads 15 us, 6.7 TB/s. A page id outside the
+// cache gives NaN. With `check`: every `step`-th page of the list from `from` on is compared instead of written.
 struct ExpandParams {
   const uint8_t* codes;
   const float* scales;

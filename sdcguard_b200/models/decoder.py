@@ -294,7 +294,8 @@ class CheckedDecoder:
     def forward(self, meta: StepMeta, cache: torch.Tensor, layer_range: Optional[tuple] = None,
                 hidden: Optional[tuple] = None, last: bool = True):
         """Runs one step; returns logits (L, vocab) bf16 for meta.logits_rows. cache: (layers, blocks, 2, nkv,
-        16, 128) bf16, or a KV8Cache of as many layers (a prefill then needs meta.plan8). Pipeline stages: layer_range=(lo, hi) runs only those layers (cache then holds hi - lo layers),
+        16, 128) bf16, or a KV8Cache of as many layers (a prefill then needs meta.plan8). Pipeline stages:
+        layer_range=(lo, hi) runs only those layers (cache then holds hi - lo layers),
         hidden=(x, resid) enters after layer lo - 1 instead of the embedding, and last=False returns the (x, resid)
         pair after layer hi - 1 (x: the last sublayer's output, not yet added to the residual resid)."""
         cfg = self.cfg

@@ -203,8 +203,9 @@ def decode8(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_req
     if nq != plan.nq or nkv != plan.nkv or b > plan.nseq:
         raise ValueError(f"q {tuple(q.shape)} and {nkv} kv heads do not fit the plan ({plan.nseq} sequences, {plan.nq} "
                          f"query and {plan.nkv} kv heads)")
-    if block_table.dtype is not torch.int32 or block_table.device != dev or block_table.dim() != 2 \
-            or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
+    table, stride = block_table.shape, block_table.stride()
+    if block_table.dtype is not torch.int32 or block_table.device != dev or len(table) != 2 \
+            or (stride[1] != 1 and table[1] > 1):
         raise ValueError("block_table must be int32 (requests, pages) with contiguous rows on the cache's device")
     kv8.want(seq_req, torch.int32, (b,), dev, "seq_req")
     kv8.want(ctx, torch.int32, (b,), dev, "ctx")
@@ -220,7 +221,7 @@ def decode8(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, seq_req
         _want_extra(row_sq, check, b, dev)
     kv8.launch("sdc_kv8_decode", dev, (
         q.data_ptr(), out.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks,
-        block_table.data_ptr(), block_table.shape[0], block_table.shape[1], block_table.stride(0), seq_req.data_ptr(),
+        block_table.data_ptr(), table[0], table[1], stride[0], seq_req.data_ptr(),
         ctx.data_ptr(), kv8.ptr(seq_idx), b if seq_idx is None else seq_idx.shape[0], b, nq, nkv, plan.seg_pages,
         plan.max_segs, _SCALE if scale is None else scale, kv8.ptr(plan.part), kv8.ptr(row_sq), kv8.ptr(check)))
     return out
@@ -301,9 +302,10 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
              check: Optional[torch.Tensor] = None, pages_from: int = 0, pages_step: int = 64) -> torch.Tensor:
     """`prefill` over a cache of 8 bits: the plan's pages are expanded to bf16 (exact for power-of-two scales), then the
     tensor-core prefill reads those; a call of few tokens (T kv heads <= FEW_ROWS) runs through the decode kernel instead, a
-    sequence for each token, so a row's last bits depend on which of the two its call takes. q (T, nq, 128), tiles from `prefill_tiles`, requests numbered as in the plan. A
-    position outside the plan's table gives a row of zeros, a page outside the cache NaN. With `check`: the rows of the
-    replay tiles are compared, and every pages_step-th expanded page (where there are such) from pages_from on."""
+    sequence for each token, so a row's last bits depend on which of the two its call takes. q (T, nq, 128), tiles from
+    `prefill_tiles`, requests numbered as in the plan. A position outside the plan's table gives a row of zeros, a page
+    outside the cache NaN. With `check`: the rows of the replay tiles are compared, and every pages_step-th expanded page
+    (where there are such) from pages_from on."""
     given = out
     t, nq, out = _want_q(q, cache, out)
     dev, nkv = cache.device, cache.nkv

@@ -72,13 +72,13 @@ def qk_norm_rope_kv8(qkv: torch.Tensor, nq: int, nkv: int, pos: torch.Tensor, sl
     A token whose slot lies outside the cache, or whose position lies outside the table, is not stored, and its row of
     q_out is NaN. With `check` (a state row) and `rows`: the sampled tokens are recomputed and compared with q_out and
     the cache instead of written; this holds until a later call raises the scale of their page."""
-    t = qkv.shape[0]
-    heads = nq + 2 * nkv
-    dev = cache.device
+    shape, stride = qkv.shape, qkv.stride()              # (each read of a tensor's attribute costs a tenth of a microsecond)
+    t, heads, dev = shape[0], nq + 2 * nkv, cache.device
     if not cache.one_layer or cache.nkv != nkv:
         raise ValueError(f"cache must be one layer with {nkv} kv heads, got {tuple(cache.codes.shape)}")
-    if qkv.shape != (t, heads * 128) or qkv.dtype is not torch.bfloat16 or qkv.device != dev or qkv.data_ptr() % 8 \
-            or qkv.stride(1) != 1 or (t > 1 and qkv.stride(0) % 4):
+    at = qkv.data_ptr()
+    if shape != (t, heads * 128) or qkv.dtype is not torch.bfloat16 or qkv.device != dev or at % 8 or stride[1] != 1 \
+            or (t > 1 and stride[0] % 4):
         raise ValueError(f"qkv must be bf16 (T, {heads * 128}) on {dev} with contiguous rows on 8-byte boundaries")
     kv8.want(q_out, torch.bfloat16, (t, nq, 128), dev, "q_out", align=8)
     kv8.want(pos, torch.int32, (t,), dev, "pos")
@@ -88,7 +88,8 @@ def qk_norm_rope_kv8(qkv: torch.Tensor, nq: int, nkv: int, pos: torch.Tensor, sl
             kv8.want(w, torch.bfloat16, (128,), dev, name, align=8)
     table_rows = rotary = 0
     if cos_sin is not None:
-        table_rows, rotary = cos_sin.shape[0], 2 * cos_sin.shape[1]
+        shape = cos_sin.shape
+        table_rows, rotary = shape[0], 2 * shape[1]
         kv8.want(cos_sin, torch.float32, (table_rows, rotary // 2, 2), dev, "cos_sin", align=16)
         if rotary % 8 or not 0 < rotary <= 128:
             raise ValueError(f"{rotary} rotated dims: a multiple of 8, at most 128")
@@ -98,7 +99,7 @@ def qk_norm_rope_kv8(qkv: torch.Tensor, nq: int, nkv: int, pos: torch.Tensor, sl
         kv8.want(rows, torch.int32, (rows.shape[0],), dev, "rows")
         kv8.want_state(check, dev)
     kv8.launch("sdc_kv8_append", dev, (
-        qkv.data_ptr(), qkv.stride(0) if t > 1 else heads * 128, t, nq, nkv, pos.data_ptr(), slots.data_ptr(),
+        at, stride[0] if t > 1 else heads * 128, t, nq, nkv, pos.data_ptr(), slots.data_ptr(),
         kv8.ptr(q_norm), kv8.ptr(k_norm), eps, kv8.ptr(cos_sin), table_rows, rotary, interleaved, q_out.data_ptr(),
         cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, kv8.ptr(rows),
         0 if rows is None else rows.shape[0], kv8.ptr(check)))

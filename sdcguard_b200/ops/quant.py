@@ -161,12 +161,13 @@ class QuantWeights:
 
         With `check` (a state row) and `blocks` (int32 indices of 16 outputs each): those outputs are recomputed and
         compared with `out` (the call's result), bit for bit, instead of written."""
-        dev, m, given = self.codes.device, x.shape[0], out
+        shape, stride, at = x.shape, x.stride(), x.data_ptr()
+        dev, m, given = self.codes.device, shape[0], out
         if self.bits != 4 or self.group % 32:
             raise ValueError("matvec reads INT4 codes with groups of a multiple of 32")
         kv8.want(self.codes, torch.uint8, (self.n, self.k // 2), dev, "codes", align=16)
-        if x.shape != (m, self.k) or x.dtype is not torch.bfloat16 or x.device != dev or x.data_ptr() % 16 \
-                or x.stride(1) != 1 or (m > 1 and x.stride(0) % 8):
+        if shape != (m, self.k) or x.dtype is not torch.bfloat16 or x.device != dev or at % 16 or stride[1] != 1 \
+                or (m > 1 and stride[0] % 8):
             raise ValueError(f"x must be bf16 (m, {self.k}) on {dev} with contiguous rows on 16-byte boundaries")
         if m > MATVEC_ROWS:
             raise ValueError(f"{m} rows: matvec takes up to {MATVEC_ROWS} (more go to the GEMM on the effective weights)")
@@ -192,7 +193,7 @@ class QuantWeights:
         if m > 8 and blocks is None and self.n * self.k > 1 << 24:
             packed = torch.empty(-(-self.k // 128) * 128 * (16 if m <= 16 else 32), dtype=torch.bfloat16, device=dev)
         kv8.launch("sdc_matvec4", dev, (
-            x.data_ptr(), x.stride(0) if m > 1 else self.k, m, self.n, self.k, self.group, self.codes.data_ptr(),
+            at, stride[0] if m > 1 else self.k, m, self.n, self.k, self.group, self.codes.data_ptr(),
             self.scales.data_ptr(), kv8.ptr(self.zeros), mode, kv8.ptr(bias), out.data_ptr(),
             out.stride(0) if m > 1 else self.n, kv8.ptr(packed), kv8.ptr(blocks),
             0 if blocks is None else blocks.shape[0], kv8.ptr(check)))

@@ -13,6 +13,7 @@
 // CTAs/SMs at a different time and compared bit for bit (sdcguard_b200/ops/attention.py). The reference checks
 // attention by a sampled fp32 recompute against an error bound (src/sdcguard/serve_attn.py:5-48, kernels
 // `_attn_part` :335 and `_attn_judge` :414); an exact replay needs no bound and sees every flipped bit.
+#include <atomic>
 #include <cstdlib>
 
 #include "common.cuh"
@@ -454,7 +455,7 @@ constexpr int PG_BYTES = PAGE * D * 2;
 struct Ctl {
   uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2];
   uint64_t s_full[2], p_full[2], o_done[2];   // per query tile
-  uint64_t q_ready, drain;
+  uint64_t q_ready[2], drain;
   uint32_t tmem_base;
   int abort_flag;
   int maxpos[2];
@@ -480,6 +481,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// The eight softmax warps of query tile x.
+__device__ __forceinline__ void tile_sync(int x) { asm volatile("bar.sync %0, 256;" ::"r"(9 + x) : "memory"); }
 // The two warps that share 32 rows of query tile x (warps w and w + 4).
 __device__ __forceinline__ void pair_sync(int x, int quarter) {
   asm volatile("bar.sync %0, 64;" ::"r"(1 + x * 4 + quarter) : "memory");
@@ -488,6 +491,8 @@ constexpr int P_COL = 64;                 // P_x lives in columns [64, 128) of S
 }  // namespace pp
 
 __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid_constant__ CUtensorMap tm,
+                                                                    const __grid_constant__ CUtensorMap tq,
+                                                                    const __grid_constant__ CUtensorMap to,
                                                                     const PrefillParams p) {
   pdl_trigger();
   using namespace pp;
@@ -511,7 +516,8 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
       mbar_init(&ctl->o_done[i], 1);
       ctl->maxpos[i] = -1;
     }
-    mbar_init(&ctl->q_ready, 4 * ROWS);
+    mbar_init(&ctl->q_ready[0], 2 * ROWS + 1);
+    mbar_init(&ctl->q_ready[1], 2 * ROWS + 1);
     mbar_init(&ctl->drain, 1);
     ctl->abort_flag = 0;
     fence_mbar_init();
@@ -524,6 +530,21 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // A whole tile of consecutive tokens is a box of Q and of O (G heads of each token): TMA moves it. Through the load units
+  // its 32 KB took 4700 cycles: little of the L1 is left beside the shared memory, and a load in flight needs its lines.
+  const auto whole = [&](const int4& tl) { return tl.x == req && tl.z >= tpc && tl.w < 0; };
+  if (warp == 3 && lane == 0) {
+    for (int x = 0; x < 2; ++x) {
+      const int4 tl = x ? t1 : t0;
+      if (whole(tl)) {
+        mbar_arrive_expect_tx(&ctl->q_ready[x], TILE_B);
+        tma_load_3d(sm + OFF_Q + x * TILE_B, &tq, &ctl->q_ready[x], 0, kvh * G, tl.y);
+        tma_load_3d(sm + OFF_Q + x * TILE_B + HALF_B, &tq, &ctl->q_ready[x], 64, kvh * G, tl.y);
+      } else {
+        mbar_arrive(&ctl->q_ready[x]);
+      }
+    }
+  }
   // softmax thread: query tile x = (warp - 4) / 8, row = TMEM lane it may access = (warp % 4) * 32 + lane
   if (warp >= 4 && ((warp >> 2) & 1)) {
     const int x = (warp - 4) >> 3, r = (warp & 3) * 32 + lane;
@@ -593,7 +614,7 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
   } else if (warp == 1 && ntiles > 0) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {
-      bool ok = mbar_wait(&ctl->q_ready, 0, abort_flag);
+      bool ok = mbar_wait(&ctl->q_ready[0], 0, abort_flag) && mbar_wait(&ctl->q_ready[1], 0, abort_flag);
       const uint32_t idesc_s = idesc_bf16_f32(128, KT);
       const uint32_t idesc_o = idesc_bf16_f32(128, D) | (1u << 16);     // B (V) MN-major
       const int nt[2] = {nt0, nt1};
@@ -654,7 +675,8 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
     const int pos = ctl->pos[x][r];
     const int head = kvh * G + (r % G);
     const int my_tiles = x ? nt1 : nt0;
-    {
+    const bool boxed = whole(x ? t1 : t0);
+    if (!boxed) {
       // 16 of the pair's 32 Q rows -> shared memory (128-byte swizzle, dims halves in separate 16 KB halves of the tile),
       // two whole rows an instruction: a row per lane met 32 cache lines each time and took 5 us of a CTA (G divides ROWS,
       // so it is a power of two)
@@ -674,8 +696,8 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
         *reinterpret_cast<uint4*>(qd + (c >> 3) * HALF_B + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
       }
       fence_proxy_async_smem();
-      mbar_arrive(&ctl->q_ready);
     }
+    mbar_arrive(&ctl->q_ready[x]);
     const uint32_t s_col = tmem + x * KT + lane_off, o_col = tmem + 2 * KT + x * D + lane_off;
     const int key0 = (1 - part) * 64;
     float m_use = -INFINITY, l = 0.f;      // l: part 1's
@@ -831,8 +853,9 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
           }
         return sq;
       };
+      if (boxed && p.check == nullptr) fence_proxy_async_smem();
       pair_sync(x, quarter);             // (l was read, both halves of the rows wait in shared memory)
-      if (p.check == nullptr) {
+      if (p.check == nullptr && !boxed) {
         const int c = lane & 15;
 #pragma unroll 4
         for (int i = 0; i < 8; ++i) {
@@ -854,7 +877,26 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
         if (part == 1 && p.check == nullptr && p.row_sq != nullptr) atomicAdd(p.row_sq + tok, squares(ctl->sum[x][r]));
       }
     }
+    if (boxed && p.check == nullptr && my_tiles > 0) {
+      // every warp of the tile comes here, whether its waits held or not
+      ctl->stop[x][part][r] = stop;
+      tile_sync(x);
+      if (r == 0 && part == 0) {
+        bool all = true;
+        for (int i = 0; i < ROWS; i += 32) all = all && !ctl->stop[x][0][i];
+        if (all) {
+          tma_store_3d(&to, sm + OFF_Q + x * TILE_B, 0, kvh * G, (x ? t1 : t0).y);
+          tma_store_3d(&to, sm + OFF_Q + x * TILE_B + HALF_B, 64, kvh * G, (x ? t1 : t0).y);
+          bulk_commit();
+          bulk_wait_read0();
+        }
+      }
+    }
     if (p.check != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && r == 0 && x == 0 && part == 0) atomicAdd(p.check + 2, 1ull);
+  }
+  if (warp == 3 && lane == 0) {           // Q is there before the CTA ends, whether a product read it or not
+    mbar_wait(&ctl->q_ready[0], 0, nullptr);
+    mbar_wait(&ctl->q_ready[1], 0, nullptr);
   }
   tc_fence_before();
   __syncthreads();
@@ -1258,14 +1300,23 @@ static int launch_prefill(const void* q, void* o, const void* cache, long long n
   if (p.check != nullptr && row_idx == nullptr) return -1;
   CUtensorMap tm;
   if (!make_map_bf16_sw128(&tm, cache, num_blocks * 2 * nkv * PAGE, D, D, 64, PAGE)) return -2;
-  static bool attr = false;
-  if (!attr) {
-    cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pf::SMEM);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    e = cudaFuncSetAttribute(prefill_pp_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pp::SMEM);
-    if (e != cudaSuccess) return static_cast<int>(e);
-    attr = true;
+  // Q and O by token: the tiles say which tokens there are
+  CUtensorMap tq, to;
+  const int G = nq / nkv;
+  if (!make_map3_bf16_sw128(&tq, q, 1ll << 31, nq, D, 64, G, ROWS / G) ||
+      !make_map3_bf16_sw128(&to, o, 1ll << 31, nq, D, 64, G, ROWS / G))
+    return -2;
+  // the attributes belong to a device; one bit for each that has them (setting them twice does no harm)
+  static std::atomic<unsigned long long> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev > 63 || !(ready.load() >> dev & 1))) {
+    e = cudaFuncSetAttribute(prefill_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pf::SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(prefill_pp_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pp::SMEM);
+    if (e == cudaSuccess && dev <= 63) ready.fetch_or(1ull << dev);
   }
+  if (e != cudaSuccess) return static_cast<int>(e);
   static const bool pingpong = [] {
     const char* v = std::getenv("SDCGUARD_PREFILL_PINGPONG");
     return v == nullptr || v[0] != '0';
@@ -1282,7 +1333,7 @@ static int launch_prefill(const void* q, void* o, const void* cache, long long n
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = overlap ? 1 : 0;
-  return static_cast<int>(pingpong ? cudaLaunchKernelEx(&cfg, prefill_pp_kernel, tm, p)
+  return static_cast<int>(pingpong ? cudaLaunchKernelEx(&cfg, prefill_pp_kernel, tm, tq, to, p)
                                    : cudaLaunchKernelEx(&cfg, prefill_tc_kernel, tm, p));
 }
 

@@ -41,6 +41,23 @@ static inline bool make_map_bf16_sw128(CUtensorMap* m, const void* base, long lo
   return r == CUDA_SUCCESS;
 }
 
+// 3-D bf16 tensor [planes, rows, cols], contiguous, box {box_cols, box_rows, box_planes}, 128-byte swizzle (box_cols * 2
+// must be 128).
+static inline bool make_map3_bf16_sw128(CUtensorMap* m, const void* base, long long planes, long long rows, long long cols,
+                                        int box_cols, int box_rows, int box_planes) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) return false;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(planes)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(cols * 2), static_cast<cuuint64_t>(rows * cols * 2)};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows),
+                       static_cast<cuuint32_t>(box_planes)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS;
+}
+
 // 2-D tensor of 1-byte elements (fp8 data moved as bytes) [rows, cols] with row stride ld (bytes), box
 // {box_cols, box_rows}, 128-byte swizzle (box_cols must be 128).
 static inline bool make_map_u8_sw128(CUtensorMap* m, const void* base, long long rows, long long cols, long long ld,

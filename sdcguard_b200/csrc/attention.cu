@@ -425,12 +425,14 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
 }
 
 // ---------------------------------------------------------------------------------------------- prefill, ping-pong
-// Two query tiles per CTA that share their key / value tiles (consecutive tiles of one request, so they attend to
-// the same keys), so the tensor pipe always has one tile's MMAs to run while the other tile's softmax runs:
+// Two query tiles at a time that share their key / value tiles (consecutive tiles of one request, so they attend to
+// the same keys), so the tensor pipe always has one tile's MMAs to run while the other tile's softmax runs. A CTA goes
+// through pairs until none is left: it takes over those of CTAs that have not started.
 //   warps 0, 2  TMA: K and V pages of each 128-key tile into one of two stages (shared by both query tiles);
 //   warp 1      MMA, in the order PV0(j-1), S0(j), PV1(j-1), S1(j) for key tile j: S_x = Q_x K_j^T into TMEM,
 //               O_x += P_x V_{j-1} with P_x read from TMEM (the A operand of a tcgen05 MMA may live in tensor
 //               memory), so P never goes through shared memory;
+//   warp 3      the next pair: which it is, its rows' tokens and positions, its Q tiles by TMA;
 //   warps 4-11  softmax of query tile 0, warps 12-19 of query tile 1: two threads per row, of warps w and w + 4, each
 //               with half of the key tile: masked maximum (exchanged), conditional rescale of O (only when the
 //               reference maximum moves by more than 2^8), P = exp2(S - max) rounded to bf16 and written back
@@ -438,9 +440,12 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
 //               goes on from the first's sum while the MMAs run); at the end O / l
 // Bound by the chain of one tile: its softmax (2290 cycles a 128-key tile, 1600 of them the exponentials, which the two
 // tiles share the unit for) and the MMAs behind it (1500), against 2048 cycles for the exponentials or the MMAs of both
-// tiles alone. 8 x 2048 tokens, 16 / 8 heads: 190 us, 725 TFLOP/s, 0.43 of a dense bf16 product's rate. One thread a row:
-// 193 us; 37, 517 and 1 tokens behind 301, 0 and 1000 (32 / 8 heads) 26.8 against 23.1, 1 x 4096 (8 / 8) 79 against 74,
-// the other way 16 x 512 (16 / 8) 54 against 57, where CTAs are short and start slower.
+// tiles alone. 8 x 2048 tokens, 16 / 8 heads: 162 us, 849 TFLOP/s, 0.50 of a dense bf16 product's rate; 32 x 1024 210 us,
+// 16 x 512 43 us. A CTA for each pair took 182, 244 and 53 us: its start, first positions and Q took 10000 cycles. Pairs
+// ordered by kv head first, then length: 176, 202, 47. Q through the load units instead of TMA (little of the L1 is left
+// beside the shared memory, and a load in flight needs its lines): 190, 260, 57. One softmax thread a row: 193, 257, 54,
+// and 37, 517 and 1 tokens behind 301, 0 and 1000 (32 / 8 heads) 26.8 against 23.1. The other way 200, 77 and 130 tokens
+// behind 0, 40 and 16 (4 / 1), where there is one pair a CTA: 12.3 against 13.5.
 // TMEM: S_0, S_1, O_0, O_1 (128 columns each). S_x(j + 1) overwrites P_x(j) only after PV_x(j) in the MMA order
 // (tcgen05 MMAs of one thread run in issue order), and the commit that signals S_x(j) also covers PV_x(j - 1), so
 // the softmax may rescale O_x as soon as it sees S_x(j). Every decision is per row and key tiles start at absolute
@@ -452,18 +457,27 @@ constexpr int TILE_B = 2 * HALF_B;
 constexpr int OFF_Q = 0, OFF_K = 2 * TILE_B, OFF_V = 4 * TILE_B, OFF_CTL = 6 * TILE_B;
 constexpr float RESCALE_LOG2 = 8.f;
 constexpr int PG_BYTES = PAGE * D * 2;
+// A pair of query tiles, as warp 3 makes it known to the others.
+struct Pair {
+  int live, bx, kvh, req;
+  int nt[2];                                  // key tiles
+  int maxpos;
+  int tok[2][ROWS], pos[2][ROWS];             // a row's token and position, -1: none
+};
 struct Ctl {
+  uint4 next;                                 // the hardware's answer: the next pair (16-byte aligned)
   uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2];
-  uint64_t s_full[2], p_full[2], o_done[2];   // per query tile
-  uint64_t q_ready[2], drain;
+  uint64_t s_full[2], p_full[2], o_done[2], q_full[2], q_empty[2];   // per query tile
+  uint64_t pair_full[2], pair_empty[2];
+  uint64_t next_full, drain;
   uint32_t tmem_base;
   int abort_flag;
-  int maxpos[2];
-  int tok[2][ROWS];
-  int pos[2][ROWS];
-  float part_max[2][2][ROWS];               // [query tile][thread of the row]
-  float sum[2][ROWS];                       // passed from a row's first thread to its second
-  int stop[2][2][ROWS];
+  Pair pair[2];                               // this pair and the next, in turn
+  float part_max[2][2][ROWS];                 // [query tile][thread of the row]
+  float sum[2][ROWS], sq[2][ROWS];            // passed from a row's first thread to its second
+  float l[2][ROWS];                           // and back
+  int begin[2][2][ROWS], stop[2][2][ROWS];    // whether waits ran out, at a pair's begin and behind its key tiles
+  int bad[2][ROWS];                           // check mode: the first half's first difference
 };
 constexpr int SMEM = OFF_CTL + static_cast<int>(sizeof(Ctl)) + 1024;
 constexpr int THREADS = 128 + 4 * ROWS;   // warpgroup 0: warps 0, 2 TMA, warp 1 TMEM + MMA; warpgroups 1-4: softmax
@@ -476,13 +490,17 @@ __device__ __forceinline__ float2 fma2(uint32_t a, uint32_t b, float s, float d)
       : "r"(a), "r"(b), "f"(s), "f"(d));
   return r;
 }
+// 32 bytes, a whole sector, in one store.
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// The eight softmax warps of query tile x.
-__device__ __forceinline__ void tile_sync(int x) { asm volatile("bar.sync %0, 256;" ::"r"(9 + x) : "memory"); }
 // The two warps that share 32 rows of query tile x (warps w and w + 4).
 __device__ __forceinline__ void pair_sync(int x, int quarter) {
   asm volatile("bar.sync %0, 64;" ::"r"(1 + x * 4 + quarter) : "memory");
@@ -490,9 +508,31 @@ __device__ __forceinline__ void pair_sync(int x, int quarter) {
 constexpr int P_COL = 64;                 // P_x lives in columns [64, 128) of S_x (bf16 pairs)
 }  // namespace pp
 
+// Work of CTAs that have not started yet can be taken over: the hardware cancels such a CTA and names its index.
+__device__ __forceinline__ void request_next(uint4* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ bool next_index(const uint4* answer, int& x, int& y) {
+  uint32_t got, a = 0, b = 0;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t.reg .b32 c;\n\t"
+      "ld.shared.b128 h, [%3];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, c, _}, h;\n\t}\n"
+      : "=r"(got), "+r"(a), "+r"(b)
+      : "r"(smem_u32(answer))
+      : "memory");
+  x = static_cast<int>(a);
+  y = static_cast<int>(b);
+  return got != 0;
+}
 __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid_constant__ CUtensorMap tm,
                                                                     const __grid_constant__ CUtensorMap tq,
-                                                                    const __grid_constant__ CUtensorMap to,
+                                                                    const __grid_constant__ CUtensorMap tq1,
                                                                     const PrefillParams p) {
   pdl_trigger();
   using namespace pp;
@@ -502,9 +542,6 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.nq / p.nkv;
   const int tpc = ROWS / G;
-  const int kvh = blockIdx.y;
-  const int4 t0 = p.tiles[2 * blockIdx.x], t1 = p.tiles[2 * blockIdx.x + 1];
-  const int req = t0.x;
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl->k_full[i], 1);
@@ -514,10 +551,12 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
       mbar_init(&ctl->s_full[i], 1);
       mbar_init(&ctl->p_full[i], 2 * ROWS);
       mbar_init(&ctl->o_done[i], 1);
-      ctl->maxpos[i] = -1;
+      mbar_init(&ctl->q_full[i], 1);
+      mbar_init(&ctl->q_empty[i], 1);
+      mbar_init(&ctl->pair_full[i], 1);
+      mbar_init(&ctl->pair_empty[i], THREADS / 32 - 1);
     }
-    mbar_init(&ctl->q_ready[0], 2 * ROWS + 1);
-    mbar_init(&ctl->q_ready[1], 2 * ROWS + 1);
+    mbar_init(&ctl->next_full, 1);
     mbar_init(&ctl->drain, 1);
     ctl->abort_flag = 0;
     fence_mbar_init();
@@ -530,45 +569,101 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // A whole tile of consecutive tokens is a box of Q and of O (G heads of each token): TMA moves it. Through the load units
-  // its 32 KB took 4700 cycles: little of the L1 is left beside the shared memory, and a load in flight needs its lines.
-  const auto whole = [&](const int4& tl) { return tl.x == req && tl.z >= tpc && tl.w < 0; };
-  if (warp == 3 && lane == 0) {
-    for (int x = 0; x < 2; ++x) {
-      const int4 tl = x ? t1 : t0;
-      if (whole(tl)) {
-        mbar_arrive_expect_tx(&ctl->q_ready[x], TILE_B);
-        tma_load_3d(sm + OFF_Q + x * TILE_B, &tq, &ctl->q_ready[x], 0, kvh * G, tl.y);
-        tma_load_3d(sm + OFF_Q + x * TILE_B + HALF_B, &tq, &ctl->q_ready[x], 64, kvh * G, tl.y);
-      } else {
-        mbar_arrive(&ctl->q_ready[x]);
-      }
-    }
-  }
-  // softmax thread: query tile x = (warp - 4) / 8, row = TMEM lane it may access = (warp % 4) * 32 + lane
-  if (warp >= 4 && ((warp >> 2) & 1)) {
-    const int x = (warp - 4) >> 3, r = (warp & 3) * 32 + lane;
-    const int4 tl = x ? t1 : t0;
-    const int ti = r / G;
-    int tok = -1;
-    if (tl.x == req && ti < tl.z && ti < tpc) tok = tl.w >= 0 ? p.row_idx[tl.w + ti] : tl.y + ti;
-    ctl->tok[x][r] = tok;
-    int ps = tok >= 0 ? p.pos[tok] : -1;
-    if (ps >= p.limit) ps = -1;
-    ctl->pos[x][r] = ps;
-    const int top = __reduce_max_sync(0xffffffffu, ps);
-    if (lane == 0 && top >= 0) atomicMax(&ctl->maxpos[x], top);
-  }
-  __syncthreads();
-  const int nt0 = ctl->maxpos[0] >= 0 ? ctl->maxpos[0] / KT + 1 : 0;
-  const int nt1 = ctl->maxpos[1] >= 0 ? ctl->maxpos[1] / KT + 1 : 0;
-  const int ntiles = max(nt0, nt1);
-  const int maxpos = max(ctl->maxpos[0], ctl->maxpos[1]);
   const uint32_t tmem = ctl->tmem_base;
   volatile int* abort_flag = &ctl->abort_flag;
-  const int* bt = p.block_table + static_cast<long long>(req) * p.max_pages;
+  // Pair n of this CTA: null where a wait ran out (`live` is 0 behind the last pair).
+  const auto pair_of = [&](int n) -> const Pair* {
+    return mbar_wait(&ctl->pair_full[n & 1], (n >> 1) & 1, abort_flag) ? &ctl->pair[n & 1] : nullptr;
+  };
 
-  if ((warp == 0 || warp == 2) && ntiles > 0) {
+  if (warp == 3) {
+    // ------------------------------------------------------------ pairs: which, their rows, and Q
+    // One pair ahead of the others, in the order in which the CTAs would have started.
+    bool ok = true;
+    int gx = blockIdx.x, gy = blockIdx.y, loads[2] = {0, 0};
+    bool live = true;
+    for (int n = 0;; ++n) {
+      Pair& pr = ctl->pair[n & 1];
+      // the launch order, kv heads fastest: the longest pairs of all heads come first
+      const int at = gx + static_cast<int>(gridDim.x) * gy, bx = at / p.nkv, kvh = at % p.nkv;
+      if (n >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&ctl->pair_empty[n & 1], ((n - 2) >> 1) & 1, abort_flag));
+      if (!ok) break;
+      int4 tl[2];
+      int top = -1;
+      if (live) {
+        tl[0] = p.tiles[2 * bx];
+        tl[1] = p.tiles[2 * bx + 1];
+        const int req = tl[0].x;
+        for (int x = 0; x < 2; ++x) {
+          int tok[4], ps[4], mx = -1;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int ti = (lane + 32 * i) / G;
+            tok[i] = -1;
+            if (tl[x].x == req && ti < tl[x].z && ti < tpc) tok[i] = tl[x].w >= 0 ? p.row_idx[tl[x].w + ti] : tl[x].y + ti;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ps[i] = tok[i] >= 0 ? p.pos[tok[i]] : -1;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (ps[i] >= p.limit || ps[i] < 0) ps[i] = -1;
+            mx = max(mx, ps[i]);
+            pr.tok[x][lane + 32 * i] = tok[i];
+            pr.pos[x][lane + 32 * i] = ps[i];
+          }
+          mx = __reduce_max_sync(0xffffffffu, mx);
+          if (lane == 0) pr.nt[x] = mx >= 0 ? mx / KT + 1 : 0;
+          top = max(top, mx);
+        }
+      }
+      if (lane == 0) {
+        pr.live = live;
+        pr.bx = bx;
+        pr.kvh = kvh;
+        pr.req = live ? tl[0].x : 0;
+        pr.maxpos = top;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->pair_full[n & 1]);
+      if (!live) break;
+      // Q_x once S_x of the pair before is formed. A whole tile of consecutive tokens is one box (G heads of each token) for
+      // each half of the dims, else every token has its own; rows without a token keep what was there (they are masked).
+      for (int x = 0; x < 2; ++x) {
+        if (n >= 1) ok = __all_sync(0xffffffffu, mbar_wait(&ctl->q_empty[x], (n - 1) & 1, abort_flag));
+        if (!ok) break;
+        const int count = tl[x].x == tl[0].x ? max(0, min(tl[x].z, tpc)) : 0;
+        uint8_t* qd = sm + OFF_Q + x * TILE_B;
+        if (lane == 0) {
+          if (count > 0) mbar_arrive_expect_tx(&ctl->q_full[x], count * G * D * 2);
+          else mbar_arrive(&ctl->q_full[x]);
+        }
+        __syncwarp();
+        loads[x] = n + 1;
+        if (count == tpc && tl[x].w < 0) {
+          if (lane < 2) tma_load_3d(qd + lane * HALF_B, &tq, &ctl->q_full[x], lane * 64, kvh * G, tl[x].y);
+        } else {
+          for (int i = lane; i < 2 * count; i += 32)
+            tma_load_3d(qd + (i & 1) * HALF_B + (i >> 1) * G * 128, &tq1, &ctl->q_full[x], (i & 1) * 64, kvh * G,
+                        pr.tok[x][(i >> 1) * G]);
+        }
+      }
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&ctl->next_full, 16);
+        request_next(&ctl->next, &ctl->next_full);
+      }
+      __syncwarp();
+      ok = __all_sync(0xffffffffu, mbar_wait(&ctl->next_full, n & 1, nullptr));
+      if (!ok) break;
+      live = next_index(&ctl->next, gx, gy);
+      fence_proxy_async_smem();
+      __syncwarp();
+    }
+    if (!ok && lane == 0) *abort_flag = 1;
+    // what is on its way has to land before the CTA ends
+    for (int x = 0; x < 2; ++x)
+      if (loads[x] > 0) mbar_wait(&ctl->q_full[x], (loads[x] - 1) & 1, nullptr);
+  } else if (warp == 0 || warp == 2) {
     // ------------------------------------------------------------ TMA producers (all 32 lanes issue): warp 0 K, warp 2 V
     // K's stage is free once S of both query tiles is formed, a softmax and a product before V's: taken apart, the next
     // K is on its way that much earlier (with one barrier for both, the MMAs waited for K in half of the time)
@@ -577,85 +672,103 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
     uint64_t* full = kv ? ctl->v_full : ctl->k_full;
     uint64_t* empty = kv ? ctl->v_empty : ctl->k_empty;
     bool ok = true;
-    int last = -1;
-    for (int j = 0; j < ntiles && ok; ++j) {
-      const int st = j & 1;
-      bool got = true;
-      if (lane == 0) got = mbar_wait(&empty[st], ((j >> 1) & 1u) ^ 1u, abort_flag);
-      if (!__shfl_sync(0xffffffffu, got ? 1 : 0, 0)) {
-        ok = false;
-        break;
-      }
-      const int npg = min(KT / PAGE, maxpos / PAGE - j * (KT / PAGE) + 1);
-      uint8_t* buf = sm + (kv ? OFF_V : OFF_K) + st * TILE_B;
-      if (kv && npg < KT / PAGE) {
-        // the weights of keys past the last page are zero, but stale shared memory could hold NaN patterns
-        for (int i = lane; i < (KT - npg * PAGE) * 16; i += 32) {
-          const int rr = npg * PAGE + (i >> 4), c = i & 15;
-          *reinterpret_cast<uint4*>(buf + (c >> 3) * HALF_B + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+    int kt = 0;                           // key tiles so far, over all pairs
+    for (int n = 0; ok; ++n) {
+      const Pair* pr = pair_of(n);
+      ok = __all_sync(0xffffffffu, pr != nullptr);
+      if (!ok || !pr->live) break;
+      const int ntiles = max(pr->nt[0], pr->nt[1]), maxpos = pr->maxpos, kvh = pr->kvh;
+      const int* bt = p.block_table + static_cast<long long>(pr->req) * p.max_pages;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->pair_empty[n & 1]);
+      for (int j = 0; j < ntiles; ++j, ++kt) {
+        const int st = kt & 1;
+        bool got = true;
+        if (lane == 0) got = mbar_wait(&empty[st], ((kt >> 1) & 1u) ^ 1u, abort_flag);
+        if (!__shfl_sync(0xffffffffu, got ? 1 : 0, 0)) {
+          ok = false;
+          break;
         }
-        fence_proxy_async_smem();
+        const int npg = min(KT / PAGE, maxpos / PAGE - j * (KT / PAGE) + 1);
+        uint8_t* buf = sm + (kv ? OFF_V : OFF_K) + st * TILE_B;
+        if (kv && npg < KT / PAGE) {
+          // the weights of keys past the last page are zero, but stale shared memory could hold NaN patterns
+          for (int i = lane; i < (KT - npg * PAGE) * 16; i += 32) {
+            const int rr = npg * PAGE + (i >> 4), c = i & 15;
+            *reinterpret_cast<uint4*>(buf + (c >> 3) * HALF_B + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], npg * PG_BYTES);
+        __syncwarp();
+        if (lane < 2 * npg) {
+          const int pg = lane >> 1, half = lane & 1;
+          const long long blk = bt[j * (KT / PAGE) + pg];
+          const int row = static_cast<int>(((blk * 2 + kv) * p.nkv + kvh) * PAGE);
+          tma_load_2d(buf + half * HALF_B + pg * PAGE * 128, &tm, &full[st], half * 64, row);
+        }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive_expect_tx(&full[st], npg * PG_BYTES);
-      __syncwarp();
-      if (lane < 2 * npg) {
-        const int pg = lane >> 1, half = lane & 1;
-        const long long blk = bt[j * (KT / PAGE) + pg];
-        const int row = static_cast<int>(((blk * 2 + kv) * p.nkv + kvh) * PAGE);
-        tma_load_2d(buf + half * HALF_B + pg * PAGE * 128, &tm, &full[st], half * 64, row);
-      }
-      last = j;
     }
-    if (!ok && lane == 0) {
-      *abort_flag = 1;
-      for (int j = last > 0 ? last - 1 : 0; j <= last; ++j) mbar_wait(&full[j & 1], (j >> 1) & 1u, nullptr);
+    if (!ok) {
+      if (lane == 0) *abort_flag = 1;
+      for (int j = kt > 1 ? kt - 2 : 0; j < kt; ++j) mbar_wait(&full[j & 1], (j >> 1) & 1u, nullptr);
     }
-  } else if (warp == 1 && ntiles > 0) {
+  } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {
-      bool ok = mbar_wait(&ctl->q_ready[0], 0, abort_flag) && mbar_wait(&ctl->q_ready[1], 0, abort_flag);
+      bool ok = true;
       const uint32_t idesc_s = idesc_bf16_f32(128, KT);
       const uint32_t idesc_o = idesc_bf16_f32(128, D) | (1u << 16);     // B (V) MN-major
-      const int nt[2] = {nt0, nt1};
-      for (int j = 0; j <= ntiles && ok; ++j) {
-        if (j < ntiles) {
-          ok = mbar_wait(&ctl->k_full[j & 1], (j >> 1) & 1u, abort_flag);
-          if (!ok) break;
-        }
-        if (j >= 1) {
-          ok = mbar_wait(&ctl->v_full[(j - 1) & 1], ((j - 1) >> 1) & 1u, abort_flag);
-          if (!ok) break;
-        }
-        tc_fence_after();
+      int kt = 0, turn[2] = {0, 0};       // key tiles before this pair, turns of P_x so far
+      for (int n = 0; ok; ++n) {
+        const Pair* pr = pair_of(n);
+        ok = pr != nullptr;
+        if (!ok || !pr->live) break;
+        const int nt[2] = {pr->nt[0], pr->nt[1]};
+        const int ntiles = max(nt[0], nt[1]);
+        mbar_arrive(&ctl->pair_empty[n & 1]);
         for (int x = 0; x < 2 && ok; ++x) {
-          const uint32_t s_col = tmem + x * KT, o_col = tmem + 2 * KT + x * D;
-          if (j >= 1 && j - 1 < nt[x]) {
-            // O_x += P_x(j-1) V(j-1): P_x in columns [64, 128) of S_x (bf16 pairs), 8 columns per K = 16 step
-            ok = mbar_wait(&ctl->p_full[x], (j - 1) & 1u, abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t va = smem_u32(sm + OFF_V + ((j - 1) & 1) * TILE_B);
-#pragma unroll
-            for (int ks = 0; ks < KT / 16; ++ks) {
-              const uint64_t bd = umma_desc_sw128_mn(va + ks * 2048, HALF_B, 1024);
-              umma_f16_tmem_a(o_col, s_col + P_COL + ks * 8, bd, idesc_o, (j - 1 > 0 || ks > 0) ? 1u : 0u);
-            }
-            if (j - 1 == nt[x] - 1) umma_commit(&ctl->o_done[x]);
-          }
-          if (j < nt[x]) {
-            const uint32_t qa = smem_u32(sm + OFF_Q + x * TILE_B);
-            const uint32_t ka = smem_u32(sm + OFF_K + (j & 1) * TILE_B);
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-              const uint32_t off = (ks >> 2) * HALF_B + (ks & 3) * 32;
-              umma_f16(s_col, umma_desc_sw128(qa + off), umma_desc_sw128(ka + off), idesc_s, ks ? 1u : 0u);
-            }
-            umma_commit(&ctl->s_full[x]);
-          }
+          ok = mbar_wait(&ctl->q_full[x], n & 1, abort_flag);
+          if (ok && nt[x] == 0) mbar_arrive(&ctl->q_empty[x]);
         }
-        if (ok && j < ntiles) umma_commit(&ctl->k_empty[j & 1]);
-        if (ok && j >= 1) umma_commit(&ctl->v_empty[(j - 1) & 1]);
+        for (int j = 0; j <= ntiles && ntiles > 0 && ok; ++j) {
+          const int now = kt + j, was = kt + j - 1;
+          if (j < ntiles) ok = mbar_wait(&ctl->k_full[now & 1], (now >> 1) & 1u, abort_flag);
+          if (ok && j >= 1) ok = mbar_wait(&ctl->v_full[was & 1], (was >> 1) & 1u, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          for (int x = 0; x < 2 && ok; ++x) {
+            const uint32_t s_col = tmem + x * KT, o_col = tmem + 2 * KT + x * D;
+            if (j >= 1 && j - 1 < nt[x]) {
+              // O_x += P_x(j-1) V(j-1): P_x in columns [64, 128) of S_x (bf16 pairs), 8 columns per K = 16 step
+              ok = mbar_wait(&ctl->p_full[x], turn[x]++ & 1u, abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t va = smem_u32(sm + OFF_V + (was & 1) * TILE_B);
+#pragma unroll
+              for (int ks = 0; ks < KT / 16; ++ks) {
+                const uint64_t bd = umma_desc_sw128_mn(va + ks * 2048, HALF_B, 1024);
+                umma_f16_tmem_a(o_col, s_col + P_COL + ks * 8, bd, idesc_o, (j - 1 > 0 || ks > 0) ? 1u : 0u);
+              }
+              if (j - 1 == nt[x] - 1) umma_commit(&ctl->o_done[x]);
+            }
+            if (j < nt[x]) {
+              const uint32_t qa = smem_u32(sm + OFF_Q + x * TILE_B);
+              const uint32_t ka = smem_u32(sm + OFF_K + (now & 1) * TILE_B);
+#pragma unroll
+              for (int ks = 0; ks < D / 16; ++ks) {
+                const uint32_t off = (ks >> 2) * HALF_B + (ks & 3) * 32;
+                umma_f16(s_col, umma_desc_sw128(qa + off), umma_desc_sw128(ka + off), idesc_s, ks ? 1u : 0u);
+              }
+              umma_commit(&ctl->s_full[x]);
+              if (j == nt[x] - 1) umma_commit(&ctl->q_empty[x]);
+            }
+          }
+          if (ok && j < ntiles) umma_commit(&ctl->k_empty[now & 1]);
+          if (ok && j >= 1) umma_commit(&ctl->v_empty[was & 1]);
+        }
+        kt += ntiles;
       }
       if (!ok) {
         record_error(nullptr, ERR_TIMEOUT_MMA);
@@ -664,239 +777,196 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
         mbar_wait(&ctl->drain, 0, nullptr);
       }
     }
-  } else if (warp >= 4) {
+  } else {
     // ------------------------------------------------------------ softmax / output: two threads a row of tile x
     // part 0: keys [64, 128) of each key tile and dims [0, 64) of O; part 1: keys [0, 64), dims [64, 128). Both threads
     // of a row go through every pair_sync, whatever fails: a wait that ran out sets the abort flag and goes on.
     const int x = (warp - 4) >> 3, part = ((warp >> 2) & 1) ^ 1, quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const int tok = ctl->tok[x][r];
-    const int pos = ctl->pos[x][r];
-    const int head = kvh * G + (r % G);
-    const int my_tiles = x ? nt1 : nt0;
-    const bool boxed = whole(x ? t1 : t0);
-    if (!boxed) {
-      // 16 of the pair's 32 Q rows -> shared memory (128-byte swizzle, dims halves in separate 16 KB halves of the tile),
-      // two whole rows an instruction: a row per lane met 32 cache lines each time and took 5 us of a CTA (G divides ROWS,
-      // so it is a power of two)
-      uint8_t* qd = sm + OFF_Q + x * TILE_B;
-      const int c = lane & 15;
-      uint4 v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int rr = quarter * 32 + part * 16 + 2 * i + (lane >> 4), tk = ctl->tok[x][rr];
-        v[i] = tk >= 0 ? *reinterpret_cast<const uint4*>(
-                             p.q + (static_cast<long long>(tk) * p.nq + kvh * G + (rr & (G - 1))) * D + c * 8)
-                       : make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int rr = quarter * 32 + part * 16 + 2 * i + (lane >> 4);
-        *reinterpret_cast<uint4*>(qd + (c >> 3) * HALF_B + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v[i];
-      }
-      fence_proxy_async_smem();
-    }
-    mbar_arrive(&ctl->q_ready[x]);
     const uint32_t s_col = tmem + x * KT + lane_off, o_col = tmem + 2 * KT + x * D + lane_off;
     const int key0 = (1 - part) * 64;
-    float m_use = -INFINITY, l = 0.f;      // l: part 1's
-    bool stop = false;
-    for (int j = 0; j < my_tiles; ++j) {
-      if (!mbar_wait(&ctl->s_full[x], j & 1u, abort_flag)) {
+    int turn = 0, outs = 0;               // turns of S_x and O_x so far
+    for (int n = 0;; ++n) {
+      const Pair* pr = pair_of(n);
+      bool stop = pr == nullptr;
+      if (stop) *abort_flag = 1;
+      // both warps give up, or neither
+      ctl->begin[x][part][r] = stop;
+      pair_sync(x, quarter);
+      if (__any_sync(0xffffffffu, stop || ctl->begin[x][part ^ 1][r])) break;
+      pr = &ctl->pair[n & 1];
+      if (!pr->live) break;
+      const int tok = pr->tok[x][r], pos = pr->pos[x][r], my_tiles = pr->nt[x];
+      float m_use = -INFINITY, l = 0.f;   // l: part 1's
+      for (int j = 0; j < my_tiles; ++j) {
+        if (!mbar_wait(&ctl->s_full[x], turn++ & 1u, abort_flag)) {
+          *abort_flag = 1;
+          stop = true;
+        }
+        __syncwarp();
+        tc_fence_after();
+        // This half of the S row, and the maximum over both. P (bf16 pairs) goes to columns [64, 128): the weights of keys
+        // [64, 128) over columns [96, 128) and those of keys [0, 64) over [64, 96), written after part 0 read the S
+        // values under them (pair_sync).
+        const int lim = pos - j * KT - key0;      // keys [0, lim] of this half are visible to the row
+        // every key visible to every row of the warp (all but a prompt's last tiles): no masks, the same values
+        const bool full = __all_sync(0xffffffffu, lim >= 63);
+        uint32_t v[2][32];
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (a maximum does not depend on the order)
+        tmem_ld32(s_col + key0, v[0]);
+        tmem_ld32(s_col + key0 + 32, v[1]);
+        tmem_wait_ld();
+        if (full) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; i += 2)
+              mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], u32_as_f32(v[c][i]), u32_as_f32(v[c][i + 1]));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i <= lim) mx4[i & 3] = fmaxf(mx4[i & 3], u32_as_f32(v[c][i]));
+        }
+        float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        ctl->part_max[x][part][r] = mx;
+        tc_fence_before();
+        pair_sync(x, quarter);
+        tc_fence_after();
+        mx = fmaxf(mx, ctl->part_max[x][part ^ 1][r]);
+        mx *= p.scale_log2;                // scale > 0: the maximum commutes with it
+        float alpha = 1.f;
+        if (mx > -INFINITY && (m_use == -INFINITY || mx > m_use + RESCALE_LOG2)) {
+          alpha = m_use == -INFINITY ? 1.f : ex2(m_use - mx);
+          l *= alpha;
+          m_use = mx;
+        }
+        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+          // PV_x(j-1) is complete (the commit of S_x(j) covers it): rescale this half of the row of O_x
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o_col + part * 64 + c * 16, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(u32_as_f32(o[i]) * alpha);
+            tmem_st16(o_col + part * 64 + c * 16, o);
+          }
+        }
+        const bool live = m_use > -INFINITY;
+        const bool plain = full && __all_sync(0xffffffffu, live);
+        uint32_t pk[2][16];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (plain) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 e = fma2(v[c][i], v[c][i + 1], p.scale_log2, -m_use);
+              pk[c][i >> 1] = pack_bf16x2(ex2(e.x), ex2(e.y));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const int key = c * 32 + i;
+              const float p0 = (key <= lim && live) ? ex2(u32_as_f32(v[c][i]) * p.scale_log2 - m_use) : 0.f;
+              const float p1 = (key + 1 <= lim && live) ? ex2(u32_as_f32(v[c][i + 1]) * p.scale_log2 - m_use) : 0.f;
+              pk[c][i >> 1] = pack_bf16x2(p0, p1);
+            }
+          }
+          tmem_st16(s_col + P_COL + (1 - part) * 32 + c * 16, pk[c]);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&ctl->p_full[x]);
+        // the row's sum over keys [64, 128), then [0, 64), one order whoever holds them
+        const auto add = [&](float s) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s += u32_as_f32(pk[c][i] << 16) + u32_as_f32(pk[c][i] & 0xffff0000u);
+          return s;
+        };
+        if (part == 0) ctl->sum[x][r] = add(0.f);
+        pair_sync(x, quarter);
+        if (part == 1) l += add(ctl->sum[x][r]);
+      }
+      if (my_tiles > 0 && !mbar_wait(&ctl->o_done[x], outs++ & 1u, abort_flag)) {
         *abort_flag = 1;
         stop = true;
       }
-      __syncwarp();
-      tc_fence_after();
-      // This half of the S row, and the maximum over both. P (bf16 pairs) goes to columns [64, 128): the weights of keys
-      // [64, 128) over columns [96, 128) and those of keys [0, 64) over [64, 96), written after part 0 read the S
-      // values under them (pair_sync).
-      const int lim = pos - j * KT - key0;      // keys [0, lim] of this half are visible to the row
-      // every key visible to every row of the warp (all but a prompt's last tiles): no masks, the same values
-      const bool full = __all_sync(0xffffffffu, lim >= 63);
-      uint32_t v[2][32];
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // (a maximum does not depend on the order)
-      tmem_ld32(s_col + key0, v[0]);
-      tmem_ld32(s_col + key0 + 32, v[1]);
-      tmem_wait_ld();
-      if (full) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; i += 2)
-            mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], u32_as_f32(v[c][i]), u32_as_f32(v[c][i + 1]));
-      } else {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c * 32 + i <= lim) mx4[i & 3] = fmaxf(mx4[i & 3], u32_as_f32(v[c][i]));
-      }
-      float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-      ctl->part_max[x][part][r] = mx;
-      tc_fence_before();
+      ctl->stop[x][part][r] = stop;
+      if (part == 1) ctl->l[x][r] = l;
       pair_sync(x, quarter);
-      tc_fence_after();
-      mx = fmaxf(mx, ctl->part_max[x][part ^ 1][r]);
-      mx *= p.scale_log2;                // scale > 0: the maximum commutes with it
-      float alpha = 1.f;
-      if (mx > -INFINITY && (m_use == -INFINITY || mx > m_use + RESCALE_LOG2)) {
-        alpha = m_use == -INFINITY ? 1.f : ex2(m_use - mx);
-        l *= alpha;
-        m_use = mx;
-      }
-      if (__any_sync(0xffffffffu, alpha != 1.f)) {
-        // PV_x(j-1) is complete (the commit of S_x(j) covers it): rescale this half of the row of O_x
+      stop = __any_sync(0xffffffffu, stop || ctl->stop[x][part ^ 1][r]);
+      const int bx = pr->bx, kvh = pr->kvh;
+      if (!stop && my_tiles > 0) {
+        const int head = kvh * G + (r % G);
+        tc_fence_after();
+        l = ctl->l[x][r];
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        __nv_bfloat16* orow = p.o + (static_cast<long long>(tok < 0 ? 0 : tok) * p.nq + head) * D;
+        int bad = -1;
+        uint32_t w[2][16];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[16];
-          tmem_ld16(o_col + part * 64 + c * 16, o);
+        for (int c = 0; c < 2; ++c) {
+          uint32_t v[32];
+          tmem_ld32(o_col + part * 64 + c * 32, v);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(u32_as_f32(o[i]) * alpha);
-          tmem_st16(o_col + part * 64 + c * 16, o);
-        }
-      }
-      const bool live = m_use > -INFINITY;
-      const bool plain = full && __all_sync(0xffffffffu, live);
-      uint32_t pk[2][16];
+          for (int i = 0; i < 16; ++i) w[c][i] = pack_bf16x2(u32_as_f32(v[2 * i]) * inv, u32_as_f32(v[2 * i + 1]) * inv);
+          if (p.check == nullptr) {
+            if (tok >= 0) {
+              store32(orow + part * 64 + c * 32, &w[c][0]);
+              store32(orow + part * 64 + c * 32 + 16, &w[c][8]);
+            }
+          } else if (tok >= 0) {
+            uint4* dst = reinterpret_cast<uint4*>(orow + part * 64 + c * 32);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        if (plain) {
+            for (int i = 0; i < 4; ++i) {
+              const uint4 nv = make_uint4(w[c][4 * i], w[c][4 * i + 1], w[c][4 * i + 2], w[c][4 * i + 3]);
+              if (bad < 0) {
+                const uint4 ov = dst[i];
+                const uint32_t a[4] = {nv.x, nv.y, nv.z, nv.w}, b[4] = {ov.x, ov.y, ov.z, ov.w};
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float2 e = fma2(v[c][i], v[c][i + 1], p.scale_log2, -m_use);
-            pk[c][i >> 1] = pack_bf16x2(ex2(e.x), ex2(e.y));
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const int key = c * 32 + i;
-            const float p0 = (key <= lim && live) ? ex2(u32_as_f32(v[c][i]) * p.scale_log2 - m_use) : 0.f;
-            const float p1 = (key + 1 <= lim && live) ? ex2(u32_as_f32(v[c][i + 1]) * p.scale_log2 - m_use) : 0.f;
-            pk[c][i >> 1] = pack_bf16x2(p0, p1);
-          }
-        }
-        tmem_st16(s_col + P_COL + (1 - part) * 32 + c * 16, pk[c]);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&ctl->p_full[x]);
-      // the row's sum over keys [64, 128), then [0, 64), one order whoever holds them
-      const auto add = [&](float s) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s += u32_as_f32(pk[c][i] << 16) + u32_as_f32(pk[c][i] & 0xffff0000u);
-        return s;
-      };
-      if (part == 0) ctl->sum[x][r] = add(0.f);
-      pair_sync(x, quarter);
-      if (part == 1) l += add(ctl->sum[x][r]);
-    }
-    if (my_tiles > 0 && !mbar_wait(&ctl->o_done[x], 0, abort_flag)) {
-      *abort_flag = 1;
-      stop = true;
-    }
-    // both warps give up, or neither
-    ctl->stop[x][part][r] = stop;
-    if (part == 1) ctl->sum[x][r] = l;
-    pair_sync(x, quarter);
-    stop = __any_sync(0xffffffffu, stop || ctl->stop[x][part ^ 1][r]);
-    if (!stop && my_tiles > 0) {
-      tc_fence_after();
-      l = ctl->sum[x][r];
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      __nv_bfloat16* orow = p.o + (static_cast<long long>(tok < 0 ? 0 : tok) * p.nq + head) * D;
-      int bad = -1;
-      uint32_t w[2][16];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t v[32];
-        tmem_ld32(o_col + part * 64 + c * 32, v);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) w[c][i] = pack_bf16x2(u32_as_f32(v[2 * i]) * inv, u32_as_f32(v[2 * i + 1]) * inv);
-        if (p.check == nullptr) {
-          // through the Q tile, which the MMAs are done with, to whole rows
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int ch = c * 4 + i;
-            *reinterpret_cast<uint4*>(sm + OFF_Q + x * TILE_B + part * HALF_B + r * 128 + ((ch ^ (r & 7)) << 4)) =
-                make_uint4(w[c][4 * i], w[c][4 * i + 1], w[c][4 * i + 2], w[c][4 * i + 3]);
-          }
-        } else if (tok >= 0) {
-          uint4* dst = reinterpret_cast<uint4*>(orow + part * 64 + c * 32);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint4 nv = make_uint4(w[c][4 * i], w[c][4 * i + 1], w[c][4 * i + 2], w[c][4 * i + 3]);
-            if (bad < 0) {
-              const uint4 ov = dst[i];
-              const uint32_t a[4] = {nv.x, nv.y, nv.z, nv.w}, b[4] = {ov.x, ov.y, ov.z, ov.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int dd = bf16x2_diff(a[e], b[e]);
-                if (bad < 0 && dd >= 0) bad = part * 64 + c * 32 + i * 8 + e * 2 + dd;
+                for (int e = 0; e < 4; ++e) {
+                  const int dd = bf16x2_diff(a[e], b[e]);
+                  if (bad < 0 && dd >= 0) bad = part * 64 + c * 32 + i * 8 + e * 2 + dd;
+                }
               }
             }
           }
         }
-      }
-      const auto squares = [&](float sq) {
+        const auto squares = [&](float sq) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[c][i]));
-            sq = fmaf(f.x, f.x, fmaf(f.y, f.y, sq));
+            for (int i = 0; i < 16; ++i) {
+              const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[c][i]));
+              sq = fmaf(f.x, f.x, fmaf(f.y, f.y, sq));
+            }
+          return sq;
+        };
+        if (p.check != nullptr || p.row_sq != nullptr) {
+          if (part == 0) {
+            ctl->sq[x][r] = squares(0.f);
+            ctl->bad[x][r] = bad;
           }
-        return sq;
-      };
-      if (boxed && p.check == nullptr) fence_proxy_async_smem();
-      pair_sync(x, quarter);             // (l was read, both halves of the rows wait in shared memory)
-      if (p.check == nullptr && !boxed) {
-        const int c = lane & 15;
-#pragma unroll 4
-        for (int i = 0; i < 8; ++i) {
-          const int rr = quarter * 32 + part * 16 + 2 * i + (lane >> 4), tk = ctl->tok[x][rr];
-          const uint4 v = *reinterpret_cast<const uint4*>(sm + OFF_Q + x * TILE_B + (c >> 3) * HALF_B + rr * 128 +
-                                                          (((c & 7) ^ (rr & 7)) << 4));
-          if (tk >= 0)
-            *reinterpret_cast<uint4*>(p.o + (static_cast<long long>(tk) * p.nq + kvh * G + (rr & (G - 1))) * D + c * 8) = v;
+          pair_sync(x, quarter);
+          if (tok >= 0) {
+            if (p.check != nullptr && bad >= 0 && (part == 0 || ctl->bad[x][r] < 0))      // the row's first difference
+              report_replay_mismatch(p.check, static_cast<unsigned long long>(tok) * p.nq * D + head * D + bad);
+            if (part == 1 && p.check == nullptr) atomicAdd(p.row_sq + tok, squares(ctl->sq[x][r]));
+          }
         }
       }
-      if (part == 0) {
-        ctl->sum[x][r] = squares(0.f);
-        ctl->stop[x][0][r] = bad;
-      }
-      pair_sync(x, quarter);
-      if (tok >= 0) {
-        if (p.check != nullptr && bad >= 0 && (part == 0 || ctl->stop[x][0][r] < 0))      // the row's first difference
-          report_replay_mismatch(p.check, static_cast<unsigned long long>(tok) * p.nq * D + head * D + bad);
-        if (part == 1 && p.check == nullptr && p.row_sq != nullptr) atomicAdd(p.row_sq + tok, squares(ctl->sum[x][r]));
-      }
+      if (p.check != nullptr && bx == 0 && kvh == 0 && r == 0 && x == 0 && part == 0) atomicAdd(p.check + 2, 1ull);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->pair_empty[n & 1]);
+      if (stop) break;
     }
-    if (boxed && p.check == nullptr && my_tiles > 0) {
-      // every warp of the tile comes here, whether its waits held or not
-      ctl->stop[x][part][r] = stop;
-      tile_sync(x);
-      if (r == 0 && part == 0) {
-        bool all = true;
-        for (int i = 0; i < ROWS; i += 32) all = all && !ctl->stop[x][0][i];
-        if (all) {
-          tma_store_3d(&to, sm + OFF_Q + x * TILE_B, 0, kvh * G, (x ? t1 : t0).y);
-          tma_store_3d(&to, sm + OFF_Q + x * TILE_B + HALF_B, 64, kvh * G, (x ? t1 : t0).y);
-          bulk_commit();
-          bulk_wait_read0();
-        }
-      }
-    }
-    if (p.check != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && r == 0 && x == 0 && part == 0) atomicAdd(p.check + 2, 1ull);
-  }
-  if (warp == 3 && lane == 0) {           // Q is there before the CTA ends, whether a product read it or not
-    mbar_wait(&ctl->q_ready[0], 0, nullptr);
-    mbar_wait(&ctl->q_ready[1], 0, nullptr);
   }
   tc_fence_before();
   __syncthreads();
@@ -1300,11 +1370,11 @@ static int launch_prefill(const void* q, void* o, const void* cache, long long n
   if (p.check != nullptr && row_idx == nullptr) return -1;
   CUtensorMap tm;
   if (!make_map_bf16_sw128(&tm, cache, num_blocks * 2 * nkv * PAGE, D, D, 64, PAGE)) return -2;
-  // Q and O by token: the tiles say which tokens there are
-  CUtensorMap tq, to;
+  // Q by token: the tiles say which tokens there are
+  CUtensorMap tq, tq1;
   const int G = nq / nkv;
   if (!make_map3_bf16_sw128(&tq, q, 1ll << 31, nq, D, 64, G, ROWS / G) ||
-      !make_map3_bf16_sw128(&to, o, 1ll << 31, nq, D, 64, G, ROWS / G))
+      !make_map3_bf16_sw128(&tq1, q, 1ll << 31, nq, D, 64, G, 1))
     return -2;
   // the attributes belong to a device; one bit for each that has them (setting them twice does no harm)
   static std::atomic<unsigned long long> ready{0};
@@ -1333,7 +1403,7 @@ static int launch_prefill(const void* q, void* o, const void* cache, long long n
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = overlap ? 1 : 0;
-  return static_cast<int>(pingpong ? cudaLaunchKernelEx(&cfg, prefill_pp_kernel, tm, tq, to, p)
+  return static_cast<int>(pingpong ? cudaLaunchKernelEx(&cfg, prefill_pp_kernel, tm, tq, tq1, p)
                                    : cudaLaunchKernelEx(&cfg, prefill_tc_kernel, tm, p));
 }
 

@@ -490,8 +490,14 @@ __device__ __forceinline__ float2 fma2(uint32_t a, uint32_t b, float s, float d)
       : "r"(a), "r"(b), "f"(s), "f"(d));
   return r;
 }
-// 32 bytes, a whole sector, in one store.
-__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+// 32 bytes, a whole sector: in one store where the output lies on 32-byte boundaries (`wide`), else in two.
+__device__ __forceinline__ void store32(void* p, const uint32_t* w, bool wide) {
+  if (!wide) {
+    uint4* q = static_cast<uint4*>(p);
+    q[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    q[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    return;
+  }
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
@@ -786,6 +792,7 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t s_col = tmem + x * KT + lane_off, o_col = tmem + 2 * KT + x * D + lane_off;
     const int key0 = (1 - part) * 64;
+    const bool wide = (reinterpret_cast<uintptr_t>(p.o) & 31) == 0;
     int turn = 0, outs = 0;               // turns of S_x and O_x so far
     for (int n = 0;; ++n) {
       const Pair* pr = pair_of(n);
@@ -918,8 +925,8 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
           for (int i = 0; i < 16; ++i) w[c][i] = pack_bf16x2(u32_as_f32(v[2 * i]) * inv, u32_as_f32(v[2 * i + 1]) * inv);
           if (p.check == nullptr) {
             if (tok >= 0) {
-              store32(orow + part * 64 + c * 32, &w[c][0]);
-              store32(orow + part * 64 + c * 32 + 16, &w[c][8]);
+              store32(orow + part * 64 + c * 32, &w[c][0], wide);
+              store32(orow + part * 64 + c * 32 + 16, &w[c][8], wide);
             }
           } else if (tok >= 0) {
             uint4* dst = reinterpret_cast<uint4*>(orow + part * 64 + c * 32);

@@ -544,6 +544,31 @@ def test_prefill_of_few_tokens(nq, nkv, lens, prior):
     assert out[starts[-1]:].isnan().all() and torch.equal(out[:starts[-1]], want[:starts[-1]])
 
 
+def test_prefill_tensors_on_16_byte_boundaries():
+    """Views whose rows begin 16 bytes behind a 32-byte boundary, over both caches: the same bits."""
+    lens, nq, nkv = [300, 77], 8, 2
+    _, cache, bt, _, _, _ = _decode_case(lens, nq, nkv, seed=6, spread=1.0)
+    q = torch.randn(377, nq, 128, device=DEV).bfloat16()
+    pos = torch.cat([torch.arange(n) for n in lens]).int().to(DEV)
+    tiles = attention.prefill_tiles([0, 300], lens, nq // nkv).to(DEV)
+    plain = cache.values().bfloat16().contiguous()
+    off = [torch.zeros(q.numel() + 16, dtype=torch.bfloat16, device=DEV)[8:8 + q.numel()].view(q.shape) for _ in range(2)]
+    off[0].copy_(q)
+    assert all(t.data_ptr() % 32 == 16 for t in off)
+    plan = attention.prefill8_plan(bt, lens, nkv)
+    want = attention.prefill8(q, cache, plan, pos, tiles)
+    assert torch.equal(attention.prefill8(off[0], cache, plan, pos, tiles, out=off[1]), want)
+    off[1].zero_()
+    assert torch.equal(attention.prefill(off[0], plain, bt, pos, tiles, nq, nkv, out=off[1]), want)
+    few = torch.zeros_like(want[:40])
+    plan = attention.prefill8_plan(bt[:1], [40], nkv)
+    tiles = attention.prefill_tiles([0], [40], nq // nkv).to(DEV)
+    attention.prefill8(q[:40], cache, plan, pos[:40].contiguous(), tiles, out=few)
+    off[1].zero_()
+    attention.prefill8(off[0][:40], cache, plan, pos[:40].contiguous(), tiles, out=off[1][:40])
+    assert torch.equal(off[1][:40], few) and (off[1][40:] == 0).all()
+
+
 def test_prefill_pages_and_positions_outside():
     """A page outside the cache gives NaN to its request alone; a position outside the plan's table gives zeros."""
     lens = [40, 33]

@@ -123,7 +123,7 @@ SIGNATURES: dict[str, tuple] = {
     "sdc_kv8_append": (I, [P]),
     "sdc_kv8_expand": (I, [P]),
     "sdc_attn_prefill_expanded": (I, [P]),
-    "sdc_kv8_tokens": (I, [P]),
+    "sdc_kv8_prefill_few": (I, [P]),
     "sdc_kv8_decode": (I, [P]),
     "sdc_matvec4": (I, [P]),
     "sdc_ep_receive_grouped": (I, [P, P, P, P, P, I, I, I, I, I, P, P, P, P, P, P, P, P, P]),
@@ -134,7 +134,7 @@ STRUCTS: dict[str, struct.Struct] = {
     "sdc_kv8_append": struct.Struct("@PqiiiPPPPdPiiiPPPqPiPP"),
     "sdc_kv8_expand": struct.Struct("@PPqPiiPiiPP"),
     "sdc_attn_prefill_expanded": struct.Struct("@PPPqPiPPiPiifPPP"),
-    "sdc_kv8_tokens": struct.Struct("@PiiPiPiiPPPP"),
+    "sdc_kv8_prefill_few": struct.Struct("@PiiPiPiiPPPP" "PPPPqPiiqPPPiiiiiifPPPP"),
     "sdc_kv8_decode": struct.Struct("@PPPPqPiiqPPPiiiiiifPPPP"),
     "sdc_matvec4": struct.Struct("@PqiiiiPPPiPPqPPiPP"),
 }

@@ -1286,8 +1286,8 @@ struct Kv8TokensArgs {
   void* idx;
   void* stream;
 };
-int sdc_kv8_tokens(const Kv8TokensArgs* args) {
-  const auto& [tiles, ntiles, tile_tokens, row_idx, nrows, pos, limit, T, req, ctx, idx, stream] = *args;
+static int list_tokens(const Kv8TokensArgs& args) {
+  const auto& [tiles, ntiles, tile_tokens, row_idx, nrows, pos, limit, T, req, ctx, idx, stream] = args;
   if (T <= 0) return 0;
   if (ntiles < 0 || nrows < 0 || (nrows > 0 && row_idx == nullptr)) return -1;
   const TokensParams p{static_cast<const int4*>(tiles), ntiles, tile_tokens, row_idx, nrows, pos, limit, T,
@@ -1364,6 +1364,16 @@ int sdc_kv8_decode(const Kv8DecodeArgs* args) {
   auto st = static_cast<cudaStream_t>(stream);
   return p.G <= 8 ? launch_decode<1>(tm, p, nrun, static_cast<int>(z), st)
                   : launch_decode<2>(tm, p, nrun, static_cast<int>(z), st);
+}
+
+// A prefill of few tokens: its tiles' tokens as sequences (lists that `decode` reads), then those.
+struct Kv8FewArgs {
+  Kv8TokensArgs tokens;
+  Kv8DecodeArgs decode;
+};
+int sdc_kv8_prefill_few(const Kv8FewArgs* args) {
+  const int rc = list_tokens(args->tokens);
+  return rc != 0 ? rc : sdc_kv8_decode(&args->decode);
 }
 
 }  // extern "C"

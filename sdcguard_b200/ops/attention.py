@@ -282,17 +282,19 @@ def _prefill8_few(q, cache, plan, pos, tiles, out, row_idx, row_sq, scale, check
         raise ValueError(f"{cache.num_blocks} pages of {nkv} heads (below 2^26 in all)")
     rows = 0 if row_idx is None else row_idx.shape[0]
     seg, segs = decode8_cut(t, nkv, keys)
-    lists = torch.empty(3 * t + rows, dtype=torch.int32, device=dev)
-    part = torch.empty(t * nq * segs * 132, dtype=torch.float32, device=dev) if segs > 1 else None
-    at = lists.data_ptr()
-    kv8.launch("sdc_kv8_tokens", dev, (
-        tiles.data_ptr(), tiles.shape[0], ROWS // (nq // nkv), kv8.ptr(row_idx), rows, pos.data_ptr(), keys, t, at,
-        at + 4 * t, at + 8 * t))
-    bt = plan.block_table
-    kv8.launch("sdc_kv8_decode", dev, (
+    part = t * nq * segs * 132 if segs > 1 else 0         # floats, then the lists, where the expanded pages would go
+    need = part + 3 * t + rows
+    work = plan.work if plan.work.numel() >= 2 * need else torch.empty(need, dtype=torch.int32, device=dev)
+    part_at, bt = work.data_ptr(), plan.block_table
+    req_at = part_at + 4 * part
+    ctx_at, idx_at = req_at + 4 * t, req_at + 8 * t
+    stream = kv8.stream(dev)                              # (of the first half of the arguments)
+    kv8.launch("sdc_kv8_prefill_few", dev, (
+        tiles.data_ptr(), tiles.shape[0], ROWS // (nq // nkv), kv8.ptr(row_idx), rows, pos.data_ptr(), keys, t, req_at,
+        ctx_at, idx_at, stream,
         q.data_ptr(), out.data_ptr(), cache.codes.data_ptr(), cache.scales.data_ptr(), cache.num_blocks, bt.data_ptr(),
-        bt.shape[0], bt.shape[1], bt.stride(0), at, at + 4 * t, at + 8 * t, t + rows, t, nq, nkv, seg, segs,
-        _SCALE if scale is None else scale, kv8.ptr(part), kv8.ptr(row_sq), kv8.ptr(check)))
+        bt.shape[0], bt.shape[1], bt.shape[1], req_at, ctx_at, idx_at, t + rows, t, nq, nkv, seg, segs,
+        _SCALE if scale is None else scale, part_at, kv8.ptr(row_sq), kv8.ptr(check)))
     return out
 
 

@@ -56,6 +56,13 @@ def on(device: torch.device):
     return _same if _here() == device.index else torch.cuda.device(device.index)
 
 
+def stream(device: torch.device) -> int:
+    """`device`'s current stream as a bare handle."""
+    if device.index is None:
+        raise ValueError(f"the kernels run on a CUDA device, not on {device}")
+    return _stream(device.index)
+
+
 def launch(entry: str, device: torch.device, args: tuple) -> None:
     """Calls the library's `entry` with args (addresses as integers, 0 for none) and `device`'s current stream. (These
     operators run for a few microseconds: the arguments cross as one struct, and the stream is taken as the bare

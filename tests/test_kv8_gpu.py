@@ -526,6 +526,11 @@ def test_prefill_of_few_tokens(nq, nkv, lens, prior):
     assert torch.allclose(rs[:T], out[:T].float().square().sum((1, 2)), rtol=2e-5)
     req = torch.repeat_interleave(torch.arange(len(lens)), torch.tensor(lens)).int().to(DEV)
     _check_decode((q[:T], cache, bt, req, pos[:T] + 1, None), out[:T])
+    small = attention.prefill8_plan(bt, ctxs, nkv)           # where the plan's pages are too small for the partial sums
+    small.work = small.work[:0]
+    again = torch.full_like(q, 7.0)
+    attention.prefill8(q, cache, small, pos, tiles, out=again)
+    assert torch.equal(again, out)
     rt, ridx = attention.replay_tiles([[s + n - 1] for s, n in zip(starts, lens)], G)
     rt, ridx = rt.to(DEV), ridx.to(DEV)
     st = _state(2)

@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
 //
 // Measured (16 query, 8 kv heads, device time): 256 x 1600 keys 135 us, 6.2 TB/s, 0.95 of a copy's rate: DRAM bounds it.
 // 1 x 131072 keys 53 us, 5.1 TB/s, with the merge of its segments and the start of the CTAs in it; 61 ragged ones up to
-// 4100 keys 64 us, 4.2 TB/s, the longest rows' tail. 1 x 37 keys 3.8 us, latency. Loads into registers instead of the
+// 4100 keys 59 us, 4.5 TB/s, the longest rows' tail. 1 x 37 keys 3.8 us, latency. Loads into registers instead of the
 // ring: 162 us for the first; a ring filled by cp.async: 159; two warps a CTA: 131, but 67 and 76 us for the next two.
 constexpr int WARPS = 4;
 constexpr int REC = D + 4;               // floats a record: o[D], M, l, pad

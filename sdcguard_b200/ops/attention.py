@@ -142,14 +142,28 @@ def decode8_cut(nseq: int, nkv: int, max_ctx: int) -> tuple[int, int]:
     idle, more pay the start of a CTA and the merge again. One sequence is cut into as many as run at once (131072 keys,
     8 kv heads: 149 pages a segment 51.6 us, 112 pages 55.8 us, 74 pages 62 us). Several differ in length and
     balance better in twice as many (8 of up to 8000: 39 pages 21.3 us, 64 pages 27.0 us). At least 12 pages (1 x 20000
-    keys, one kv head: 12 pages 11.2 us, 8 pages 12.9 us, 24 pages 12.4 us), at most 256, at most 256 segments (what
+    keys, one kv head: 12 pages 11.2 us, 8 pages 12.9 us, 24 pages 12.4 us), of several sequences 20 (16 x 1200: 15.2 us, 12
+    pages 18.5), at most 256, at most 256 segments (what
     one combine CTA merges), and no cut up to 24 pages, where the merge costs more than it saves (4 x 300 keys: 6.3 us,
-    in two 7.7 us)."""
+    in two 7.7 us).
+
+    Several sequences with 200 rows (a sequence and kv head) or more fill the SMs by themselves, and what a cut saves in
+    the longest row's time it pays in starts and merges. Ragged and uniform lengths, uncut against two segments: 320 rows
+    of up to 44 pages 12.2 and 16.0 us, 14.1 and 21.5 (of 100 pages, three segments: 24.7 and 28.4, 21.2 and 34.1: cut);
+    448 of 177 pages 48.9 and 58.6, 50.4 and 80.6; 640 of 57 pages 22.3 and 39.1, 27.4 and 41.3 (720 of 125 pages 44.8 and
+    80.8, 44.9 and 74.6: cut); 880 of 125 pages 53.7 and 84.2, 58.3 and 97.2. Two segments are 3/5 and 2/5 of the longest
+    row, which leaves more rows whole than halves do: 488 rows of 257 pages 58.5 and 98.0 us, halves 63.9 and 99.2."""
     pages = -(-max_ctx // PAGE)
     if pages <= 24:
         return pages, 1
+    rows = nseq * nkv
+    if nseq > 1 and rows >= 200:
+        if pages <= (64 if rows < 388 else 192 if rows <= 148 * 4 else 96 if rows < 800 else 256):
+            return pages, 1
+        if 388 <= rows < 800 and pages * 3 // 5 <= 252:
+            return -(-pages * 3 // 20) * 4, 2
     ctas = DECODE8_CTAS if nseq == 1 else 2 * DECODE8_CTAS
-    seg = max(12, min(256, -(-nseq * nkv * pages // ctas)), -(-pages // DECODE8_MAX_SEGS))
+    seg = max(12 if nseq == 1 else 20, min(256, -(-nseq * nkv * pages // ctas)), -(-pages // DECODE8_MAX_SEGS))
     segs = -(-pages // seg)
     seg = -(-pages // segs)                       # alike, and a multiple of the four warps where that adds no segment
     seg = min(-(-seg // 4) * 4, pages)

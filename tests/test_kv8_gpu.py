@@ -326,6 +326,22 @@ def test_decode_matches_64_bits_and_replays_exactly(nq, nkv):
     assert _flat(st[0])[::2] == (0, 1) and _flat(st[1]) == (math.inf, (8 * nq + nq - 1) * 128 + 77, 1)
 
 
+@pytest.mark.parametrize("seqs,ctx,nq,nkv,segs", [(16, 1200, 8, 8, 4), (98, 3200, 8, 4, 2), (40, 1600, 8, 8, 3)])
+def test_decode_few_segments_of_many_rows(seqs, ctx, nq, nkv, segs):
+    """Rows that end before, in and at the end of a segment (the last one shorter), each as if it were alone."""
+    seg = attention.decode8_cut(seqs, nkv, ctx)[0] * 16
+    assert attention.decode8_cut(seqs, nkv, ctx)[1] == segs
+    ends = [ctx, seg - 1, seg, seg + 1, seg * (segs - 1), seg * (segs - 1) + 1, 0, 1]
+    ctxs = (ends + [1 + (i * 7919) % ctx for i in range(seqs)])[:seqs]
+    args = _decode_case(ctxs, nq, nkv, seed=ctx)
+    out = attention.decode8(*args)
+    _check_decode(args, out, rows=range(8))
+    pick = torch.tensor([seqs - 1, 5, 3, 0], dtype=torch.int32, device=DEV)
+    again = torch.empty_like(out)
+    attention.decode8(*args, out=again, seq_idx=pick)
+    assert torch.equal(again[pick.long()], out[pick.long()])
+
+
 @pytest.mark.parametrize("seqs,ctx,nq,nkv", [(1, 4097, 8, 2), (2, 20000, 4, 1), (40, 700, 8, 8), (300, 90, 4, 2)])
 def test_decode_cut_of_the_keys(seqs, ctx, nq, nkv):
     """Batches that are cut into one, few and many segments; a row's bits do not depend on the rows around it."""

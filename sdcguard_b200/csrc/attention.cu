@@ -69,8 +69,8 @@ __device__ __forceinline__ float ex2(float x) {
 // ---------------------------------------------------------------------------------------------- prefill, tcgen05
 // The same tiles and row determinism as `prefill_kernel`, on the 5th-generation tensor cores:
 //   warp 0   TMA: the request's K and V pages of a 128-key tile (one 16-row x 128-byte box per page, half the head
-//            dim, K or V, 128-byte swizzle) into one of two stages; the unloaded V rows of a partial last tile are
-//            cleared (their weights are zero, stale shared memory could hold NaN patterns);
+//            dim, K or V, 128-byte swizzle) into one of two stages; V rows behind the last key that a row of the tile
+//            sees are cleared (see v_rows);
 //   warp 1   MMA: S = Q K^T into one of two TMEM accumulators (M = 128 rows, N = 128 keys, K = 128), and
 //            O += P V into a third (V as an MN-major operand, dims contiguous); S of tile j+1 is computed while
 //            the softmax works on tile j;
@@ -102,7 +102,28 @@ constexpr int SMEM = OFF_CTL + static_cast<int>(sizeof(Ctl)) + 1024;
 constexpr int SOFT = 2 * ROWS;            // softmax threads: warpgroup g takes keys / dims [64 g, 64 g + 64)
 }  // namespace pf
 
+// V of a key tile, of which rows [0, n) are keys that some row of the query tiles sees. The weights of the others are zero,
+// but the MMA multiplies V by them, and 0 * NaN is NaN: what a page holds behind its sequence's end is whatever was stored
+// there last, as is shared memory that nothing was loaded to. So only keys are loaded (the last page's one by one, through
+// `tr`, whose box is one row) and the rest is cleared. (Keys that one row sees and another does not stay: a V of NaN reaches
+// its dim in rows of the same tiles up to 127 places before it.) One warp; returns behind the clearing, which the loads'
+// barrier publishes.
+constexpr int V_HALF = 128 * 128;         // bytes of 64 dims of a tile
+__device__ __forceinline__ void clear_v(uint8_t* buf, int n, int lane) {
+  for (int i = lane; i < (128 - n) * 16; i += 32) {
+    const int r = n + (i >> 4), c = i & 15;
+    *reinterpret_cast<uint4*>(buf + (c >> 3) * V_HALF + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+}
+// The keys of the last, partial page: `row` is its first row in the map, n the tile's keys.
+__device__ __forceinline__ void load_v_rest(uint8_t* buf, const CUtensorMap* tr, uint64_t* bar, int row, int n, int lane) {
+  const int r = lane >> 1, half = lane & 1;
+  if (r < n % PAGE) tma_load_2d(buf + half * V_HALF + (n / PAGE * PAGE + r) * 128, tr, bar, half * 64, row + r);
+}
+
 __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __grid_constant__ CUtensorMap tm,
+                                                            const __grid_constant__ CUtensorMap tr,
                                                             const PrefillParams p) {
   pdl_trigger();   // a dependent GEMM may start its prologue and weight loads now
   using namespace pf;
@@ -169,29 +190,24 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
         ok = false;
         break;
       }
-      const int npg = min(KT / PAGE, maxpos / PAGE - j * (KT / PAGE) + 1);
+      const int nkeys = min(KT, maxpos + 1 - j * KT), npg = (nkeys + PAGE - 1) / PAGE;
       uint8_t* kbuf = sm + OFF_K + st * TILE_B;
       uint8_t* vbuf = sm + OFF_V + st * TILE_B;
-      if (npg < KT / PAGE) {
-        for (int i = lane; i < (KT - npg * PAGE) * 16; i += 32) {
-          const int rr = npg * PAGE + (i >> 4), c = i & 15;
-          *reinterpret_cast<uint4*>(vbuf + (c >> 3) * HALF_B + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-      }
+      if (nkeys < KT) clear_v(vbuf, nkeys, lane);
       __syncwarp();
       if (lane == 0) {
         mbar_arrive_expect_tx(&ctl->k_full[st], npg * PG_BYTES);
-        mbar_arrive_expect_tx(&ctl->v_full[st], npg * PG_BYTES);
+        mbar_arrive_expect_tx(&ctl->v_full[st], nkeys * (PG_BYTES / PAGE));
       }
       __syncwarp();
-      if (lane < 4 * npg) {
-        const int pg = lane >> 2, kv = (lane >> 1) & 1, half = lane & 1;
-        const long long blk = bt[j * (KT / PAGE) + pg];
-        const int row = static_cast<int>(((blk * 2 + kv) * p.nkv + kvh) * PAGE);
-        uint8_t* dst = (kv ? vbuf : kbuf) + half * HALF_B + pg * PAGE * 128;
-        tma_load_2d(dst, &tm, kv ? &ctl->v_full[st] : &ctl->k_full[st], half * 64, row);
-      }
+      const auto row_of = [&](int pg, int kv) {
+        return static_cast<int>(((static_cast<long long>(bt[j * (KT / PAGE) + pg]) * 2 + kv) * p.nkv + kvh) * PAGE);
+      };
+      const int pg = lane >> 2, kv = (lane >> 1) & 1, half = lane & 1;
+      if (pg < (kv ? nkeys / PAGE : npg))
+        tma_load_2d((kv ? vbuf : kbuf) + half * HALF_B + pg * PAGE * 128, &tm, kv ? &ctl->v_full[st] : &ctl->k_full[st],
+                    half * 64, row_of(pg, kv));
+      if (nkeys % PAGE) load_v_rest(vbuf, &tr, &ctl->v_full[st], row_of(npg - 1, 1), nkeys, lane);
       last = j;
     }
     if (!ok && lane == 0) {
@@ -539,6 +555,7 @@ __device__ __forceinline__ bool next_index(const uint4* answer, int& x, int& y) 
 __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid_constant__ CUtensorMap tm,
                                                                     const __grid_constant__ CUtensorMap tq,
                                                                     const __grid_constant__ CUtensorMap tq1,
+                                                                    const __grid_constant__ CUtensorMap tr,
                                                                     const PrefillParams p) {
   pdl_trigger();
   using namespace pp;
@@ -695,25 +712,21 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
           ok = false;
           break;
         }
-        const int npg = min(KT / PAGE, maxpos / PAGE - j * (KT / PAGE) + 1);
+        // whole pages of K (masked scores are not used), of V the keys alone
+        const int nkeys = min(KT, maxpos + 1 - j * KT), npg = kv ? nkeys / PAGE : (nkeys + PAGE - 1) / PAGE;
         uint8_t* buf = sm + (kv ? OFF_V : OFF_K) + st * TILE_B;
-        if (kv && npg < KT / PAGE) {
-          // the weights of keys past the last page are zero, but stale shared memory could hold NaN patterns
-          for (int i = lane; i < (KT - npg * PAGE) * 16; i += 32) {
-            const int rr = npg * PAGE + (i >> 4), c = i & 15;
-            *reinterpret_cast<uint4*>(buf + (c >> 3) * HALF_B + rr * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-        }
+        if (kv && nkeys < KT) clear_v(buf, nkeys, lane);
         __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&full[st], npg * PG_BYTES);
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], kv ? nkeys * (PG_BYTES / PAGE) : npg * PG_BYTES);
         __syncwarp();
+        const auto row_of = [&](int pg) {
+          return static_cast<int>(((static_cast<long long>(bt[j * (KT / PAGE) + pg]) * 2 + kv) * p.nkv + kvh) * PAGE);
+        };
         if (lane < 2 * npg) {
           const int pg = lane >> 1, half = lane & 1;
-          const long long blk = bt[j * (KT / PAGE) + pg];
-          const int row = static_cast<int>(((blk * 2 + kv) * p.nkv + kvh) * PAGE);
-          tma_load_2d(buf + half * HALF_B + pg * PAGE * 128, &tm, &full[st], half * 64, row);
+          tma_load_2d(buf + half * HALF_B + pg * PAGE * 128, &tm, &full[st], half * 64, row_of(pg));
         }
+        if (kv && nkeys % PAGE) load_v_rest(buf, &tr, &full[st], row_of(npg), nkeys, lane);
       }
     }
     if (!ok) {
@@ -1375,8 +1388,10 @@ static int launch_prefill(const void* q, void* o, const void* cache, long long n
   p.row_sq = static_cast<float*>(row_sq);
   p.check = static_cast<unsigned long long*>(check);
   if (p.check != nullptr && row_idx == nullptr) return -1;
-  CUtensorMap tm;
-  if (!make_map_bf16_sw128(&tm, cache, num_blocks * 2 * nkv * PAGE, D, D, 64, PAGE)) return -2;
+  CUtensorMap tm, tr;
+  if (!make_map_bf16_sw128(&tm, cache, num_blocks * 2 * nkv * PAGE, D, D, 64, PAGE) ||
+      !make_map_bf16_sw128(&tr, cache, num_blocks * 2 * nkv * PAGE, D, D, 64, 1))
+    return -2;
   // Q by token: the tiles say which tokens there are
   CUtensorMap tq, tq1;
   const int G = nq / nkv;
@@ -1410,8 +1425,8 @@ static int launch_prefill(const void* q, void* o, const void* cache, long long n
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = overlap ? 1 : 0;
-  return static_cast<int>(pingpong ? cudaLaunchKernelEx(&cfg, prefill_pp_kernel, tm, tq, tq1, p)
-                                   : cudaLaunchKernelEx(&cfg, prefill_tc_kernel, tm, p));
+  return static_cast<int>(pingpong ? cudaLaunchKernelEx(&cfg, prefill_pp_kernel, tm, tq, tq1, tr, p)
+                                   : cudaLaunchKernelEx(&cfg, prefill_tc_kernel, tm, tr, p));
 }
 
 extern "C" {

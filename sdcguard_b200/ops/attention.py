@@ -75,7 +75,7 @@ def prefill(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, pos
             row_idx: Optional[torch.Tensor] = None, row_sq: Optional[torch.Tensor] = None,
             scale: Optional[float] = None, check: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q: (T, nq, 128) bf16; tiles/row_idx/pos/block_table int32 on the device. out: (T, nq, 128) or, for a
-    replay, any tensor indexed by the same token ids. With `check` (a state row; replay tiles and row_idx
+    replay, any tensor indexed by the same token ids. What a page holds behind its sequence's end reaches no row. With `check` (a state row; replay tiles and row_idx
     given), the sampled rows are recomputed and compared with `out` instead of written."""
     if out is None:
         out = torch.empty_like(q)
@@ -319,8 +319,10 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
     """`prefill` over a cache of 8 bits: the plan's pages are expanded to bf16 (exact for power-of-two scales), then the
     tensor-core prefill reads those; a call of few tokens (T kv heads <= FEW_ROWS) runs through the decode kernel instead, a
     sequence for each token, so a row's last bits depend on which of the two its call takes. q (T, nq, 128), tiles from
-    `prefill_tiles`, requests numbered as in the plan. A position outside the plan's table gives a row of zeros, a page
-    outside the cache NaN. With `check`: the rows of the replay tiles are compared, and every pages_step-th expanded page
+    `prefill_tiles`, requests numbered as in the plan, each token's position below its request's ctx_lens. A position outside
+    the plan's table gives a row of zeros, a page outside the cache NaN. What a page holds behind its sequence's end reaches
+    no row. (A value of NaN inside the sequence gives its dim NaN in the rows that see it and, in calls that are not of few
+    tokens, in rows up to 127 places before it.) With `check`: the rows of the replay tiles are compared, and every pages_step-th expanded page
     (where there are such) from pages_from on."""
     given = out
     t, nq, out = _want_q(q, cache, out)

@@ -1,0 +1,128 @@
+"""Prefill attention on the tensor cores, over the 8-bit and over the bf16 cache: values that are not finite (in masked
+places, behind a sequence's end, in queries and keys), rows without keys, and pages outside the cache. Comparisons are of
+bits: what a row must not see does not change it."""
+import math
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from sdcguard_b200.ops import attention
+from sdcguard_b200.ops.kv8 import KV8Cache
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+NAN, INF = float("nan"), float("inf")
+OUTSIDE = 1 << 20
+
+
+def _flat(row):
+    from sdcguard_b200.numerics import abft
+    d = abft.decode_state_row(row.cpu().tolist())
+    return d["z"], d["flat"], d["checks"]
+
+
+class Case:
+    """A prefill batch whose sequences end inside pages; `run` takes it over either cache. `few`: through the decode kernel."""
+
+    def __init__(self, lens, prior, nq, nkv, seed=0, few=False):
+        self.lens, self.prior, self.nq, self.nkv = lens, prior, nq, nkv
+        self.ctxs = [a + b for a, b in zip(lens, prior)]
+        self.T = sum(lens)
+        assert (self.T * nkv <= attention.FEW_ROWS) == few
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        need = [-(-n // 16) for n in self.ctxs]
+        blocks = sum(need) + 2
+        v = torch.randn(blocks, 2, nkv, 16, 128, device=DEV, generator=g)
+        self.cache = KV8Cache((v * 64).to(torch.float8_e4m3fn), torch.full((blocks, nkv, 2), 2.0 ** -6, device=DEV))
+        perm = torch.randperm(blocks - 2, generator=torch.Generator().manual_seed(seed)) + 1
+        self.bt = torch.zeros(len(lens), max(need) + 1, dtype=torch.int32)
+        o = 0
+        for r, n in enumerate(need):
+            self.bt[r, :n] = perm[o:o + n]
+            o += n
+        self.bt = self.bt.to(DEV)
+        self.starts = [sum(lens[:i]) for i in range(len(lens))]
+        self.pos = torch.cat([torch.arange(p, p + n) for p, n in zip(prior, lens)]).int().to(DEV)
+        self.tiles = attention.prefill_tiles(self.starts, lens, nq // nkv).to(DEV)
+        self.q = torch.randn(self.T, nq, 128, device=DEV, generator=g).bfloat16()
+
+    def codes(self):
+        return self.cache.codes.view(torch.uint8)
+
+    def plan(self):
+        return attention.prefill8_plan(self.bt, self.ctxs, self.nkv)
+
+    def run(self, kind, **kw):
+        out = kw.pop("out", None)
+        if out is None:
+            out = torch.full_like(self.q, 7.0)
+        tiles = kw.pop("tiles", self.tiles)
+        if kind == "fp8":
+            return attention.prefill8(self.q, self.cache, kw.pop("plan", None) or self.plan(), self.pos, tiles, out=out, **kw)
+        kw.pop("plan", None)
+        return attention.prefill(self.q, self.cache.values().bfloat16(), self.bt, self.pos, tiles, self.nq, self.nkv,
+                                 out=out, **kw)
+
+
+SHAPES = [(16, 8), (2, 1), (8, 8), (16, 1)]
+
+
+@pytest.mark.parametrize("kind", ["fp8", "bf16"])
+@pytest.mark.parametrize("nq,nkv", SHAPES)
+def test_places_behind_a_sequence_may_hold_anything(kind, nq, nkv):
+    c = Case([300, 77, 130], [0, 21, 1016], nq, nkv)
+    want = c.run(kind)
+    assert torch.isfinite(want).all()
+    for r, n in enumerate(c.ctxs):
+        assert n % 16
+        c.codes()[c.bt[r, n // 16].long(), :, :, n % 16:] = (0x7F, 0xFF)[r % 2]
+    c.cache.scales[0] = NAN                       # the page that fills up the table's rows
+    assert torch.equal(c.run(kind), want)
+
+
+def test_places_behind_a_sequence_of_few_tokens():
+    c = Case([30, 17], [3, 40], 4, 2, few=True)
+    want = c.run("fp8")
+    for r, n in enumerate(c.ctxs):
+        c.codes()[c.bt[r, n // 16].long(), :, :, n % 16:] = 0x7F
+    assert torch.equal(c.run("fp8"), want)
+
+
+@pytest.mark.parametrize("few", [False, True])
+@pytest.mark.parametrize("kind", ["fp8", "bf16"])
+def test_a_value_that_is_not_finite_reaches_its_dim(kind, few):
+    """A V of NaN that every row sees: its dim in the heads of its kv head, and nothing else."""
+    c = Case([150], [7], 4, 2, few=True) if few else Case([300, 77], [7, 150], 4, 2)
+    want = c.run(kind)
+    c.codes()[c.bt[0, 0].long(), 1, 0, 3, 17] = 0x7F
+    out = c.run(kind)
+    n = c.lens[0]
+    assert out[:n, :2, 17].isnan().all()
+    out[:n, :2, 17] = want[:n, :2, 17]
+    assert torch.equal(out, want)
+
+
+def test_pages_outside_the_cache_give_nan_to_their_request():
+    c = Case([300, 77], [0, 150], 4, 2)
+    want = c.run("fp8")
+    c.bt[1, 0] = OUTSIDE
+    out = c.run("fp8")
+    assert torch.equal(out[:300], want[:300]) and out[300:].isnan().all()
+    c.bt[1, 0] = -1
+    assert c.run("fp8")[300:].isnan().all()
+
+
+def test_one_tile_a_cta():
+    """The kernel that takes one query tile a CTA (its choice is read once in a process) answers the same calls."""
+    if os.environ.get("SDCGUARD_PREFILL_PINGPONG") == "0":
+        pytest.skip("this is that process")
+    env = dict(os.environ, SDCGUARD_PREFILL_PINGPONG="0")
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-m", "pytest", "-q", "-x", "-m", "gpu", "-p", "no:cacheprovider",
+                        os.path.join(here, "test_prefill_rows_gpu.py"),
+                        os.path.join(here, "test_kv8_gpu.py") + "::test_prefill_matches_64_bits_and_replays_exactly"],
+                       env=env, capture_output=True, text=True, timeout=600, cwd=os.path.dirname(here))
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-1000:]

@@ -106,7 +106,7 @@ constexpr int SOFT = 2 * ROWS;            // softmax threads: warpgroup g takes 
 // but the MMA multiplies V by them, and 0 * NaN is NaN: what a page holds behind its sequence's end is whatever was stored
 // there last, as is shared memory that nothing was loaded to. So only keys are loaded (the last page's one by one, through
 // `tr`, whose box is one row) and the rest is cleared. (Keys that one row sees and another does not stay: a V of NaN reaches
-// its dim in rows of the same tiles up to 127 places before it.) One warp; returns behind the clearing, which the loads'
+// its dim in rows of the same query tile up to 254 places before it.) One warp; returns behind the clearing, which the loads'
 // barrier publishes.
 constexpr int V_HALF = 128 * 128;         // bytes of 64 dims of a tile
 __device__ __forceinline__ void clear_v(uint8_t* buf, int n, int lane) {
@@ -320,7 +320,9 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
         l *= alpha;
         m_use = mx;
       }
-      // pass 2: weights as bf16, their partial row sum
+      // pass 2: weights as bf16, their partial row sum. Scores that are all NaN leave the maximum at -inf: 0 stands for it
+      // then, so that they reach the weights
+      const float ref = m_use > -INFINITY ? m_use : 0.f;
       uint32_t pk[32];
       float ls = 0.f;
 #pragma unroll
@@ -331,8 +333,8 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           const int key = kbase + c * 32 + i;
-          const float p0 = (key <= pos && m_use > -INFINITY) ? ex2(u32_as_f32(v[i]) * p.scale_log2 - m_use) : 0.f;
-          const float p1 = (key + 1 <= pos && m_use > -INFINITY) ? ex2(u32_as_f32(v[i + 1]) * p.scale_log2 - m_use) : 0.f;
+          const float p0 = key <= pos ? ex2(u32_as_f32(v[i]) * p.scale_log2 - ref) : 0.f;
+          const float p1 = key + 1 <= pos ? ex2(u32_as_f32(v[i + 1]) * p.scale_log2 - ref) : 0.f;
           const uint32_t w = pack_bf16x2(p0, p1);
           pk[(c * 32 + i) >> 1] = w;
           const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
       ctl->xl[gi][r] = l;
       named_bar_sync(2, SOFT);
       const float lt = ctl->xl[0][r] + ctl->xl[1][r];
-      const float inv = lt > 0.f ? 1.f / lt : 0.f;
+      const float inv = pos >= 0 ? 1.f / lt : 0.f;   // a row with keys and no weight (scores of -inf alone): 0 / 0
       const uint32_t oa = tmem + 2 * KT + gi * 64 + lane_off;
       __nv_bfloat16* orow = p.o + (static_cast<long long>(tok < 0 ? 0 : tok) * p.nq + head) * D + gi * 64;
       float sq = 0.f;
@@ -875,23 +877,23 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
             tmem_st16(o_col + part * 64 + c * 16, o);
           }
         }
-        const bool live = m_use > -INFINITY;
-        const bool plain = full && __all_sync(0xffffffffu, live);
+        // scores that are all NaN leave the maximum at -inf: 0 stands for it then, so that they reach the weights
+        const float ref = m_use > -INFINITY ? m_use : 0.f;
         uint32_t pk[2][16];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          if (plain) {
+          if (full) {
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              const float2 e = fma2(v[c][i], v[c][i + 1], p.scale_log2, -m_use);
+              const float2 e = fma2(v[c][i], v[c][i + 1], p.scale_log2, -ref);
               pk[c][i >> 1] = pack_bf16x2(ex2(e.x), ex2(e.y));
             }
           } else {
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               const int key = c * 32 + i;
-              const float p0 = (key <= lim && live) ? ex2(u32_as_f32(v[c][i]) * p.scale_log2 - m_use) : 0.f;
-              const float p1 = (key + 1 <= lim && live) ? ex2(u32_as_f32(v[c][i + 1]) * p.scale_log2 - m_use) : 0.f;
+              const float p0 = key <= lim ? ex2(u32_as_f32(v[c][i]) * p.scale_log2 - ref) : 0.f;
+              const float p1 = key + 1 <= lim ? ex2(u32_as_f32(v[c][i + 1]) * p.scale_log2 - ref) : 0.f;
               pk[c][i >> 1] = pack_bf16x2(p0, p1);
             }
           }
@@ -925,7 +927,7 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
         const int head = kvh * G + (r % G);
         tc_fence_after();
         l = ctl->l[x][r];
-        const float inv = l > 0.f ? 1.f / l : 0.f;
+        const float inv = pos >= 0 ? 1.f / l : 0.f;   // a row with keys and no weight (scores of -inf alone): 0 / 0
         __nv_bfloat16* orow = p.o + (static_cast<long long>(tok < 0 ? 0 : tok) * p.nq + head) * D;
         int bad = -1;
         uint32_t w[2][16];

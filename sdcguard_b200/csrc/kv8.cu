@@ -639,7 +639,8 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
 //   y, so the weights w = 2^(x - M + 14) s_V <= 2^15 are the largest f16 can hold whatever the pages' scales; the row
 //   sum takes 2^(x - M + 30) in fp32: x - M reaches from 60 (a page of the least scale) to -128 and below, so the bias
 //   keeps both ends inside fp32. Rounding w to f16 costs 2^-11 of it, less than the output's rounding to bf16 (2^-8).
-//   Masked keys: x = -inf and V's codes cleared (0 * NaN); rows without keys give 0.
+//   Masked keys: x = -inf and V's codes cleared (0 * NaN); rows without keys give 0, rows with scores of NaN, or of -inf
+//   alone, NaN.
 //
 // A CTA (4 warps) takes one segment of seg_pages pages of one (sequence, kv head), warp w its pages w, w + 4, ...; a
 // sequence of one segment is written at once, else a partial record per segment and head goes to `part` and
@@ -1014,7 +1015,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv8_decode_kernel
         ls = fmaf(sm.l[w][h], e, ls);
       }
       if (nseg == 1) {
-        const float inv = ls == 0.f ? 0.f : 1.f / W_SCALE / ls;
+        const float inv = 1.f / W_SCALE / ls;          // no weight (scores of -inf alone): 0 / 0
 #pragma unroll
         for (int i = 0; i < D / (WARPS * 32); ++i)
           sq += put(p, b, kvh * p.G + h, dim_of(tid + i * WARPS * 32), acc[i] * inv);
@@ -1083,7 +1084,7 @@ __global__ void __launch_bounds__(PARTS * D) kv8_combine_kernel(const DecodePara
   __syncthreads();
   if (part != 0) return;
   const float o = (osm[0][d] + osm[1][d]) + (osm[2][d] + osm[3][d]);
-  float sq = put(p, b, head, dim_of(d), lsum == 0.f ? 0.f : o / lsum * (1.f / W_SCALE));
+  float sq = put(p, b, head, dim_of(d), o / lsum * (1.f / W_SCALE));
   if (p.check == nullptr && p.row_sq != nullptr) {
     sq = warp_sum(sq);
     if ((tid & 31) == 0) atomicAdd(p.row_sq + b, sq);

@@ -321,8 +321,8 @@ def prefill8(q: torch.Tensor, cache: KV8Cache, plan: Prefill8Plan, pos: torch.Te
     sequence for each token, so a row's last bits depend on which of the two its call takes. q (T, nq, 128), tiles from
     `prefill_tiles`, requests numbered as in the plan, each token's position below its request's ctx_lens. A position outside
     the plan's table gives a row of zeros, a page outside the cache NaN. What a page holds behind its sequence's end reaches
-    no row. (A value of NaN inside the sequence gives its dim NaN in the rows that see it and, in calls that are not of few
-    tokens, in rows up to 127 places before it.) With `check`: the rows of the replay tiles are compared, and every pages_step-th expanded page
+    no row; a query of NaN, or a key that a row sees, makes the row NaN. (A value of NaN inside the sequence gives its dim NaN
+    in the rows that see it and, in calls that are not of few tokens, in rows up to 254 places before it.) With `check`: the rows of the replay tiles are compared, and every pages_step-th expanded page
     (where there are such) from pages_from on."""
     given = out
     t, nq, out = _want_q(q, cache, out)

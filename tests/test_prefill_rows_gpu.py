@@ -93,6 +93,38 @@ def test_places_behind_a_sequence_of_few_tokens():
 
 @pytest.mark.parametrize("few", [False, True])
 @pytest.mark.parametrize("kind", ["fp8", "bf16"])
+def test_queries_that_are_not_finite(kind, few):
+    c = Case([40, 33], [0, 7], 4, 2, few=True) if few else Case([300, 77], [0, 150], 4, 2)
+    want = c.run(kind)
+    a, b = c.starts[1] - 1, c.starts[1] + 5
+    c.q[0] = NAN                                  # a row with one key
+    c.q[a, 1] = NAN                               # one head
+    c.q[a, 2, 5] = INF
+    c.q[b, 3, 100] = NAN
+    out = c.run(kind)
+    bad = out.isnan().any(-1)
+    assert bad.nonzero().tolist() == [[0, 0], [0, 1], [0, 2], [0, 3], [a, 1], [a, 2], [b, 3]]
+    assert out[bad].isnan().all() and torch.equal(out[~bad], want[~bad])
+
+
+@pytest.mark.parametrize("few", [False, True])
+@pytest.mark.parametrize("kind", ["fp8", "bf16"])
+@pytest.mark.parametrize("lo,hi", [(0, 1), (130, 131), (0, 128)])
+def test_keys_that_are_not_finite_reach_the_rows_that_see_them(kind, few, lo, hi):
+    """K of NaN at the first place (all that the first row sees), in the second key tile, in all of the first tile (rows with
+    finite scores behind it)."""
+    c = Case([150], [0], 4, 2, few=True) if few else Case([300, 77], [0, 150], 4, 2)
+    want = c.run(kind)
+    for at in range(lo, hi):
+        c.codes()[c.bt[0, at // 16].long(), 0, 1, at % 16, 9] = 0x7F         # of kv head 1: query heads 2 and 3
+    out = c.run(kind)
+    hit = torch.zeros(c.T, 4, dtype=torch.bool, device=DEV)
+    hit[lo:c.lens[0], 2:] = True
+    assert out[hit].isnan().all() and torch.equal(out[~hit], want[~hit])
+
+
+@pytest.mark.parametrize("few", [False, True])
+@pytest.mark.parametrize("kind", ["fp8", "bf16"])
 def test_a_value_that_is_not_finite_reaches_its_dim(kind, few):
     """A V of NaN that every row sees: its dim in the heads of its kv head, and nothing else."""
     c = Case([150], [7], 4, 2, few=True) if few else Case([300, 77], [7, 150], 4, 2)
@@ -103,6 +135,27 @@ def test_a_value_that_is_not_finite_reaches_its_dim(kind, few):
     assert out[:n, :2, 17].isnan().all()
     out[:n, :2, 17] = want[:n, :2, 17]
     assert torch.equal(out, want)
+
+
+def test_scores_of_minus_infinity_alone_give_nan():
+    """exp(-inf - max) with a maximum of -inf: 0 / 0, as in the formula, on every path."""
+    for few in (True, False):
+        c = Case([40], [0], 2, 1, few=True) if few else Case([450], [0], 2, 1)
+        c.codes()[:, 0] = 0x38                    # keys of ones
+        c.q[1, 0] = -INF
+        for kind in ("fp8", "bf16"):
+            out = c.run(kind)
+            assert out[1, 0].isnan().all() and out.isnan().any(-1).sum() == 1
+    c = Case([40], [0], 2, 1, few=True)
+    c.codes()[:, 0] = 0x38
+    c.q[:2, 0] = -INF
+    for segs in (1, 2):
+        plan = attention.decode8_plan(2, 2, 1, 40, DEV)
+        if segs == 2:
+            plan = attention.Decode8Plan(2, 2, 1, 40, 2, 2, torch.empty(2 * 2 * 2 * 132, device=DEV))
+        out = attention.decode8(c.q[:2], c.cache, c.bt, torch.zeros(2, dtype=torch.int32, device=DEV),
+                                torch.tensor([40, 20], dtype=torch.int32, device=DEV), plan)
+        assert out[:, 0].isnan().all() and torch.isfinite(out[:, 1]).all()
 
 
 def test_pages_outside_the_cache_give_nan_to_their_request():

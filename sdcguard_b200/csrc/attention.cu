@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
       mbar_arrive(&ctl->q_ready);
     }
     float m_use = -INFINITY, l = 0.f;
-    bool stop = ntiles == 0;
+    bool stop = false;
     for (int j = 0; j < ntiles; ++j) {
       const int st = j & 1;
       const bool got = mbar_wait(&ctl->s_full[st], (j >> 1) & 1u, abort_flag);
@@ -385,12 +385,12 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
         stop = true;
       }
     }
-    if (!stop && ntiles > 0) {
+    if (!stop) {                          // (a row without keys is zeros)
       tc_fence_after();
       ctl->xl[gi][r] = l;
       named_bar_sync(2, SOFT);
       const float lt = ctl->xl[0][r] + ctl->xl[1][r];
-      const float inv = pos >= 0 ? 1.f / lt : 0.f;   // a row with keys and no weight (scores of -inf alone): 0 / 0
+      const float inv = 1.f / lt;         // a row with keys and no weight (scores of -inf alone): 0 / 0
       const uint32_t oa = tmem + 2 * KT + gi * 64 + lane_off;
       __nv_bfloat16* orow = p.o + (static_cast<long long>(tok < 0 ? 0 : tok) * p.nq + head) * D + gi * 64;
       float sq = 0.f;
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          w[i] = pack_bf16x2(u32_as_f32(v[2 * i]) * inv, u32_as_f32(v[2 * i + 1]) * inv);
+          w[i] = pos >= 0 ? pack_bf16x2(u32_as_f32(v[2 * i]) * inv, u32_as_f32(v[2 * i + 1]) * inv) : 0u;
           const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
           sq = fmaf(f.x, f.x, fmaf(f.y, f.y, sq));
         }
@@ -455,7 +455,8 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
 //               with half of the key tile: masked maximum (exchanged), conditional rescale of O (only when the
 //               reference maximum moves by more than 2^8), P = exp2(S - max) rounded to bf16 and written back
 //               over the last 64 columns of S_x, the row sum of those bf16 weights (in one order: the second thread
-//               goes on from the first's sum while the MMAs run); at the end O / l
+//               goes on from the first's sum while the MMAs run); at the end O / l,
+//               zeros for a row without keys
 // Bound by the chain of one tile: its softmax (2290 cycles a 128-key tile, 1600 of them the exponentials, which the two
 // tiles share the unit for) and the MMAs behind it (1500), against 2048 cycles for the exponentials or the MMAs of both
 // tiles alone. 8 x 2048 tokens, 16 / 8 heads: 162 us, 849 TFLOP/s, 0.50 of a dense bf16 product's rate; 32 x 1024 210 us,
@@ -923,11 +924,12 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
       pair_sync(x, quarter);
       stop = __any_sync(0xffffffffu, stop || ctl->stop[x][part ^ 1][r]);
       const int bx = pr->bx, kvh = pr->kvh;
-      if (!stop && my_tiles > 0) {
+      // a row without keys is zeros, whether or not others of its tile have some
+      if (!stop && __any_sync(0xffffffffu, tok >= 0)) {
         const int head = kvh * G + (r % G);
         tc_fence_after();
         l = ctl->l[x][r];
-        const float inv = pos >= 0 ? 1.f / l : 0.f;   // a row with keys and no weight (scores of -inf alone): 0 / 0
+        const float inv = 1.f / l;        // a row with keys and no weight (scores of -inf alone): 0 / 0
         __nv_bfloat16* orow = p.o + (static_cast<long long>(tok < 0 ? 0 : tok) * p.nq + head) * D;
         int bad = -1;
         uint32_t w[2][16];
@@ -937,7 +939,8 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
           tmem_ld32(o_col + part * 64 + c * 32, v);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) w[c][i] = pack_bf16x2(u32_as_f32(v[2 * i]) * inv, u32_as_f32(v[2 * i + 1]) * inv);
+          for (int i = 0; i < 16; ++i)
+            w[c][i] = pos >= 0 ? pack_bf16x2(u32_as_f32(v[2 * i]) * inv, u32_as_f32(v[2 * i + 1]) * inv) : 0u;
           if (p.check == nullptr) {
             if (tok >= 0) {
               store32(orow + part * 64 + c * 32, &w[c][0], wide);

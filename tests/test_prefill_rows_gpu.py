@@ -158,6 +158,34 @@ def test_scores_of_minus_infinity_alone_give_nan():
         assert out[:, 0].isnan().all() and torch.isfinite(out[:, 1]).all()
 
 
+@pytest.mark.parametrize("nq,nkv", [(16, 8), (4, 1), (8, 8)])
+def test_positions_outside_the_table_give_rows_of_zeros(nq, nkv):
+    """One row of a live tile, a tile of one token, every row of a request (both tiles of its pairs)."""
+    per = 128 // (nq // nkv)                                 # tokens of a tile
+    c = Case([2 * per + 1, 300, 5, 40], [0, 9, 30, 0], nq, nkv)
+    want = c.run("fp8")
+    c.pos[7] = OUTSIDE
+    c.pos[2 * per] = OUTSIDE                                 # the remainder tile
+    c.pos[c.starts[2]:c.starts[3]] = OUTSIDE
+    c.pos[c.starts[3] + 3] = -1
+    rows = [7, 2 * per, c.starts[3] + 3] + list(range(c.starts[2], c.starts[3]))
+    rest = [i for i in range(c.T) if i not in rows]
+    sq = torch.zeros(c.T, device=DEV)
+    plan = c.plan()
+    out = c.run("fp8", row_sq=sq, plan=plan)
+    assert (out[rows] == 0).all() and torch.equal(out[rest], want[rest])
+    assert (sq[rows] == 0).all() and torch.allclose(sq, out.float().square().sum((1, 2)), rtol=2e-5)
+    # the replay compares such rows too
+    tiles, idx = attention.replay_tiles([[2 * per], [], [c.starts[2] + 1], []], nq // nkv)
+    tiles, idx = tiles.to(DEV), idx.to(DEV)
+    st = torch.zeros(2, 4, dtype=torch.int64, device=DEV)
+    c.run("fp8", out=out, row_idx=idx, tiles=tiles, check=st[0], plan=plan)
+    out[c.starts[2] + 1, nq - 1, 70] = 1.0
+    c.run("fp8", out=out, row_idx=idx, tiles=tiles, check=st[1], plan=plan)
+    assert _flat(st[0])[::2] == (0, 1)
+    assert _flat(st[1]) == (math.inf, ((c.starts[2] + 1) * nq + nq - 1) * 128 + 70, 1)
+
+
 def test_pages_outside_the_cache_give_nan_to_their_request():
     c = Case([300, 77], [0, 150], 4, 2)
     want = c.run("fp8")
@@ -166,6 +194,23 @@ def test_pages_outside_the_cache_give_nan_to_their_request():
     assert torch.equal(out[:300], want[:300]) and out[300:].isnan().all()
     c.bt[1, 0] = -1
     assert c.run("fp8")[300:].isnan().all()
+
+
+def test_many_pairs_a_cta():
+    """More pairs than SMs: a CTA takes over others, with rows and whole tiles that have no keys among them."""
+    lens = [700 + 37 * i for i in range(12)]
+    c = Case(lens, [0] * 12, 16, 8)
+    assert c.tiles.shape[0] // 2 * 8 > 148 * 2
+    want = c.run("fp8")
+    keep = torch.ones(c.T, dtype=torch.bool, device=DEV)
+    for r in (1, 4, 11):
+        keep[c.starts[r]:c.starts[r] + 64 * (r + 3)] = False
+    c.pos[~keep] = OUTSIDE
+    for r, n in enumerate(c.ctxs):
+        if n % 16:
+            c.codes()[c.bt[r, n // 16].long(), :, :, n % 16:] = 0x7F
+    out = c.run("fp8")
+    assert (out[~keep] == 0).all() and torch.equal(out[keep], want[keep])
 
 
 def test_one_tile_a_cta():

@@ -1276,11 +1276,10 @@ __global__ void __launch_bounds__(128) decode_split_kernel(const __grid_constant
     l_run = fmaf(l_run, alpha, lsum);
     ok = mbar_wait(&sm.bar[buf][1], par, nullptr) && ok;
     if (nk < SPLIT) {
-      // the last chunk of the sequence: V rows past its last page were not loaded (their weights are zero, but
-      // stale shared memory could hold NaN bit patterns); clear them
-      const int r0 = ((nk + PAGE - 1) / PAGE) * PAGE;
-      for (int i = tid; i < (SPLIT - r0) * 16; i += 128) {
-        const int r = r0 + (i >> 4), c = i & 15;
+      // the last chunk of the sequence: V behind its end has weights of zero, but what its last page holds there, or the
+      // shared memory of pages that were not loaded, may be NaN; clear it
+      for (int i = tid; i < (SPLIT - nk) * 16; i += 128) {
+        const int r = nk + (i >> 4), c = i & 15;
         *reinterpret_cast<uint4*>(sm.v[buf] + (c >> 3) * HALF_BYTES + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
       }
       __syncthreads();

@@ -1,0 +1,30 @@
+"""Decode attention over the bf16 cache: what a page holds behind its sequence's end reaches no row."""
+import pytest
+import torch
+
+from sdcguard_b200.ops import attention
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+
+@pytest.mark.parametrize("nq,nkv", [(2, 2), (4, 2), (8, 2), (8, 1)])
+@pytest.mark.parametrize("batch", [1, 400])                 # a CTA for each segment, or for a whole row
+def test_places_behind_a_sequence_may_hold_anything(nq, nkv, batch):
+    lens = [1, 15, 16, 17, 50, 64, 65, 300] * (batch // 8) if batch > 1 else [300]
+    g = torch.Generator(device=DEV).manual_seed(nq)
+    cache = torch.randn(19 * batch + 1, 2, nkv, 16, 128, device=DEV, generator=g).bfloat16()
+    bt = (1 + torch.arange(19 * batch, dtype=torch.int32, device=DEV)).view(batch, 19)
+    q = torch.randn(batch, nq, 128, device=DEV, generator=g).bfloat16()
+    req = torch.arange(batch, dtype=torch.int32, device=DEV)
+    ctx = torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+    def run():
+        return attention.decode(q, cache, bt, req, ctx, nq, nkv, max_ctx=512)
+
+    want = run()
+    assert torch.isfinite(want).all()
+    for b, n in enumerate(lens):
+        for page in range(n // 16, 19):
+            cache[bt[b, page].long(), :, :, n % 16 if page == n // 16 else 0:] = float("nan")
+    assert torch.equal(run(), want)

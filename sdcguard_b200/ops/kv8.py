@@ -119,6 +119,10 @@ class KV8Cache:
     def shape(self) -> torch.Size:
         return self.codes.shape
 
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.codes.dtype
+
     def values(self, pages: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The stored values in float32 (of one layer; of the given pages): [pages, 2, kv heads, 16, 128]."""
         codes, scales = (self.codes, self.scales) if pages is None else (self.codes[pages], self.scales[pages])

@@ -153,3 +153,10 @@ def test_pages_used_before_do_not_change_a_prefill():
     eng.cache.codes.view(torch.uint8).fill_(0x7F)
     got = eng.score([_prompts()[0, :201].tolist()], topk=5)
     assert all(torch.equal(a, b) for a, b in zip(want[0], got[0]))
+
+
+def test_engine_refuses_an_8_bit_cache_it_was_not_asked_for():
+    from sdcguard_b200.models.decoder import TINY
+    from sdcguard_b200.serve.engine import LLMEngine
+    with pytest.raises(ValueError, match="bf16"):
+        LLMEngine(TINY, device="cuda:0", max_num_seqs=8, cache=KV8Cache.empty(8, 2, 2, DEV))

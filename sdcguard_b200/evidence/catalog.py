@@ -24,7 +24,8 @@ _R = {
     # static deployment contracts (evidence/config.py)
     "capacity.planned": ("config", "The declared KV page pool holds the advertised context for the declared batch "
                                    "and fits the declared device memory."),
-    "capacity.startup": ("config", "The engine's saved startup line reports at least the declared KV pages."),
+    "capacity.startup": ("config", "The engine's saved startup line reports at least the declared KV pages, of the "
+                                   "declared size and type."),
     "protection.gemm_abft": ("config", "Every linear layer runs on the checked GEMM (ABFT in the epilogue)."),
     "protection.replay": ("config", "Norm, attention and elementwise kernels replay a row sample of at most 1/64."),
     "protection.kv_checksum": ("config", "KV pages moved between prefill and decode are hashed on arrival and "

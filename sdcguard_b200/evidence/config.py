@@ -8,12 +8,14 @@ and no device work is done.
 DEPLOYMENT.json ("sdcguard_b200.deployment.v1"):
     {"model": {"name", "layers", "kv_heads", "head_dim"}, "advertised_context_tokens": int,
      "workers": [{"id", "role": "prefill" | "decode" | "both", "version", "build", "gpu_memory_gb",
-                  "kv_pages", "page_tokens", "max_num_seqs", "checked", "sample_every", "kv_checksums",
+                  "kv_pages", "page_tokens", "kv_cache": "bf16" (the default) | "fp8", "max_num_seqs", "checked",
+                  "sample_every", "kv_checksums",
                   "release": "after_consumer_done" | "early", "verify_cached_prefix", "startup_log": path}]}
 
 Each worker gets the capacity and protection rules, the deployment the peer rules (`evidence.catalog` states each).
 A rule is "unknown" whenever its facts are missing or malformed: an absent fact is never read as a good one. The
-startup log is the line `LLMEngine.startup_line()` prints (`sdcguard_b200 engine: kv_pages=... page_tokens=...`);
+startup log is the line `LLMEngine.startup_line()` prints (`sdcguard_b200 engine: kv_pages=... page_tokens=...`, and
+`kv_cache=...` where it is not bf16);
 the declared geometry is the operator's statement, not an attestation of what ran.
 
 Reference: src/sdcguard/config_safety.py:1-20 (`assess`, `render`), config_capacity.py:1-10 (planned and startup
@@ -39,6 +41,7 @@ SCOPE = ("declared configuration and saved startup lines only; a satisfied rule 
          "request isolation, build authenticity or the engines' current state")
 MAX_BYTES = 1 << 20
 MAX_WORKERS = 256
+KV_CACHES = ("bf16", "fp8")       # cache types of the engine; a worker or startup line that names none has the first
 KV_MEMORY_FRACTION = 0.9          # of device memory that the KV pool may take in a plan (weights, activations: rest)
 STARTUP = re.compile(r"sdcguard_b200 engine: (.*)$", re.M)
 
@@ -100,22 +103,24 @@ def _f(rule, verdict, message, basis, facts=None) -> dict:
     return catalog.finding(rule, verdict, message, basis, facts or {})
 
 
-def kv_page_bytes(model: dict, page_tokens: int) -> Optional[int]:
+def kv_page_bytes(model: dict, page_tokens: int, kv_cache="bf16") -> Optional[int]:
+    """Bytes of one page over every layer: K and V, in bf16 or ("fp8") in 8 bits with a float32 scale for each head."""
     vals = [_int(model.get(k)) for k in ("layers", "kv_heads", "head_dim")]
-    if None in vals or not page_tokens:
+    if None in vals or not page_tokens or kv_cache not in KV_CACHES:
         return None
     layers, kvh, hd = vals
-    return layers * 2 * kvh * page_tokens * hd * 2          # K and V, bf16
+    return layers * 2 * kvh * (page_tokens * hd * 2 if kv_cache == "bf16" else page_tokens * hd + 4)
 
 
 def capacity(worker: dict, model: dict, context: Optional[int], startup: dict) -> list[dict]:
     out = []
     pages, pt, seqs = _int(worker.get("kv_pages")), _int(worker.get("page_tokens")), _int(worker.get("max_num_seqs"))
     mem = worker.get("gpu_memory_gb")
-    pb = kv_page_bytes(model, pt or 0)
+    kind = worker.get("kv_cache", "bf16")
+    pb = kv_page_bytes(model, pt or 0, kind)
     if None in (pages, pt, seqs, pb, _int(context)) or not isinstance(mem, (int, float)) or mem <= 0:
-        out.append(_f("capacity.planned", "unknown", "Pages, page size, batch, context, memory or model geometry "
-                      "is missing or malformed.", "missing evidence"))
+        out.append(_f("capacity.planned", "unknown", "Pages, page size, cache type, batch, context, memory or model "
+                      "geometry is missing or malformed.", "missing evidence"))
     else:
         need = seqs * -(-context // pt) + 1                  # page 0 is the engine's reserved zero page
         pool = pages * pb
@@ -137,10 +142,11 @@ def capacity(worker: dict, model: dict, context: Optional[int], startup: dict) -
             out.append(_f("capacity.startup", "unknown", "The startup line has no integer kv_pages/page_tokens.",
                           "malformed startup evidence"))
         else:
-            ok = pages is not None and sp >= pages and spt == pt
+            ok = pages is not None and sp >= pages and spt == pt and got.get("kv_cache", "bf16") == kind
             out.append(_f("capacity.startup", "satisfied" if ok else "violated",
                           "The saved startup line reports the declared pool." if ok else
-                          "The saved startup line reports fewer pages or another page size than declared.",
+                          "The saved startup line reports fewer pages, another page size or another cache type than "
+                          "declared.",
                           "saved startup line", {"startup_kv_pages": sp, "startup_page_tokens": spt,
                                                  "declared_kv_pages": pages, "log_sha256": startup["sha256"]}))
     return out

@@ -152,6 +152,21 @@ class QuantWeights:
              else torch.full_like(q, float(self.center)))
         return ((q - z) * s).to(torch.bfloat16).double()
 
+    def matvec_serves(self) -> bool:
+        """Whether `matvec` multiplies by these weights: INT4 codes in groups of a multiple of 32, tensors as it reads them,
+        scales below 2^27 (read from the device)."""
+        if self.bits != 4 or self.group % 32 or self.k > 1 << 25 or self.n * (self.k // 32) > 0x7fffffff:
+            return False
+        ng, dev = self.k // self.group, self.codes.device
+        try:
+            kv8.want(self.codes, torch.uint8, (self.n, self.k // 2), dev, "codes", align=16)
+            kv8.want(self.scales, torch.bfloat16, (self.n, ng), dev, "scales")
+            if self.zeros is not None:
+                kv8.want(self.zeros, torch.uint8, (self.n, ng), dev, "zeros")
+        except ValueError:
+            return False
+        return bool((self.scales.abs() < 2.0 ** 27).all())
+
     def matvec(self, x: torch.Tensor, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
                blocks: Optional[torch.Tensor] = None, check: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x W^T (+ bias) for up to 32 rows x (m, k) bf16, read from the 4-bit codes (`csrc/matvec4.cu`): W is the
@@ -211,12 +226,14 @@ class CheckedQuantLinear:
 
     With `decode_slot` (a state slot of its own, `state.add(name, 1)`), calls of up to 32 rows read the 4-bit codes
     instead of the effective weights (`QuantWeights.matvec`: a quarter of the bytes, which is what a decode step's time
-    is made of); a rotating 1/64 of their outputs is recomputed and compared bit for bit in that slot."""
+    is made of); a rotating 1/64 of their outputs is recomputed and compared bit for bit in that slot. Weights that `matvec`
+    does not serve (INT8, other groups, scales of 2^27 and more) take the GEMM at every size."""
 
     def __init__(self, qw: QuantWeights, bias: Optional[torch.Tensor] = None):
         self.qw = qw
         self.cw = gemm.CheckedWeight(qw.effective_weight(), bias)
         self.codes_fp = qw.fingerprint()
+        self.reads_codes = qw.matvec_serves()
         # row i: blocks i, i + turns, ... of 16 outputs, the sample of every turns-th call
         blocks = -(-qw.n // 16)
         turns = min(64, blocks)
@@ -236,10 +253,11 @@ class CheckedQuantLinear:
 
     def __call__(self, x: torch.Tensor, state: torch.Tensor, slot: int, decode_slot: Optional[int] = None,
                  **kw) -> torch.Tensor:
-        if decode_slot is None or not 0 < x.shape[0] <= MATVEC_ROWS:
+        if decode_slot is not None and set(kw) - {"out", "row_sq"}:
+            raise ValueError(f"{sorted(set(kw) - {'out', 'row_sq'})}: arguments of the GEMM alone, not of a call with a "
+                             "decode_slot, whatever its size")
+        if decode_slot is None or not self.reads_codes or not 0 < x.shape[0] <= MATVEC_ROWS:
             return gemm.checked_linear(x, self.cw, state, slot, **kw)
-        if set(kw) - {"out", "row_sq"}:
-            raise ValueError(f"{sorted(set(kw) - {'out', 'row_sq'})}: arguments of the GEMM path")
         y = self.qw.matvec(x, self.cw.bias, out=kw.get("out"))
         self._sampled = self._sample()
         self.qw.matvec(x, self.cw.bias, out=y, blocks=self._sampled, check=state[decode_slot])

@@ -194,8 +194,9 @@ class QuantWeights:
             kv8.want(bias, torch.float32, (self.n,), dev, "bias")
         if out is None:
             out = torch.empty(m, self.n, dtype=torch.bfloat16, device=dev)
-        elif out.shape != (m, self.n) or out.dtype != torch.bfloat16 or out.device != dev or out.stride(1) != 1:
-            raise ValueError(f"out must be bf16 ({m}, {self.n}) on {dev} with contiguous rows")
+        elif out.shape != (m, self.n) or out.dtype != torch.bfloat16 or out.device != dev or out.stride(1) != 1 \
+                or (m > 1 and out.stride(0) < self.n):
+            raise ValueError(f"out must be bf16 ({m}, {self.n}) on {dev} with contiguous rows that do not overlap")
         if (blocks is None) != (check is None) or (check is not None and given is None):
             raise ValueError("blocks and check go together, with out, which they compare")
         if blocks is not None:

@@ -207,3 +207,14 @@ def test_want():
                 lambda: kv8.want(t.view(-1)[1:], torch.float32, (31,), cpu, "t", align=16)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_matvec_refuses_an_output_whose_rows_overlap():
+    qw = QuantWeights.quantize(torch.randn(8, 64), bits=4, group=32)
+    x = torch.zeros(3, 64, dtype=torch.bfloat16)
+    buf = torch.zeros(64, dtype=torch.bfloat16)
+    for out in (buf[:8].expand(3, 8), buf.as_strided((3, 8), (7, 1))):
+        with pytest.raises(ValueError, match="rows"):
+            qw.matvec(x, out=out)
+    with pytest.raises(ValueError, match="CUDA"):                # every other call of these arguments ends at the device
+        qw.matvec(x, out=buf.as_strided((3, 8), (8, 1)))

@@ -243,24 +243,25 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) matvec4_kernel(const Params 
 
 template <int NT, int MT, int WARPS, int PF, int CTAS, int MODE, bool PACKED>
 static int launch_mode(const Params& p, int grid, cudaStream_t st) {
-  if (!PACKED) {
+  if constexpr (!PACKED) {
     matvec4_kernel<NT, MT, WARPS, PF, CTAS, MODE, false><<<grid, WARPS * 32, 0, st>>>(p);
     return static_cast<int>(cudaGetLastError());
+  } else {
+    const int nkb = (p.K + KB - 1) / KB;
+    pack_x_kernel<NT><<<(nkb * 4 * NT * 32 + 255) / 256, 256, 0, st>>>(p);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return static_cast<int>(e);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, matvec4_kernel<NT, MT, WARPS, PF, CTAS, MODE, true>, p));
   }
-  const int nkb = (p.K + KB - 1) / KB;
-  pack_x_kernel<NT><<<(nkb * 4 * NT * 32 + 255) / 256, 256, 0, st>>>(p);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return static_cast<int>(e);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(WARPS * 32);
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, matvec4_kernel<NT, MT, WARPS, PF, CTAS, MODE, PACKED>, p));
 }
 template <int NT, int MT, int WARPS, int PF, int CTAS, bool PACKED = false>
 static int launch(const Params& p, int mode, int grid, cudaStream_t st) {

@@ -764,6 +764,7 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 4 : 3) kv8_decode_kernel
     const float v = fits ? 0.f : __int_as_float(0x7fffffff);
     for (int h = 0; h < p.G; ++h)
       for (int i = tid; i < D; i += WARPS * 32) put(p, b, kvh * p.G + h, i, v);
+    if (!fits && p.check == nullptr && p.row_sq != nullptr && tid == 0) atomicAdd(p.row_sq + b, v);
     return;
   }
   const int nseg = (pages + p.seg_pages - 1) / p.seg_pages;

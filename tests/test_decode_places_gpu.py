@@ -28,3 +28,17 @@ def test_places_behind_a_sequence_may_hold_anything(nq, nkv, batch):
         for page in range(n // 16, 19):
             cache[bt[b, page].long(), :, :, n % 16 if page == n // 16 else 0:] = float("nan")
     assert torch.equal(run(), want)
+
+
+def test_rows_that_do_not_fit_have_a_norm_of_nan():
+    """8-bit cache: a row of NaN adds NaN to its sum of squares, whatever made it NaN; a row without keys adds nothing."""
+    from sdcguard_b200.ops.kv8 import KV8Cache
+    cache = KV8Cache.empty(8, 1, device=DEV)
+    q = torch.randn(5, 2, 128, device=DEV).bfloat16()
+    q[4, 1, 0] = float("nan")
+    bt = torch.tensor([[1, 2], [3, 4], [5, 99], [6, 7], [6, 7]], dtype=torch.int32, device=DEV)
+    req = torch.tensor([0, 9, 2, 3, 4], dtype=torch.int32, device=DEV)
+    ctx = torch.tensor([0, 20, 20, 33, 20], dtype=torch.int32, device=DEV)
+    sq = torch.zeros(5, device=DEV)
+    out = attention.decode8(q, cache, bt, req, ctx, attention.decode8_plan(5, 2, 1, 32, DEV), row_sq=sq)
+    assert out.isnan().any(-1).any(-1).tolist() == sq.isnan().tolist() == [False, True, True, True, True] and sq[0] == 0

@@ -224,3 +224,86 @@ def test_one_tile_a_cta():
                         os.path.join(here, "test_kv8_gpu.py") + "::test_prefill_matches_64_bits_and_replays_exactly"],
                        env=env, capture_output=True, text=True, timeout=600, cwd=os.path.dirname(here))
     assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-1000:]
+
+
+@pytest.mark.parametrize("kind", ["fp8", "bf16"])
+@pytest.mark.parametrize("nq,nkv", [(32, 1), (128, 1), (128, 4)])
+def test_many_heads_of_a_kv_head(kind, nq, nkv):
+    """Four tokens a tile and one, in calls of few tokens too: output to bf16 (2^-8), weights to bf16 in the products and the
+    sum (2 x 2^-8), ex2 and sums (2^-17), scores of 128 products in fp32, each rounded or cut (in weight and sum)."""
+    lens, prior = [37, 1, 20], [100, 0, 333]
+    c = Case(lens, prior, nq, nkv, few=True)
+    out = c.run(kind)
+    for r, (n, p0, s) in enumerate(zip(lens, prior, c.starts)):
+        x = c.cache.values(c.bt[r, :-(-c.ctxs[r] // 16)].long()).double().permute(1, 2, 0, 3, 4).flatten(2, 3)
+        late = torch.arange(c.ctxs[r], device=DEV)[None] > torch.arange(p0, p0 + n, device=DEV)[:, None]
+        for h in range(nq):
+            k, v = (t[:c.ctxs[r]] for t in x[:, h // (nq // nkv)])
+            qd = c.q[s:s + n, h].double()
+            w = torch.softmax((qd @ k.t() * 128 ** -0.5).masked_fill(late, -math.inf), -1)
+            ds = float((qd.abs() @ k.abs().t()).max()) * 128 ** -0.5 * 128 * 2.0 ** -23
+            tol = (w @ v).abs() * 2 ** -8 + w @ v.abs() * (2 * 2 ** -8 + 2 ** -17 + 2 * ds)
+            assert ((out[s:s + n, h].double() - w @ v).abs() <= tol).all(), (r, h)
+
+
+@pytest.mark.parametrize("kind", ["fp8", "bf16"])
+def test_rows_that_no_tile_names_stay(kind):
+    c = Case([300, 77], [0, 150], 4, 2)
+    want = c.run(kind)
+    c.q = torch.cat([c.q, torch.full((3, 4, 128), NAN, device=DEV).bfloat16()])
+    c.pos = torch.cat([c.pos, torch.zeros(3, dtype=torch.int32, device=DEV)])
+    sq = torch.zeros(c.T + 3, device=DEV)
+    out = c.run(kind, row_sq=sq)
+    assert torch.equal(out[:c.T], want) and (out[c.T:] == 7).all() and (sq[c.T:] == 0).all()
+
+
+@pytest.mark.parametrize("few", [False, True])
+def test_captured_and_on_two_streams(few):
+    """Two graphs with a plan each, replayed on two streams at once over caches that change between the replays, and eager
+    calls on a side stream: the eager bits."""
+    cases = [Case([40, 33], [0, 7], 4, 2, seed=s, few=True) if few else Case([700, 77], [0, 150], 4, 2, seed=s)
+             for s in (0, 1)]
+    other = [Case(c.lens, c.prior, 4, 2, seed=5 + i, few=few).cache.codes.view(torch.uint8) for i, c in enumerate(cases)]
+    plans, outs = [c.plan() for c in cases], [torch.zeros_like(c.q) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    graphs = []
+    for c, plan, out in zip(cases, plans, outs):
+        c.run("fp8", plan=plan, out=out)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.run("fp8", plan=plan, out=out)
+        graphs.append(g)
+    for turn in range(3):
+        want = [c.run("fp8") for c in cases]
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for out, w in zip(outs, want):
+            assert torch.equal(out, w)
+        got = []
+        for s, c in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(c.run("fp8", plan=plans[0 if c is cases[0] else 1]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        for c, o in zip(cases, other):
+            c.codes().copy_(o if turn == 0 else c.codes().flip(0))
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("few", [False, True])
+def test_scale(few):
+    """A scale of zero weighs all keys alike: the mean of the values that the row sees."""
+    c = Case([40, 33], [0, 7], 4, 2, few=True) if few else Case([300, 77], [0, 150], 4, 2)
+    out = c.run("fp8", scale=0.0).double()
+    for r, (n, p0, s) in enumerate(zip(c.lens, c.prior, c.starts)):
+        v = c.cache.values(c.bt[r, :-(-c.ctxs[r] // 16)].long()).double().permute(1, 2, 0, 3, 4).flatten(2, 3)[1]
+        at = torch.arange(p0, p0 + n, device=DEV)
+        mean, mag = (t.cumsum(1)[:, at] / (at + 1)[:, None] for t in (v, v.abs()))
+        ref = mean.transpose(0, 1).repeat_interleave(2, 1)
+        tol = ref.abs() * 2 ** -8 + mag.transpose(0, 1).repeat_interleave(2, 1) * 2 ** -11
+        assert ((out[s:s + n] - ref).abs() <= tol).all()

@@ -102,6 +102,10 @@ constexpr int SMEM = OFF_CTL + static_cast<int>(sizeof(Ctl)) + 1024;
 constexpr int SOFT = 2 * ROWS;            // softmax threads: warpgroup g takes keys / dims [64 g, 64 g + 64)
 }  // namespace pf
 
+// The reference maximum of a row without a score above -inf so far. Maxima pass over NaN: with -inf in its place scores of
+// NaN would look like masked ones; against this one their weights are NaN, and those of -inf 0.
+constexpr float NO_SCORE = -3.402823466e38f;
+
 // V of a key tile, of which rows [0, n) are keys that some row of the query tiles sees. The weights of the others are zero,
 // but the MMA multiplies V by them, and 0 * NaN is NaN: what a page holds behind its sequence's end is whatever was stored
 // there last, as is shared memory that nothing was loaded to. So only keys are loaded (the last page's one by one, through
@@ -287,7 +291,7 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
       fence_proxy_async_smem();
       mbar_arrive(&ctl->q_ready);
     }
-    float m_use = -INFINITY, l = 0.f;
+    float m_use = NO_SCORE, l = 0.f;
     bool stop = false;
     for (int j = 0; j < ntiles; ++j) {
       const int st = j & 1;
@@ -315,14 +319,12 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
       named_bar_sync(2, SOFT);
       mx = fmaxf(ctl->xm[j & 1][0][r], ctl->xm[j & 1][1][r]);
       float alpha = 1.f;
-      if (mx > -INFINITY && (m_use == -INFINITY || mx > m_use + RESCALE_LOG2)) {
-        alpha = m_use == -INFINITY ? 1.f : ex2(m_use - mx);
+      if (mx > m_use + RESCALE_LOG2) {
+        alpha = m_use == NO_SCORE ? 1.f : ex2(m_use - mx);
         l *= alpha;
         m_use = mx;
       }
-      // pass 2: weights as bf16, their partial row sum. Scores that are all NaN leave the maximum at -inf: 0 stands for it
-      // then, so that they reach the weights
-      const float ref = m_use > -INFINITY ? m_use : 0.f;
+      // pass 2: weights as bf16, their partial row sum
       uint32_t pk[32];
       float ls = 0.f;
 #pragma unroll
@@ -333,8 +335,8 @@ __global__ void __launch_bounds__(128 + 2 * ROWS, 1) prefill_tc_kernel(const __g
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           const int key = kbase + c * 32 + i;
-          const float p0 = key <= pos ? ex2(u32_as_f32(v[i]) * p.scale_log2 - ref) : 0.f;
-          const float p1 = key + 1 <= pos ? ex2(u32_as_f32(v[i + 1]) * p.scale_log2 - ref) : 0.f;
+          const float p0 = key <= pos ? ex2(u32_as_f32(v[i]) * p.scale_log2 - m_use) : 0.f;
+          const float p1 = key + 1 <= pos ? ex2(u32_as_f32(v[i + 1]) * p.scale_log2 - m_use) : 0.f;
           const uint32_t w = pack_bf16x2(p0, p1);
           pk[(c * 32 + i) >> 1] = w;
           const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
@@ -820,8 +822,8 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
       if (__any_sync(0xffffffffu, stop || ctl->begin[x][part ^ 1][r])) break;
       pr = &ctl->pair[n & 1];
       if (!pr->live) break;
-      const int tok = pr->tok[x][r], pos = pr->pos[x][r], my_tiles = pr->nt[x];
-      float m_use = -INFINITY, l = 0.f;   // l: part 1's
+      const int pos = pr->pos[x][r], my_tiles = pr->nt[x];
+      float m_use = NO_SCORE, l = 0.f;    // l: part 1's
       for (int j = 0; j < my_tiles; ++j) {
         if (!mbar_wait(&ctl->s_full[x], turn++ & 1u, abort_flag)) {
           *abort_flag = 1;
@@ -861,8 +863,8 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
         mx = fmaxf(mx, ctl->part_max[x][part ^ 1][r]);
         mx *= p.scale_log2;                // scale > 0: the maximum commutes with it
         float alpha = 1.f;
-        if (mx > -INFINITY && (m_use == -INFINITY || mx > m_use + RESCALE_LOG2)) {
-          alpha = m_use == -INFINITY ? 1.f : ex2(m_use - mx);
+        if (mx > m_use + RESCALE_LOG2) {
+          alpha = m_use == NO_SCORE ? 1.f : ex2(m_use - mx);
           l *= alpha;
           m_use = mx;
         }
@@ -878,23 +880,21 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
             tmem_st16(o_col + part * 64 + c * 16, o);
           }
         }
-        // scores that are all NaN leave the maximum at -inf: 0 stands for it then, so that they reach the weights
-        const float ref = m_use > -INFINITY ? m_use : 0.f;
         uint32_t pk[2][16];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           if (full) {
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              const float2 e = fma2(v[c][i], v[c][i + 1], p.scale_log2, -ref);
+              const float2 e = fma2(v[c][i], v[c][i + 1], p.scale_log2, -m_use);
               pk[c][i >> 1] = pack_bf16x2(ex2(e.x), ex2(e.y));
             }
           } else {
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               const int key = c * 32 + i;
-              const float p0 = key <= lim ? ex2(u32_as_f32(v[c][i]) * p.scale_log2 - ref) : 0.f;
-              const float p1 = key + 1 <= lim ? ex2(u32_as_f32(v[c][i + 1]) * p.scale_log2 - ref) : 0.f;
+              const float p0 = key <= lim ? ex2(u32_as_f32(v[c][i]) * p.scale_log2 - m_use) : 0.f;
+              const float p1 = key + 1 <= lim ? ex2(u32_as_f32(v[c][i + 1]) * p.scale_log2 - m_use) : 0.f;
               pk[c][i >> 1] = pack_bf16x2(p0, p1);
             }
           }
@@ -923,7 +923,7 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
       if (part == 1) ctl->l[x][r] = l;
       pair_sync(x, quarter);
       stop = __any_sync(0xffffffffu, stop || ctl->stop[x][part ^ 1][r]);
-      const int bx = pr->bx, kvh = pr->kvh;
+      const int bx = pr->bx, kvh = pr->kvh, tok = pr->tok[x][r];
       // a row without keys is zeros, whether or not others of its tile have some
       if (!stop && __any_sync(0xffffffffu, tok >= 0)) {
         const int head = kvh * G + (r % G);
@@ -939,8 +939,11 @@ __global__ void __launch_bounds__(pp::THREADS, 1) prefill_pp_kernel(const __grid
           tmem_ld32(o_col + part * 64 + c * 32, v);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            w[c][i] = pos >= 0 ? pack_bf16x2(u32_as_f32(v[2 * i]) * inv, u32_as_f32(v[2 * i + 1]) * inv) : 0u;
+          for (int i = 0; i < 16; ++i) w[c][i] = pack_bf16x2(u32_as_f32(v[2 * i]) * inv, u32_as_f32(v[2 * i + 1]) * inv);
+          if (pos < 0) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[c][i] = 0u;
+          }
           if (p.check == nullptr) {
             if (tok >= 0) {
               store32(orow + part * 64 + c * 32, &w[c][0], wide);

@@ -650,7 +650,9 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const ExpandParams p) {
 //
 // Measured (16 query, 8 kv heads, device time): 256 x 1600 keys 135 us, 6.2 TB/s, 0.95 of a copy's rate: DRAM bounds it.
 // 1 x 131072 keys 53 us, 5.1 TB/s, with the merge of its segments and the start of the CTAs in it; 61 ragged ones up to
-// 4100 keys 59 us, 4.5 TB/s, the longest rows' tail. 1 x 37 keys 3.8 us, latency. Loads into registers instead of the
+// 4100 keys 59 us, 4.5 TB/s, the longest rows' tail. 1 x 37 keys 3.8 us, latency. More than 8 query heads a kv head pay a
+// second set of products for the same bytes, at 3 CTAs an SM: 64 x 2048 keys, 2 kv heads, of 8, 9 and 16 queries each: 29.6,
+// 34.1 and 42.1 us (bytes: 10.4); 256 x 1600, 4 kv heads, of 8 and 16: 74 and 94 us (65). Loads into registers instead of the
 // ring: 162 us for the first; a ring filled by cp.async: 159; two warps a CTA: 131, but 67 and 76 us for the next two.
 constexpr int WARPS = 4;
 constexpr int REC = D + 4;               // floats a record: o[D], M, l, pad

@@ -11,10 +11,12 @@
 // weights) of a row as they lie in memory, pairs (i, i + 4) of each word as masks give them, and reads x in the same
 // order.
 //
-// The bytes that must move are the codes' (N K / 2); what bounds is the instructions per code. Device times: 1 x 4096 x
-// 4096 4.6 us (its bytes alone 1.3), 1 x 28672 x 4096 19.2 us, 13 x 28672 x 4096 with zero points 28 us. A bare read of
-// the last matrix takes 10 us, and this kernel without forming the weights and without reading x and scales 13. Codes
-// through shared memory (TMA or cp.async rings), scales staged there and CTAs that walk over tiles gave the same times.
+// The bytes that must move are the codes' (N K / 2). Device times: 1 x 4096 x 4096 4.6 us (its bytes alone 1.3), launch and
+// one wave of CTAs; 1 x 28672 x 4096 19.2 us, 13 x 28672 x 4096 with zero points 28 us, against 10 of a bare read of the
+// matrix and 13 of this kernel without forming the weights and without reading x and scales. The last runs at 1.75
+// instructions a cycle and waits for loads longest (3.2 warps of 15 at each issue): x comes to each CTA from L2 and the scales
+// two bytes at a time, beside three instructions a pair of weights. Codes through shared memory (TMA or cp.async rings),
+// scales staged there behind a barrier and CTAs that walk over tiles gave the same times.
 //
 // A CTA computes 16 MT outputs. The k blocks (128 each) of an output go to its WARPS warps in turn, whose sums merge in
 // order at the end; WARPS follows from the matrix's shape. Each output's arithmetic depends on its codes and x's row alone

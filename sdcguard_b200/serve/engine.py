@@ -105,7 +105,10 @@ class LLMEngine:
                  max_model_len: int = 4096, precision: str = "bf16", cache: Optional[torch.Tensor] = None,
                  kv_cache: str = "bf16"):
         """kv_cache "fp8": keys and values are kept in 8 bits with a scale for each page and head (`ops.kv8`): twice the
-        tokens in the same memory, half the bytes of a decode step's attention. `cache` is then a kv8.KV8Cache."""
+        tokens in the same memory, half the bytes of a decode step's attention. `cache` is then a kv8.KV8Cache. A row's last
+        bits then depend on the batch around it: on the number of sequences of a decode step, which decides how their keys
+        are cut, and on whether a prefill is one of few tokens (the bf16 cache's attention cuts at fixed keys). Page
+        checksums, transfers between engines and the tensor- and expert-parallel servers take the bf16 cache only."""
         if kv_cache not in ("bf16", "fp8"):
             raise ValueError(f"kv_cache {kv_cache!r}: bf16 or fp8")
         self.cfg = cfg

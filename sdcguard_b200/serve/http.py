@@ -345,7 +345,8 @@ def main(argv=None) -> int:
     ap.add_argument("--unchecked", action="store_true")
     ap.add_argument("--precision", default="bf16", choices=["bf16", "fp8"])
     ap.add_argument("--kv-cache", default="bf16", choices=["bf16", "fp8"],
-                    help="fp8: keys and values in 8 bits, a scale for each page of 16 tokens and head")
+                    help="fp8: keys and values in 8 bits, a scale for each page of 16 tokens and head; a request's last bits "
+                         "then depend on the batch it runs in")
     ap.add_argument("--max-num-seqs", type=int, default=32)
     ap.add_argument("--max-model-len", type=int, default=2048)
     ap.add_argument("--batch-window-ms", type=float, default=5.0)
